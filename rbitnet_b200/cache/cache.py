@@ -40,6 +40,7 @@ class CacheLayerView:
     writes: bool               # False: this run reads what another run wrote
     group: int
     streams: tuple = ()        # every stored tensor of this layer, in the order of the need's streams
+    scales: tuple = ()         # a cache held in 8 bits: per stream, float32 [n_pages, kv heads, blocks of a page]
 
 
 class CacheGroup:

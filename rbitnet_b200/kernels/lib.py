@@ -116,6 +116,10 @@ _SIGNATURES = {
     "rb_qk_prepare": [P, P, I, P, L, P, I, P, P, I, P, P, F, P, F, I, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, L, F, I, P],
     "rb_latent_rotate_append": [P, I, P, L, P, F, P, F, I, P, P, P, P, I, I, I, I, I, I, I, I, P],
     "rb_rotate_rows": [P, L, I, I, I, P, F, I, I, P, I, P],
+    "rb_append8": [P, P, L, P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
+    "rb_cache8_values": [P, P, P, I, P, P, P, P, P, I, I, I, I, P],
+    "rb_attention8_simple": [P, P, P, P, P, P, P, I, I, P, P, I, I, I, I, F, I, P],
+    "rb_verify": [P, P, P, L, P, L, P, P, P, P, I, I, I, I, P, P],
     "rb_set_error_flag_for_test": [I],
     "rb_late_copy_for_test": [P, P, L, L, P],
     "rb_wait_probe": [L, I, P, P],
@@ -124,7 +128,7 @@ _SIGNATURES = {
 
 
 #: source files whose kernels address the cache through the checked function (each has its own word)
-CHECKED_FILES = ("elementwise", "gemm_tcgen05", "attention_simple", "attention_tiled", "latent", "prepare")
+CHECKED_FILES = ("elementwise", "gemm_tcgen05", "attention_simple", "attention_tiled", "latent", "prepare", "cache8", "attention8")
 
 
 class KernelError(RuntimeError):
@@ -173,6 +177,8 @@ class KernelLibrary:
         self.declare("rb_gemm_tc_bias", [P])
         self.declare("rb_gemm_tc_per_head", [I, I, I, P, L, I])
         self.declare("rb_gemm_tc_leave_tanh", [P, L, P, P, F])
+        self.declare("rb_cache8_block", [I])
+        self.declare("rb_verify_scratch_bytes", [I, I], restype=ctypes.c_longlong)
         self.declare("rb_device_sm_count", [])
         self.declare("rb_is_checked_build", [])
         for tu in CHECKED_FILES:

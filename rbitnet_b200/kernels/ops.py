@@ -157,6 +157,15 @@ class NormedRows:
         return self.x.shape
 
 
+@dataclass
+class CacheRanges:
+    """Pages of sequences whose values are read back (``CudaOps.cache_ranges``): ``items`` int32 [count, 3] (slot, page of the
+    sequence, positions in use), ``first_item`` the first page of every range."""
+    items: torch.Tensor
+    count: int
+    first_item: List[int]
+
+
 #: per device: the workspace of the tensor-core products (arrival counters, then partial sums of
 #: tiles whose inner dimension is shared between teams of CTAs).  One per process and device, never
 #: freed: the library keeps its address.
@@ -533,7 +542,10 @@ class CudaOps:
         return out
 
     def rotate_append(self, qkv: torch.Tensor, rotary, meta, view, n_heads: int) -> torch.Tensor:
-        """Rotates q (and k) by position, appends k and v to the cache; returns q [T, H, D]."""
+        """Rotates q (and k) by position, appends k and v to the cache; returns q [T, H, D].  A cache held in 8 bits takes
+        them as codes (csrc/cache8.cu): the scale of a block of positions is that of its largest value so far."""
+        if view.scales:
+            return self._rotate_append8(qkv, rotary, meta, view, n_heads)
         D, Kh = view.head_dim, view.n_kv_heads
         T, width = qkv.shape
         if rotary is None:
@@ -555,6 +567,8 @@ class CudaOps:
         """q/k/v product of the normed rows ``h``, rotation by position and cache append; returns the
         rotated q [T, H, D].  For a few tokens (a decode step) the product's own epilogue rotates and
         appends, from its float32 sums; otherwise the product is stored and ``rotate_append`` follows."""
+        if view.scales:
+            return self.rotate_append(self.linear(h, weight), rotary, meta, view, n_heads)
         pending = h if isinstance(h, NormedRows) else None
         if pending is not None:
             if self._takes_pending(pending, weight.w):
@@ -593,7 +607,10 @@ class CudaOps:
         """Each new token's queries over its sequence's cached keys up to its own position.  ``sinks`` (float32 [H]):
         head h's softmax denominator also holds exp(sinks[h]); ``softcap`` > 0: score <- softcap * tanh(score /
         softcap); ``keep_first`` > 0 with a window: the sequence's first so many positions stay visible wherever the window
-        is.  Every attention kernel of the library takes them all."""
+        is.  Every attention kernel of the library takes them all.  A cache held in 8 bits is read as the values its codes
+        stand for."""
+        if view.scales:
+            return self._attention8(q, meta, view, n_heads, scale, window, sinks, softcap, keep_first)
         T, H, D = q.shape
         Kh = view.n_kv_heads
         out = torch.empty((T, H * D), dtype=self.dtype, device=self.device)
@@ -659,6 +676,107 @@ class CudaOps:
             self.lib.call("rb_attention_simple", _ptr(out), _ptr(q), self.code, _ptr(view.k), _ptr(view.v),
                           _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos),
                           _ptr(meta.tok_slot), T, H, Kh, D, float(scale), win, self._stream())
+        return out
+
+    # ------------------------------------------------------------------ the cache held in 8 bits
+    def _check_cache8(self, view, what: str) -> int:
+        """Refuses what the 8-bit kernels do not take; returns the positions of a block."""
+        if self.dtype != torch.bfloat16:
+            raise KernelError(f"{what}: a cache held in 8 bits goes with the bfloat16 mode, not with {self.dtype}")
+        block = self.lib.raw("rb_cache8_block")(view.page_size)
+        if block <= 0:
+            raise KernelError(f"{what}: a page of {view.page_size} positions must be 64 at most, or a multiple of 64")
+        pool = (view.k.shape[0], view.n_kv_heads, view.page_size, view.head_dim)
+        scales = (view.k.shape[0], view.n_kv_heads, view.page_size // block)
+        for name, t, s in (("keys", view.k, view.scales[0]), ("values", view.v, view.scales[1])):
+            self._check(t, torch.float8_e4m3fn, f"{what}: {name}")
+            self._check(s, torch.float32, f"{what}: the scales of the {name}")
+            if tuple(t.shape) != pool or tuple(s.shape) != scales:
+                raise KernelError(f"{what}: {name} {tuple(t.shape)} with scales {tuple(s.shape)}, expected {pool} and {scales}")
+        self._check(view.page_table, torch.int32, f"{what}: page table")
+        return block
+
+    def _block_tiles(self, meta, block: int):
+        """(first row, rows, count) of the tiles of a step's rows that lie in one block of one sequence, made once per step;
+        nothing for a step of one token per sequence, whose rows are tiles each."""
+        if meta.single_token:
+            return None, None, meta.n_tokens
+        import numpy as np
+        key = ("block_tiles", block)
+        if key not in meta.extra:
+            tok0, ntok = [], []
+            for c in meta.seqs:
+                at = 0
+                while at < c.n_new:
+                    n = min(c.n_new - at, block - (c.start + at) % block)
+                    tok0.append(c.offset + at)
+                    ntok.append(n)
+                    at += n
+            both = upload(np.asarray([tok0, ntok], dtype=np.int32).reshape(2, -1), self.device)
+            meta.extra[key] = (both[0], both[1], len(tok0))
+        return meta.extra[key]
+
+    def _rotate_append8(self, qkv: torch.Tensor, rotary, meta, view, n_heads: int) -> torch.Tensor:
+        D, Kh = view.head_dim, view.n_kv_heads
+        T, width = qkv.shape
+        block = self._check_cache8(view, "rotate_append")
+        want = (n_heads + (2 * Kh if view.writes else 0)) * D
+        if width != want or T != meta.n_tokens:
+            raise KernelError(f"rotate_append: {T} rows of {width} values, expected {meta.n_tokens} of {want}")
+        if qkv.dtype != self.dtype or not qkv.is_cuda or qkv.stride(1) != 1:
+            raise KernelError(f"rotate_append: expected {self.dtype} CUDA rows, found {qkv.dtype} on {qkv.device}")
+        inv_freq, interleaved, rot_dim = (self._zeros_freq(D), False, 0) if rotary is None else rotary
+        tok0, ntok, n_tiles = self._block_tiles(meta, block)
+        q = torch.empty((T, n_heads, D), dtype=self.dtype, device=self.device)
+        self.lib.call("rb_append8", _ptr(q), _ptr(qkv), qkv.stride(0), _ptr(inv_freq), _ptr(meta.tok_pos), _ptr(meta.tok_slot),
+                      _ptr(tok0), _ptr(ntok), n_tiles, _ptr(view.k), _ptr(view.v), _ptr(view.scales[0]), _ptr(view.scales[1]),
+                      _ptr(view.page_table), view.max_pages, view.page_size, n_heads, Kh, D, 1 if view.writes else 0, rot_dim,
+                      1 if interleaved else 0, self._stream())
+        return q
+
+    def cache_ranges(self, view, ranges) -> CacheRanges:
+        """The pages that hold positions first .. end - 1 of each (slot, first, end), for ``cache_values`` (of any layer of
+        the group, until the sequences' pages change)."""
+        import numpy as np
+        page, slots = view.page_size, view.page_table.shape[0]
+        items, first_item = [], []
+        for slot, first, end in ranges:
+            if not 0 <= slot < slots or not 0 <= first < end <= view.max_pages * page:
+                raise KernelError(f"cache_ranges: positions {first} .. {end} of slot {slot} are not in {slots} slots of "
+                                  f"{view.max_pages * page} positions")
+            first_item.append(len(items))
+            items.extend((slot, i, min(page, end - i * page)) for i in range(first // page, -(-end // page)))
+        return CacheRanges(upload(np.asarray(items, dtype=np.int32).reshape(-1, 3), self.device), len(items), first_item)
+
+    def cache_values(self, view, ranges: CacheRanges):
+        """Keys and values of the ranges' pages as bfloat16 [pages, kv heads, page size, head size] each: what the codes of a cache
+        held in 8 bits stand for (exactly), and zeros behind a range's end."""
+        if not view.scales:
+            raise KernelError("cache_values: the cache holds its values in the compute dtype")
+        self._check_cache8(view, "cache_values")
+        shape = (ranges.count, view.n_kv_heads, view.page_size, view.head_dim)
+        k, v = (torch.empty(shape, dtype=torch.bfloat16, device=self.device) for _ in range(2))
+        self.lib.call("rb_cache8_values", _ptr(k), _ptr(v), _ptr(ranges.items), ranges.count, _ptr(view.k), _ptr(view.v),
+                      _ptr(view.scales[0]), _ptr(view.scales[1]), _ptr(view.page_table), view.max_pages, view.page_size, view.n_kv_heads,
+                      view.head_dim, self._stream())
+        return k, v
+
+    def _attention8(self, q, meta, view, n_heads: int, scale: float, window, sinks, softcap: float, keep_first: int):
+        T, H, D = q.shape
+        Kh, win = view.n_kv_heads, int(window or 0)
+        self._check_cache8(view, "attention")
+        self._check(q, self.dtype, "attention queries")
+        if D != view.head_dim or H != n_heads or H % Kh:
+            raise KernelError(f"attention: {H} heads of {D} values on {Kh} kv heads of {view.head_dim}")
+        out = torch.empty((T, H * D), dtype=self.dtype, device=self.device)
+        keep = int(keep_first or 0) if win else 0
+        if sinks is not None or softcap > 0.0 or keep > 0:
+            if sinks is not None:
+                self._check(sinks, torch.float32, "attention sinks")
+            self.lib.call("rb_attention_next", _ptr(sinks), float(softcap), keep, launches=0)
+        self.lib.call("rb_attention8_simple", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v), _ptr(view.scales[0]), _ptr(view.scales[1]),
+                      _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos), _ptr(meta.tok_slot), T, H, Kh, D,
+                      float(scale), win, self._stream())
         return out
 
     def _prefill_tiles(self, meta, tokens_per_tile: int):
@@ -1613,6 +1731,36 @@ class CudaOps:
         self.lib.call("rb_sample", _ptr(out), _ptr(logits), logits.stride(0), R, V, _ptr(temperature),
                       _ptr(uniform), _ptr(stats), self._stream(), launches=2)
         return out
+
+    def verify_drafts(self, logits: torch.Tensor, first_row: torch.Tensor, drafts: torch.Tensor, temperature: torch.Tensor,
+                      uniforms: torch.Tensor, most: int, draft_probs: Optional[torch.Tensor] = None):
+        """Drafted tokens against the target's float32 logits [R, V].  Sequence b has rows first_row[b] .. first_row[b + 1] - 1
+        (int32 [B + 1]; at most ``most`` + 1 each); row r judges ``drafts[r]`` (int32 [R]), a sequence's last row nothing.  A draft d
+        is accepted while uniforms[r, 0] q(d) < p(d), p the softmax of the row over its sequence's ``temperature`` (<= 0: the draft
+        must be the arg-max) and q the row of ``draft_probs`` (float32 [R, V]; None: the drafter was certain).  At the first row that does
+        not accept, or the last one, a token is taken from max(p - q, 0) (the last row: p) with uniforms[r, 1].
+        Returns (accepted int32 [B], tokens int32 [B, most + 1]: the accepted drafts, the token taken, then -1)."""
+        for t, dtype, what in ((logits, torch.float32, "logits"), (draft_probs, torch.float32, "draft probabilities")):
+            if t is not None and (t.dtype != dtype or not t.is_cuda or t.dim() != 2 or t.stride(1) != 1):
+                raise KernelError(f"verify_drafts {what}: expected float32 CUDA rows, found {t.dtype} {tuple(t.shape)} on {t.device}")
+        R, V = logits.shape
+        B = first_row.shape[0] - 1
+        for t, dtype, shape, what in ((first_row, torch.int32, (B + 1,), "first rows"), (drafts, torch.int32, (R,), "drafts"),
+                                      (temperature, torch.float32, (B,), "temperatures"), (uniforms, torch.float32, (R, 2), "uniform numbers")):
+            self._check(t, dtype, f"verify_drafts {what}")
+            if tuple(t.shape) != shape:
+                raise KernelError(f"verify_drafts {what}: expected {shape}, found {tuple(t.shape)}")
+        if draft_probs is not None and tuple(draft_probs.shape) != (R, V):
+            raise KernelError(f"verify_drafts draft probabilities: expected {(R, V)}, found {tuple(draft_probs.shape)}")
+        if B < 0 or most < 0 or V < 1:
+            raise KernelError(f"verify_drafts: {B} sequences of at most {most} drafts, {V} logits a row")
+        accepted = torch.empty((B,), dtype=torch.int32, device=self.device)
+        tokens = torch.empty((B, most + 1), dtype=torch.int32, device=self.device)
+        scratch = torch.empty((max(1, self.lib.raw("rb_verify_scratch_bytes")(R, V)),), dtype=torch.uint8, device=self.device)
+        self.lib.call("rb_verify", _ptr(accepted), _ptr(tokens), _ptr(logits), logits.stride(0), _ptr(draft_probs),
+                      0 if draft_probs is None else draft_probs.stride(0), _ptr(first_row), _ptr(drafts), _ptr(temperature),
+                      _ptr(uniforms), B, R, V, most, _ptr(scratch), self._stream(), launches=2)
+        return accepted, tokens
 
     def decode_advance(self, token_ids: torch.Tensor, tok_pos: torch.Tensor, sampled: torch.Tensor,
                        flag_out: Optional[torch.Tensor] = None, n_live: Optional[torch.Tensor] = None) -> None:
