@@ -119,6 +119,7 @@ _SIGNATURES = {
     "rb_append8": [P, P, L, P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
     "rb_cache8_values": [P, P, P, I, P, P, P, P, P, I, I, I, I, P],
     "rb_attention8_simple": [P, P, P, P, P, P, P, I, I, P, P, I, I, I, I, F, I, P],
+    "rb_attention8_rows": [P, P, P, P, P, P, P, I, I, P, P, P, P, I, I, I, I, I, F, I, I, I, P, P, P],
     "rb_verify": [P, P, P, L, P, L, P, P, P, P, I, I, I, I, P, P],
     "rb_set_error_flag_for_test": [I],
     "rb_late_copy_for_test": [P, P, L, L, P],
@@ -178,6 +179,8 @@ class KernelLibrary:
         self.declare("rb_gemm_tc_per_head", [I, I, I, P, L, I])
         self.declare("rb_gemm_tc_leave_tanh", [P, L, P, P, F])
         self.declare("rb_cache8_block", [I])
+        self.declare("rb_attention8_rows_supports", [I, I, I, I])
+        self.declare("rb_attention8_rows_plan", [I, I, I, I, I, P])
         self.declare("rb_verify_scratch_bytes", [I, I], restype=ctypes.c_longlong)
         self.declare("rb_device_sm_count", [])
         self.declare("rb_is_checked_build", [])

@@ -11,8 +11,9 @@ accumulation stay float32.
 """
 from __future__ import annotations
 
+import ctypes
 from ctypes import c_void_p
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import List, Optional
 
 import torch
@@ -230,6 +231,9 @@ class CudaOps:
         self.place_few_pairs = True
         #: up to 16 tokens' choices are made by the kernel that places their pairs
         self.choose_and_place = True
+        #: rows (tokens of a sequence x query heads of a kv head) up to which attention reads the codes of a cache held in 8 bits
+        #: as they are; with more the codes become bfloat16 pages first
+        self.cache8_rows = 64
         #: so does gated linear attention
         self.gla_in_chunks = True
         #: in bfloat16 mode a state-space mixer takes runs of several tokens in chunks of 64 (else token by token)
@@ -768,16 +772,71 @@ class CudaOps:
         self._check(q, self.dtype, "attention queries")
         if D != view.head_dim or H != n_heads or H % Kh:
             raise KernelError(f"attention: {H} heads of {D} values on {Kh} kv heads of {view.head_dim}")
-        out = torch.empty((T, H * D), dtype=self.dtype, device=self.device)
         keep = int(keep_first or 0) if win else 0
+        G, most_new = H // Kh, 1 if meta.single_token else max((c.n_new for c in meta.seqs), default=1)
+        aligned = not (q.data_ptr() | view.k.data_ptr() | view.v.data_ptr()) % 16
+        in_rows = aligned and self.lib.raw("rb_attention8_rows_supports")(H, Kh, D, view.page_size)
+        if not meta.single_token and not (in_rows and most_new * G <= self.cache8_rows):
+            return self._attention_unpacked(q, meta, view, n_heads, scale, window, sinks, softcap, keep)
+        out = torch.empty((T, H * D), dtype=self.dtype, device=self.device)
+        if T == 0:
+            return out
         if sinks is not None or softcap > 0.0 or keep > 0:
             if sinks is not None:
                 self._check(sinks, torch.float32, "attention sinks")
             self.lib.call("rb_attention_next", _ptr(sinks), float(softcap), keep, launches=0)
-        self.lib.call("rb_attention8_simple", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v), _ptr(view.scales[0]), _ptr(view.scales[1]),
-                      _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos), _ptr(meta.tok_slot), T, H, Kh, D,
-                      float(scale), win, self._stream())
+        if not in_rows:
+            self.lib.call("rb_attention8_simple", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v), _ptr(view.scales[0]),
+                          _ptr(view.scales[1]), _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos),
+                          _ptr(meta.tok_slot), T, H, Kh, D, float(scale), win, self._stream())
+            return out
+        tok0 = ntok = part_o = part_ml = None
+        n_tiles, rows = T, G
+        if not meta.single_token:
+            per_tile = min(most_new, 32 // G)
+            tok0, ntok, n_tiles = self._prefill_tiles(meta, per_tile)
+            rows = per_tile * G
+        # the most keys a row tile can have to visit, in whole tiles
+        context = int(meta.max_context) if not win else min(int(meta.max_context), win + 126 + rows // G + (keep + 63) // 64 * 64)
+        plan = (ctypes.c_longlong * 4)()
+        self.lib.call("rb_attention8_rows_plan", n_tiles, rows, Kh, D, context, plan, launches=0)
+        parts, blocks, n_o, n_ml = plan
+        if parts == 0:
+            part_o = torch.empty((n_o,), dtype=torch.float32, device=self.device)
+            part_ml = torch.empty((n_ml,), dtype=torch.float32, device=self.device)
+        self.lib.call("rb_attention8_rows", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v), _ptr(view.scales[0]), _ptr(view.scales[1]),
+                      _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos), _ptr(meta.tok_slot), _ptr(tok0),
+                      _ptr(ntok), n_tiles, rows, H, Kh, D, float(scale), win, parts, blocks, _ptr(part_o), _ptr(part_ml),
+                      self._stream(), launches=2 if parts == 0 else 1)
         return out
+
+    def _attention_unpacked(self, q, meta, view, n_heads: int, scale: float, window, sinks, softcap: float, keep: int):
+        """Many rows a sequence: the codes that the step sees become bfloat16 pages once, and the attention over those follows
+        (a tile of rows would have to turn every code again: 64 times in a prompt of 2,048 tokens of 32 heads)."""
+        import numpy as np
+        key = ("unpacked", view.page_size, window, keep, view.page_table.data_ptr())
+        if key not in meta.extra:
+            P, ranges = view.page_size, []
+            for c in meta.seqs:
+                first = 0 if not window or keep else max(0, c.start - int(window) + 1)
+                ranges.append((c.slot, first, c.start + c.n_new))
+            plan = self.cache_ranges(view, ranges)
+            width = max(-(-end // P) for _, _, end in ranges)
+            table = np.zeros((len(ranges), width), dtype=np.int32)
+            slots = np.zeros(meta.n_tokens, dtype=np.int32)
+            for i, ((_, first, end), at, c) in enumerate(zip(ranges, plan.first_item, meta.seqs)):
+                table[i, :] = at                       # (places that no row sees: any of the sequence's pages)
+                n = -(-end // P) - first // P
+                table[i, first // P:first // P + n] = np.arange(at, at + n)
+                slots[c.offset:c.offset + c.n_new] = i
+            both = upload(np.concatenate([table.reshape(-1), slots]), self.device)
+            step = replace(meta, tok_slot=both[table.size:], extra={},
+                           seqs=[replace(c, slot=i) for i, c in enumerate(meta.seqs)])
+            meta.extra[key] = (plan, both[:table.size].view(table.shape), step)
+        plan, table, step = meta.extra[key]
+        k, v = self.cache_values(view, plan)
+        pages = replace(view, k=k, v=v, page_table=table, max_pages=table.shape[1], streams=(k, v), scales=())
+        return self.attention(q, step, pages, n_heads, scale, window, sinks, softcap, keep)
 
     def _prefill_tiles(self, meta, tokens_per_tile: int):
         """Tiles of at most ``tokens_per_tile`` consecutive tokens of one sequence (device int32 arrays);
