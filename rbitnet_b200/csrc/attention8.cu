@@ -85,7 +85,8 @@ __global__ void __launch_bounds__(128) attn8_simple_kernel(Params8 p) {
 // ---------------------------------------------------------------- few rows a sequence: a decode step, drafted tokens
 // One block of four warps works for ONE kv head and a tile of at most 8 NT rows, (token, query head) pairs of one sequence
 // whose heads share the kv head, over a range of its keys in tiles of 64 (a page, or an aligned part of one: one scale each
-// of keys and of values).  A warp takes 16 keys of every tile and keeps a softmax of its own; they are joined at the end.
+// of keys and of values).  A warp takes 32 keys of every other tile at a time
+// and keeps a softmax of its own; they are joined at the end.
 //
 // The products are mma.sync m16n8k16 in float16 with the KEYS as the 16 rows of the first, and the head's values as the 16 rows of the
 // second, so that eight query rows fill an instruction:
@@ -107,6 +108,7 @@ __global__ void __launch_bounds__(128) attn8_simple_kernel(Params8 p) {
 namespace rows8 {
 
 constexpr int WARPS = 4, TILE = 64;
+constexpr float LOG2E = 1.4426950408889634f;
 
 struct Params {
   Params8 a;
@@ -144,14 +146,14 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // an 8 x 8 matrix of 16-bit values, a row's pair per lane, turned over its diagonal
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -162,16 +164,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 template <int D, int NT> struct Shape {
+  static constexpr int KG = 2;                            // groups of 16 keys of a tile that a warp takes at a time
   static constexpr int KP = D / 64;                       // 16-byte pieces of a key that a thread takes
   static constexpr int VB = D / 8;                        // bytes of a value that a thread takes
   static constexpr int K_BYTES = 2 * KP * 512, V_BYTES = 4 * VB * 32, S_BYTES = 256;
-  static constexpr int STAGE = K_BYTES + V_BYTES + S_BYTES;       // of a warp
-  static constexpr int NS = 4;
+  static constexpr int STAGE = KG * (K_BYTES + V_BYTES) + S_BYTES;      // of a warp
+  static constexpr int NS = NT == 1 ? 2 : 3;
   static constexpr int ROWS = 8 * NT;
+  static constexpr bool Q_SHARED = NT >= 3;               // the query operands lie in shared memory, not in registers
+  static constexpr int Q_BYTES = Q_SHARED ? (D / 16) * NT * 256 : 0;
   static constexpr int RING = WARPS * NS * STAGE;
   static constexpr int MERGE = WARPS * ROWS * (D + 2) * 4;        // over the ring: [warp][row][D], then maxima and sums
   static constexpr int SHOW = ROWS * (D + 2) * 4;                 // behind it: what the cluster's other blocks read
-  static constexpr int BYTES = RING > MERGE + SHOW ? RING : MERGE + SHOW;
+  static constexpr int OFF_Q = RING > MERGE + SHOW ? RING : MERGE + SHOW;
+  static constexpr int BYTES = OFF_Q + Q_BYTES;
 };
 
 // what a block does for one pair: tiles first .. last - 1 of the visited ones
@@ -198,45 +204,72 @@ __device__ __forceinline__ int visited_tiles(const Params& p, int tile) {
 template <int D, int NT>
 __device__ __forceinline__ void work(const Params& p, const Segment& seg, uint8_t* smem, float*& sO, float*& sM, float*& sL) {
   using S = Shape<D, NT>;
-  constexpr int KP = S::KP, MT = D / 16, ROWS = S::ROWS;
+  constexpr int KG = S::KG, KP = S::KP, MT = D / 16, ROWS = S::ROWS, VW = S::VB / 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const Where w(p, seg.tile);
   const int kvh = seg.kvh, G = p.G, H = p.a.H, n_rows = w.ntok * G;
   const RbKeyTiles tiles(w.key_lo, w.key_hi, p.a.keep, TILE);
-  const uint8_t* K = (const uint8_t*)p.a.cache.k;
-  const uint8_t* V = (const uint8_t*)p.a.cache.v;
+  // the warp's share of a tile, and of the tiles
+  constexpr int SHARES = TILE / (16 * KG), STEP = WARPS / SHARES;
+  const int in_tile = warp % SHARES * (16 * KG), kt0 = seg.first + warp / SHARES;
+  const int per = p.a.cache.page_size / TILE;      // tiles of a page
+  const int64_t tile_bytes = (int64_t)TILE * D, page_stride = (int64_t)p.Kh * per * tile_bytes;
+  const uint8_t* K = (const uint8_t*)p.a.cache.k + kvh * per * tile_bytes + (in_tile + g) * D + 16 * t;
+  const uint8_t* V = (const uint8_t*)p.a.cache.v + kvh * per * tile_bytes + (in_tile + 2 * t) * D + S::VB * g;
+  const int* pages = p.a.cache.page_table + (int64_t)w.slot * p.a.cache.max_pages;
   const uint32_t ring = shared_addr(smem) + warp * S::NS * S::STAGE;
 
-  auto request = [&](int kt, int stage) {
-    const int key0 = tiles.at(kt) * TILE + warp * 16;
-    if (key0 <= w.key_hi) {
-      const int64_t off = rb_page_offset(p.a.cache, w.slot, key0, kvh);
-      const int64_t unit = off / (TILE * D);
-      const uint32_t to = ring + stage * S::STAGE + lane * 16;
+  auto page_of = [&](int kt) -> int {
+    if (kt >= seg.last) return 0;
+    const int tile = tiles.at(kt);
+#ifdef RB_CHECKED
+    return (int)(rb_page_offset(p.a.cache, w.slot, tile * TILE, kvh) / page_stride);
+#endif
+    return pages[per == 1 ? tile : tile / per];
+  };
+  auto request = [&](int kt, int page, int stage) {
+    if (kt < seg.last) {
+      const int tile = tiles.at(kt);
+      if (tile * TILE + in_tile <= w.key_hi) {
+        const int sub = per == 1 ? 0 : tile % per;
+        const int64_t off = page * page_stride + sub * tile_bytes;
+        const uint32_t to = ring + stage * S::STAGE;
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+        for (int u = 0; u < KG; ++u) {
 #pragma unroll
-        for (int j = 0; j < KP; ++j) cp16(to + (r * KP + j) * 512, K + off + (g + 8 * r) * D + 64 * j + 16 * t);
+          for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* src = V + off + (2 * t + (i & 1) + (i >> 1) * 8) * D + S::VB * g;
-        if (S::VB == 16) cp16(to + S::K_BYTES + i * 512, src);
-        else cp8(ring + stage * S::STAGE + S::K_BYTES + i * 256 + lane * 8, src);
+            for (int j = 0; j < KP; ++j)
+              cp16(to + u * S::K_BYTES + (r * KP + j) * 512 + lane * 16, K + off + (16 * u + 8 * r) * D + 64 * j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint8_t* src = V + off + (16 * u + (i & 1) + (i >> 1) * 8) * D;
+            const uint32_t dst = to + KG * S::K_BYTES + u * S::V_BYTES + i * (S::VB * 32) + lane * S::VB;
+            if (S::VB == 16) cp16(dst, src);
+            else cp8(dst, src);
+          }
+        }
+        const int64_t unit = ((int64_t)page * p.Kh + kvh) * per + sub;
+        const uint32_t ts = to + KG * (S::K_BYTES + S::V_BYTES) + lane * 8;
+        cp4(ts, p.a.k_scale + unit);
+        cp4(ts + 4, p.a.v_scale + unit);
       }
-      const uint32_t ts = ring + stage * S::STAGE + S::K_BYTES + S::V_BYTES + lane * 8;
-      cp4(ts, p.a.k_scale + unit);
-      cp4(ts + 4, p.a.v_scale + unit);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  int next_page;
+  {
+    int first[S::NS];
 #pragma unroll
-  for (int i = 0; i < S::NS - 1; ++i) {
-    if (seg.first + i < seg.last) request(seg.first + i, i);
-    else asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int i = 0; i < S::NS; ++i) first[i] = page_of(kt0 + i * STEP);
+#pragma unroll
+    for (int i = 0; i < S::NS - 1; ++i) request(kt0 + i * STEP, first[i], i);
+    next_page = first[S::NS - 1];
   }
 
   // ---- the query rows as B operands: of row g of every eight, values 64 j + 16 t + 4 i + (0, 1) and (2, 3)
-  uint32_t qf[MT][NT][2];
+  uint32_t qf[S::Q_SHARED ? 1 : MT][S::Q_SHARED ? 1 : NT][2];
+  uint2* q_shared = reinterpret_cast<uint2*>(smem + S::OFF_Q) + lane;
   float factor[NT][2];             // of rows 2t, 2t + 1: what a score is multiplied by, in base-2 units
   int pos[NT][2];                  // their positions (-1: no such row)
 #pragma unroll
@@ -266,17 +299,28 @@ __device__ __forceinline__ void work(const Params& p, const Segment& seg, uint8_
 #pragma unroll
     for (int j = 0; j < KP; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float lo = __uint_as_float(raw[j][i] << 16), hi = __uint_as_float(raw[j][i] & 0xffff0000u);
-        qf[4 * j + i / 2][n][i & 1] = pack_half2(lo * up, hi * up);
+      for (int i = 0; i < 4; ++i) {
+        uint32_t two[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t x = raw[j][2 * i + h];
+          two[h] = pack_half2(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xffff0000u) * up);
+        }
+        if (S::Q_SHARED) {
+          if (warp == n % WARPS) q_shared[((4 * j + i) * NT + n) * 32] = make_uint2(two[0], two[1]);
+        } else {
+          qf[4 * j + i][n][0] = two[0];
+          qf[4 * j + i][n][1] = two[1];
+        }
       }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      factor[n][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4) * p.a.scale;
+      factor[n][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4) * p.a.scale * (p.a.softcap > 0.f ? 1.f : LOG2E);
       const int rc = n * 8 + 2 * t + c;
       pos[n][c] = rc < n_rows ? w.pos0 + rc / G : -1;
     }
   }
+  if (S::Q_SHARED) __syncthreads();
 
   float o[NT][MT][4], m[NT][2], l[NT][2], unit = 1.f;
 #pragma unroll
@@ -289,65 +333,106 @@ __device__ __forceinline__ void work(const Params& p, const Segment& seg, uint8_
       l[n][c] = 0.f;
       const int rc = n * 8 + 2 * t + c;
       if (p.a.sinks != nullptr && seg.first == 0 && seg.last > 0 && warp == 0 && rc < n_rows) {     // counted once: by the part with the first tile
-        m[n][c] = p.a.sinks[kvh * G + rc % G] * 1.4426950408889634f;
+        m[n][c] = p.a.sinks[kvh * G + rc % G] * LOG2E;
         l[n][c] = g == 0 ? 1.f : 0.f;
       }
     }
   }
 
   bool begun = false;
-  for (int kt = seg.first; kt < seg.last; ++kt) {
-    const int i = kt - seg.first, stage = i % S::NS;
-    if (kt + S::NS - 1 < seg.last) request(kt + S::NS - 1, (i + S::NS - 1) % S::NS);
-    else asm volatile("cp.async.commit_group;" ::: "memory");
+  int stage = 0;
+  for (int kt = kt0; kt < seg.last; kt += STEP) {
+    {
+      const int ahead = kt + (S::NS - 1) * STEP, into = stage == 0 ? S::NS - 1 : stage - 1;
+      const int after = page_of(ahead + STEP);
+      request(ahead, next_page, into);
+      next_page = after;
+    }
     asm volatile("cp.async.wait_group %0;" ::"n"(S::NS - 1) : "memory");
-    const int key0 = tiles.at(kt) * TILE + warp * 16;
-    if (key0 > w.key_hi) continue;
     const uint8_t* at = smem + (warp * S::NS + stage) * S::STAGE;
-    const float2 scales = *reinterpret_cast<const float2*>(at + S::K_BYTES + S::V_BYTES + lane * 8);
+    stage = stage + 1 == S::NS ? 0 : stage + 1;
+    const int key0 = tiles.at(kt) * TILE + in_tile;
+    if (key0 > w.key_hi) continue;
+    const float2 scales = *reinterpret_cast<const float2*>(at + KG * (S::K_BYTES + S::V_BYTES) + lane * 8);
     // ---- S^T = K Q^T
-    float s[NT][4];
+    float s[KG][NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int u = 0; u < KG; ++u)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = 0.f;
 #pragma unroll
     for (int j = 0; j < KP; ++j) {
-      const uint4 ka = *reinterpret_cast<const uint4*>(at + j * 512 + lane * 16);
-      const uint4 kb = *reinterpret_cast<const uint4*>(at + (KP + j) * 512 + lane * 16);
-      const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+      uint32_t wa[KG][4], wb[KG][4];
+#pragma unroll
+      for (int u = 0; u < KG; ++u) {
+        const uint4 ka = *reinterpret_cast<const uint4*>(at + u * S::K_BYTES + j * 512 + lane * 16);
+        const uint4 kb = *reinterpret_cast<const uint4*>(at + u * S::K_BYTES + (KP + j) * 512 + lane * 16);
+        wa[u][0] = ka.x; wa[u][1] = ka.y; wa[u][2] = ka.z; wa[u][3] = ka.w;
+        wb[u][0] = kb.x; wb[u][1] = kb.y; wb[u][2] = kb.z; wb[u][3] = kb.w;
+      }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const uint32_t a0 = half2_lo(wa[x]), a1 = half2_lo(wb[x]), a2 = half2_hi(wa[x]), a3 = half2_hi(wb[x]);
+        uint32_t q[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[4 * j + x][n][0], qf[4 * j + x][n][1]);
+        for (int n = 0; n < NT; ++n) {
+          if (S::Q_SHARED) {
+            const uint2 two = q_shared[((4 * j + x) * NT + n) * 32];
+            q[n][0] = two.x; q[n][1] = two.y;
+          } else {
+            q[n][0] = qf[4 * j + x][n][0]; q[n][1] = qf[4 * j + x][n][1];
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < KG; ++u) {
+          const uint32_t a0 = half2_lo(wa[u][x]), a1 = half2_lo(wb[u][x]), a2 = half2_hi(wa[u][x]), a3 = half2_hi(wb[u][x]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(s[u][n], a0, a1, a2, a3, q[n][0], q[n][1]);
+        }
       }
     }
-    // ---- scores in base-2 units (rows 2t, 2t + 1; keys g, g + 8); the mask only where a row sees less than all 16 keys
-    const bool whole = key0 + 15 <= w.pos0 && (p.a.window <= 0 || key0 >= w.key_hi - p.a.window + 1);
-    bool moved = false;
+    // ---- scores in base-2 units (rows 2t, 2t + 1; keys g, g + 8 of every 16); the mask only where a row sees less than all
+    const bool whole = key0 + 16 * KG - 1 <= w.pos0 && (p.a.window <= 0 || key0 >= w.key_hi - p.a.window + 1);
     float top[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const float f = factor[n][c] * scales.x;
+        float x = -INFINITY;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float v = s[n][c + 2 * h] * f;
-          if (p.a.softcap > 0.f) v = p.a.softcap * tanhf(v / p.a.softcap);
-          v *= 1.4426950408889634f;
-          if (!whole) {
-            const int key = key0 + g + 8 * h, q = pos[n][c];
-            if (key > q || (p.a.window > 0 && key <= q - p.a.window && key >= p.a.keep)) v = -INFINITY;
+        for (int u = 0; u < KG; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float& v = s[u][n][c + 2 * h];
+            v *= f;
+            x = fmaxf(x, v);
           }
-          s[n][c + 2 * h] = v;
-        }
-        float x = fmaxf(s[n][c], s[n][c + 2]);
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
         top[n][c] = x;
-        moved |= x > m[n][c] + 8.f || (m[n][c] == -INFINITY && x > -INFINITY);
       }
+    if (!whole || p.a.softcap > 0.f) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < KG; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float& v = s[u][n][c + 2 * h];
+              if (p.a.softcap > 0.f) v = p.a.softcap * tanhf(v / p.a.softcap) * LOG2E;
+              const int key = key0 + 16 * u + g + 8 * h, q = pos[n][c];
+              if (key > q || (p.a.window > 0 && key <= q - p.a.window && key >= p.a.keep)) v = -INFINITY;
+              x = fmaxf(x, v);
+            }
+          top[n][c] = x;
+        }
+    }
+    bool moved = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) moved |= top[n][c] > m[n][c] + 8.f || (m[n][c] == -INFINITY && top[n][c] > -INFINITY);
     float ratio = scales.y / unit;
     const bool other_unit = !begun || ratio > 16.f || ratio < 0.015625f;
     begun = true;
@@ -364,10 +449,14 @@ __device__ __forceinline__ void work(const Params& p, const Segment& seg, uint8_
         float corr[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+          float x = top[n][c];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
           corr[c] = 1.f;
-          if (top[n][c] > m[n][c] + 8.f || (m[n][c] == -INFINITY && top[n][c] > -INFINITY)) {
-            corr[c] = m[n][c] == -INFINITY ? 0.f : exp2f(m[n][c] - top[n][c]);
-            m[n][c] = top[n][c];
+          if (x > m[n][c] + 8.f || (m[n][c] == -INFINITY && x > -INFINITY)) {
+            corr[c] = m[n][c] == -INFINITY ? 0.f : exp2f(m[n][c] - x);
+            m[n][c] = x;
           }
           l[n][c] *= corr[c];
           corr[c] *= to;
@@ -380,46 +469,56 @@ __device__ __forceinline__ void work(const Params& p, const Segment& seg, uint8_
       }
     }
     // ---- P, its sums, and P^T as the B operand
-    uint32_t pf[NT][2];
+    uint32_t pf[KG][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
-      const float p0 = exp2_fast(s[n][0] - m0), p1 = exp2_fast(s[n][1] - m1), p2 = exp2_fast(s[n][2] - m0), p3 = exp2_fast(s[n][3] - m1);
-      l[n][0] += p0 + p2;
-      l[n][1] += p1 + p3;
-      pf[n][0] = transposed(pack_half2(p0 * ratio, p1 * ratio));
-      pf[n][1] = transposed(pack_half2(p2 * ratio, p3 * ratio));
+#pragma unroll
+      for (int u = 0; u < KG; ++u) {
+        const float p0 = exp2_fast(s[u][n][0] - m0), p1 = exp2_fast(s[u][n][1] - m1);
+        const float p2 = exp2_fast(s[u][n][2] - m0), p3 = exp2_fast(s[u][n][3] - m1);
+        l[n][0] += p0 + p2;
+        l[n][1] += p1 + p3;
+        pf[u][n][0] = transposed(pack_half2(p0 * ratio, p1 * ratio));
+        pf[u][n][1] = transposed(pack_half2(p2 * ratio, p3 * ratio));
+      }
     }
     // ---- O^T += V^T P^T: of keys 2t, 2t + 1, 2t + 8, 2t + 9 the bytes 2u (row g) and 2u + 1 (row g + 8)
-    uint32_t v[4][S::VB / 4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (S::VB == 16) {
-        const uint4 x = *reinterpret_cast<const uint4*>(at + S::K_BYTES + k * 512 + lane * 16);
-        v[k][0] = x.x; v[k][1] = x.y;
-        if (S::VB == 16) { v[k][S::VB / 4 - 2] = x.z; v[k][S::VB / 4 - 1] = x.w; }
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(at + S::K_BYTES + k * 256 + lane * 8);
-        v[k][0] = x.x; v[k][1] = x.y;
-      }
-      if (!whole) {                // a key that no row sees may hold anything: NaN times a weight of zero would stay
-        const int key = key0 + 2 * t + (k & 1) + (k >> 1) * 8;
-        if (key > w.key_hi || (key < w.key_lo && key >= p.a.keep)) {
+    for (int u = 0; u < KG; ++u) {
+      uint32_t v[4][VW];
 #pragma unroll
-          for (int x = 0; x < S::VB / 4; ++x) v[k][x] = 0u;
+      for (int k = 0; k < 4; ++k) {
+        const uint8_t* src = at + KG * S::K_BYTES + u * S::V_BYTES + k * (S::VB * 32) + lane * S::VB;
+        if constexpr (VW == 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(src);
+          v[k][0] = x.x; v[k][1] = x.y; v[k][2] = x.z; v[k][3] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(src);
+          v[k][0] = x.x; v[k][1] = x.y;
         }
       }
-    }
+      if (!whole) {                // a key that no row sees may hold anything: NaN times a weight of zero would stay
 #pragma unroll
-    for (int x = 0; x < S::VB / 4; ++x)
+        for (int k = 0; k < 4; ++k) {
+          const int key = key0 + 16 * u + 2 * t + (k & 1) + (k >> 1) * 8;
+          if (key > w.key_hi || (key < w.key_lo && key >= p.a.keep)) {
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const uint32_t ab = __byte_perm(v[0][x], v[1][x], y == 0 ? 0x5140 : 0x7362);
-        const uint32_t cd = __byte_perm(v[2][x], v[3][x], y == 0 ? 0x5140 : 0x7362);
-        const uint32_t a0 = half2_lo(ab), a1 = half2_hi(ab), a2 = half2_lo(cd), a3 = half2_hi(cd);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * x + y], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+            for (int x = 0; x < VW; ++x) v[k][x] = 0u;
+          }
+        }
       }
+#pragma unroll
+      for (int x = 0; x < VW; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint32_t ab = __byte_perm(v[0][x], v[1][x], y == 0 ? 0x5140 : 0x7362);
+          const uint32_t cd = __byte_perm(v[2][x], v[3][x], y == 0 ? 0x5140 : 0x7362);
+          const uint32_t a0 = half2_lo(ab), a1 = half2_hi(ab), a2 = half2_lo(cd), a3 = half2_hi(cd);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * x + y], a0, a1, a2, a3, pf[u][n][0], pf[u][n][1]);
+        }
+    }
   }
 
   // ---- the four warps, over the ring, which nothing more is copied to

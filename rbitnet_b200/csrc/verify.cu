@@ -81,7 +81,8 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p) {
   __shared__ double s_total, s_before;
   __shared__ float s_max;
   __shared__ int s_row, s_arg, s_owner, s_count, s_last;
-  const int b = blockIdx.x, r0 = p.first_row[b], r1 = p.first_row[b + 1];
+  // (rows outside the logits, which only a wrong first_row can name, are left out)
+  const int b = blockIdx.x, r0 = min(max(p.first_row[b], 0), p.R), r1 = min(p.first_row[b + 1], p.R);
   const float temp = p.temperature[b];
   const double inv_t = 1.0 / (double)temp;
   int* tokens = p.tokens + (int64_t)b * (p.most + 1);
