@@ -2,33 +2,15 @@
 // kv head.  Token t at position p of its sequence sees keys max(0, p - window + 1) .. p (and with keep_first the first keys);
 // score = (q.k) * scale, in float32, capped where a soft cap is set; softmax with the running maximum and sum in float32 (the
 // sink one more term of the sum); o = sum of p v.  A key that a row does not see is not multiplied by anything.
-#include "rb_common.cuh"
+#include "attention8.cuh"
 
 #include <cuda_fp8.h>
 
 RB_CHECK_READER(attention8)
 
-RB_EXPORT int rb_cache8_block(int page_size);
-
 namespace {
 
 __device__ __forceinline__ float of_code(uint8_t c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
-
-struct Params8 {
-  const __nv_bfloat16* q;     // [T, H, D]
-  __nv_bfloat16* out;         // [T, H * D]
-  RbPagedLayer cache;
-  const float* k_scale;       // [page][kv head][blocks of a page]
-  const float* v_scale;
-  int block;
-  const int* tok_pos;
-  const int* tok_slot;
-  int H;
-  float scale;
-  int window, keep;
-  const float* sinks;
-  float softcap;
-};
 
 // Any sizes: one block of threads per (token, head); a thread takes a key of every 128 for the scores, then every 128th value.
 __global__ void __launch_bounds__(128) attn8_simple_kernel(Params8 p) {
@@ -82,766 +64,6 @@ __global__ void __launch_bounds__(128) attn8_simple_kernel(Params8 p) {
 }
 
 
-// ---------------------------------------------------------------- few rows a sequence: a decode step, drafted tokens
-// One block of four warps works for ONE kv head and a tile of at most 8 NT rows, (token, query head) pairs of one sequence
-// whose heads share the kv head, over a range of its keys in tiles of 64 (a page, or an aligned part of one: one scale each
-// of keys and of values).  A warp takes 32 keys of every other tile at a time
-// and keeps a softmax of its own; they are joined at the end.
-//
-// The products are mma.sync m16n8k16 in float16 with the KEYS as the 16 rows of the first, and the head's values as the 16 rows of the
-// second, so that eight query rows fill an instruction:
-//     S^T[16 keys, 8 rows] = K[16, D] Q^T           O^T[D, 8 rows] += V^T[D, 16 keys] P^T[16 keys, 8 rows]
-// A code is a float16 value (cvt, exactly), so neither product rounds its operands but P, to float16 (2^-11; P is 256 at most and sums
-// are float32); Q, bfloat16, is brought to the middle of float16's range by a power of two a row.  The order of a product's inner index
-// and of its rows is free as long as both sides agree, and it is chosen so that every operand register is made of whole
-// 16-byte pieces of the cache as they lie: of keys g and g + 8 the pieces 16 t .. 16 t + 15 of every 64 values, of values
-// the pieces D/8 g .. of keys 2t, 2t + 1, 2t + 8, 2t + 9 (lane = 4 g + t).  So a thread only ever reads what it has copied itself: the ring in
-// shared memory is private to the thread (cp.async, no barriers, no bank conflicts), and its depth hides the latency.
-//
-// O is kept in units of a values' scale `unit`, which follows the tiles' scales lazily: P is multiplied by scale / unit, and O
-// is brought to another unit (exactly: powers of two) only where that ratio leaves 2^-6 .. 2^4.  Likewise the exponents' reference
-// moves only when a maximum has grown by more than 8.
-//
-// Ranges of keys: in a small grid the parts of a (tile, kv head) are a thread-block cluster and merge on chip.  In a larger one
-// all tiles of keys of all (row tile, kv head) pairs, in order, are dealt out evenly to the blocks, whatever the sequences' lengths; a
-// pair that several blocks have worked on is merged by a second kernel.
-namespace rows8 {
-
-constexpr int WARPS = 4, TILE = 64;
-constexpr float LOG2E = 1.4426950408889634f;
-
-struct Params {
-  Params8 a;
-  const int* tile_tok0;       // null: row tile i is row i alone
-  const int* tile_ntok;
-  int n_tiles, Kh, G;
-  int parts;                  // > 0: the parts of a pair are a cluster; 0: the tiles are dealt out to gridDim.x blocks
-  int least;                  // dealt out: tiles of a block, at least
-  float* part_o;              // dealt out: [blocks + pairs][8 NT][D], and
-  float* part_ml;             // [blocks + pairs][8 NT][2] (maximum in base-2 units, sum)
-};
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-// two codes (the low 16 bits, or the high ones) as two float16 values
-__device__ __forceinline__ uint32_t half2_lo(uint32_t w) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(r) : "r"(w));
-  return r;
-}
-__device__ __forceinline__ uint32_t half2_hi(uint32_t w) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(r) : "r"(w));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// an 8 x 8 matrix of 16-bit values, a row's pair per lane, turned over its diagonal
-__device__ __forceinline__ uint32_t transposed(uint32_t v) {
-  uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-template <int D, int NT> struct Shape {
-  static constexpr int KG = 2;                            // groups of 16 keys of a tile that a warp takes at a time
-  static constexpr int KP = D / 64;                       // 16-byte pieces of a key that a thread takes
-  static constexpr int VB = D / 8;                        // bytes of a value that a thread takes
-  static constexpr int K_BYTES = 2 * KP * 512, V_BYTES = 4 * VB * 32, S_BYTES = 256;
-  static constexpr int STAGE = KG * (K_BYTES + V_BYTES) + S_BYTES;      // of a warp
-  static constexpr int NS = NT == 1 ? 2 : 3;
-  static constexpr int ROWS = 8 * NT;
-  static constexpr bool Q_SHARED = NT >= 3;               // the query operands lie in shared memory, not in registers
-  static constexpr int Q_BYTES = Q_SHARED ? (D / 16) * NT * 256 : 0;
-  static constexpr int RING = WARPS * NS * STAGE;
-  static constexpr int MERGE = WARPS * ROWS * (D + 2) * 4;        // over the ring: [warp][row][D], then maxima and sums
-  static constexpr int SHOW = ROWS * (D + 2) * 4;                 // behind it: what the cluster's other blocks read
-  static constexpr int OFF_Q = RING > MERGE + SHOW ? RING : MERGE + SHOW;
-  static constexpr int BYTES = OFF_Q + Q_BYTES;
-};
-
-// what a block does for one pair: tiles first .. last - 1 of the visited ones
-struct Segment { int tile, kvh, first, last, visited; };
-
-// the row tile's sequence: where its rows and its keys are
-struct Where {
-  int tok0, ntok, slot, pos0, key_lo, key_hi;
-  __device__ __forceinline__ Where(const Params& p, int tile) {
-    tok0 = p.tile_tok0 ? p.tile_tok0[tile] : tile;
-    ntok = p.tile_ntok ? p.tile_ntok[tile] : 1;
-    slot = p.a.tok_slot[tok0];
-    pos0 = p.a.tok_pos[tok0];
-    key_hi = pos0 + ntok - 1;
-    key_lo = p.a.window > 0 ? max(0, pos0 - p.a.window + 1) : 0;
-  }
-};
-__device__ __forceinline__ int visited_tiles(const Params& p, int tile) {
-  const Where w(p, tile);
-  return RbKeyTiles(w.key_lo, w.key_hi, p.a.keep, TILE).n;
-}
-
-// The block's part of a pair: the four warps' sums joined in `smem` (unnormalised [row][D], maxima, sums).
-template <int D, int NT>
-__device__ __forceinline__ void work(const Params& p, const Segment& seg, uint8_t* smem, float*& sO, float*& sM, float*& sL) {
-  using S = Shape<D, NT>;
-  constexpr int KG = S::KG, KP = S::KP, MT = D / 16, ROWS = S::ROWS, VW = S::VB / 4;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const Where w(p, seg.tile);
-  const int kvh = seg.kvh, G = p.G, H = p.a.H, n_rows = w.ntok * G;
-  const RbKeyTiles tiles(w.key_lo, w.key_hi, p.a.keep, TILE);
-  // the warp's share of a tile, and of the tiles
-  constexpr int SHARES = TILE / (16 * KG), STEP = WARPS / SHARES;
-  const int in_tile = warp % SHARES * (16 * KG), kt0 = seg.first + warp / SHARES;
-  const int per = p.a.cache.page_size / TILE;      // tiles of a page
-  const int64_t tile_bytes = (int64_t)TILE * D, page_stride = (int64_t)p.Kh * per * tile_bytes;
-  const uint8_t* K = (const uint8_t*)p.a.cache.k + kvh * per * tile_bytes + (in_tile + g) * D + 16 * t;
-  const uint8_t* V = (const uint8_t*)p.a.cache.v + kvh * per * tile_bytes + (in_tile + 2 * t) * D + S::VB * g;
-  const int* pages = p.a.cache.page_table + (int64_t)w.slot * p.a.cache.max_pages;
-  const uint32_t ring = shared_addr(smem) + warp * S::NS * S::STAGE;
-
-  auto page_of = [&](int kt) -> int {
-    if (kt >= seg.last) return 0;
-    const int tile = tiles.at(kt);
-#ifdef RB_CHECKED
-    return (int)(rb_page_offset(p.a.cache, w.slot, tile * TILE, kvh) / page_stride);
-#endif
-    return pages[per == 1 ? tile : tile / per];
-  };
-  auto request = [&](int kt, int page, int stage) {
-    if (kt < seg.last) {
-      const int tile = tiles.at(kt);
-      if (tile * TILE + in_tile <= w.key_hi) {
-        const int sub = per == 1 ? 0 : tile % per;
-        const int64_t off = page * page_stride + sub * tile_bytes;
-        const uint32_t to = ring + stage * S::STAGE;
-#pragma unroll
-        for (int u = 0; u < KG; ++u) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int j = 0; j < KP; ++j)
-              cp16(to + u * S::K_BYTES + (r * KP + j) * 512 + lane * 16, K + off + (16 * u + 8 * r) * D + 64 * j);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint8_t* src = V + off + (16 * u + (i & 1) + (i >> 1) * 8) * D;
-            const uint32_t dst = to + KG * S::K_BYTES + u * S::V_BYTES + i * (S::VB * 32) + lane * S::VB;
-            if (S::VB == 16) cp16(dst, src);
-            else cp8(dst, src);
-          }
-        }
-        const int64_t unit = ((int64_t)page * p.Kh + kvh) * per + sub;
-        const uint32_t ts = to + KG * (S::K_BYTES + S::V_BYTES) + lane * 8;
-        cp4(ts, p.a.k_scale + unit);
-        cp4(ts + 4, p.a.v_scale + unit);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  int next_page;
-  {
-    int first[S::NS];
-#pragma unroll
-    for (int i = 0; i < S::NS; ++i) first[i] = page_of(kt0 + i * STEP);
-#pragma unroll
-    for (int i = 0; i < S::NS - 1; ++i) request(kt0 + i * STEP, first[i], i);
-    next_page = first[S::NS - 1];
-  }
-
-  // ---- the query rows as B operands: of row g of every eight, values 64 j + 16 t + 4 i + (0, 1) and (2, 3)
-  uint32_t qf[S::Q_SHARED ? 1 : MT][S::Q_SHARED ? 1 : NT][2];
-  uint2* q_shared = reinterpret_cast<uint2*>(smem + S::OFF_Q) + lane;
-  float factor[NT][2];             // of rows 2t, 2t + 1: what a score is multiplied by, in base-2 units
-  int pos[NT][2];                  // their positions (-1: no such row)
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r = n * 8 + g;
-    const bool in = r < n_rows;
-    uint32_t raw[KP][8];
-    const __nv_bfloat16* src = p.a.q + ((int64_t)(w.tok0 + (in ? r / G : 0)) * H + kvh * G + (in ? r % G : 0)) * D;
-    uint32_t big = 0;              // the largest exponent (and mantissa) among the row's values
-#pragma unroll
-    for (int j = 0; j < KP; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 v = in ? *reinterpret_cast<const uint4*>(src + 64 * j + 16 * t + 8 * h) : make_uint4(0, 0, 0, 0);
-        raw[j][4 * h] = v.x; raw[j][4 * h + 1] = v.y; raw[j][4 * h + 2] = v.z; raw[j][4 * h + 3] = v.w;
-      }
-#pragma unroll
-    for (int j = 0; j < KP; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) big = max(big, max(raw[j][i] << 16 & 0x7fff0000u, raw[j][i] & 0x7fff0000u));
-    big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-    big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    // the row's largest value becomes 2^8 .. 2^9; rows of zeros, infinities or NaN as they are
-    const int e = max((int)(big >> 23) - 127 - 8, -100);
-    const bool plain = big == 0 || big >= 0x7f800000u;
-    const float up = plain ? 1.f : __uint_as_float((uint32_t)(127 - e) << 23), down = plain ? 1.f : __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-    for (int j = 0; j < KP; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t two[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t x = raw[j][2 * i + h];
-          two[h] = pack_half2(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xffff0000u) * up);
-        }
-        if (S::Q_SHARED) {
-          if (warp == n % WARPS) q_shared[((4 * j + i) * NT + n) * 32] = make_uint2(two[0], two[1]);
-        } else {
-          qf[4 * j + i][n][0] = two[0];
-          qf[4 * j + i][n][1] = two[1];
-        }
-      }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      factor[n][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4) * p.a.scale * (p.a.softcap > 0.f ? 1.f : LOG2E);
-      const int rc = n * 8 + 2 * t + c;
-      pos[n][c] = rc < n_rows ? w.pos0 + rc / G : -1;
-    }
-  }
-  if (S::Q_SHARED) __syncthreads();
-
-  float o[NT][MT][4], m[NT][2], l[NT][2], unit = 1.f;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      m[n][c] = -INFINITY;
-      l[n][c] = 0.f;
-      const int rc = n * 8 + 2 * t + c;
-      if (p.a.sinks != nullptr && seg.first == 0 && seg.last > 0 && warp == 0 && rc < n_rows) {     // counted once: by the part with the first tile
-        m[n][c] = p.a.sinks[kvh * G + rc % G] * LOG2E;
-        l[n][c] = g == 0 ? 1.f : 0.f;
-      }
-    }
-  }
-
-  bool begun = false;
-  int stage = 0;
-  for (int kt = kt0; kt < seg.last; kt += STEP) {
-    {
-      const int ahead = kt + (S::NS - 1) * STEP, into = stage == 0 ? S::NS - 1 : stage - 1;
-      const int after = page_of(ahead + STEP);
-      request(ahead, next_page, into);
-      next_page = after;
-    }
-    asm volatile("cp.async.wait_group %0;" ::"n"(S::NS - 1) : "memory");
-    const uint8_t* at = smem + (warp * S::NS + stage) * S::STAGE;
-    stage = stage + 1 == S::NS ? 0 : stage + 1;
-    const int key0 = tiles.at(kt) * TILE + in_tile;
-    if (key0 > w.key_hi) continue;
-    const float2 scales = *reinterpret_cast<const float2*>(at + KG * (S::K_BYTES + S::V_BYTES) + lane * 8);
-    // ---- S^T = K Q^T
-    float s[KG][NT][4];
-#pragma unroll
-    for (int u = 0; u < KG; ++u)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = 0.f;
-#pragma unroll
-    for (int j = 0; j < KP; ++j) {
-      uint32_t wa[KG][4], wb[KG][4];
-#pragma unroll
-      for (int u = 0; u < KG; ++u) {
-        const uint4 ka = *reinterpret_cast<const uint4*>(at + u * S::K_BYTES + j * 512 + lane * 16);
-        const uint4 kb = *reinterpret_cast<const uint4*>(at + u * S::K_BYTES + (KP + j) * 512 + lane * 16);
-        wa[u][0] = ka.x; wa[u][1] = ka.y; wa[u][2] = ka.z; wa[u][3] = ka.w;
-        wb[u][0] = kb.x; wb[u][1] = kb.y; wb[u][2] = kb.z; wb[u][3] = kb.w;
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        uint32_t q[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (S::Q_SHARED) {
-            const uint2 two = q_shared[((4 * j + x) * NT + n) * 32];
-            q[n][0] = two.x; q[n][1] = two.y;
-          } else {
-            q[n][0] = qf[4 * j + x][n][0]; q[n][1] = qf[4 * j + x][n][1];
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < KG; ++u) {
-          const uint32_t a0 = half2_lo(wa[u][x]), a1 = half2_lo(wb[u][x]), a2 = half2_hi(wa[u][x]), a3 = half2_hi(wb[u][x]);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(s[u][n], a0, a1, a2, a3, q[n][0], q[n][1]);
-        }
-      }
-    }
-    // ---- scores in base-2 units (rows 2t, 2t + 1; keys g, g + 8 of every 16); the mask only where a row sees less than all
-    const bool whole = key0 + 16 * KG - 1 <= w.pos0 && (p.a.window <= 0 || key0 >= w.key_hi - p.a.window + 1);
-    float top[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float f = factor[n][c] * scales.x;
-        float x = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < KG; ++u)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float& v = s[u][n][c + 2 * h];
-            v *= f;
-            x = fmaxf(x, v);
-          }
-        top[n][c] = x;
-      }
-    if (!whole || p.a.softcap > 0.f) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float x = -INFINITY;
-#pragma unroll
-          for (int u = 0; u < KG; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float& v = s[u][n][c + 2 * h];
-              if (p.a.softcap > 0.f) v = p.a.softcap * tanhf(v / p.a.softcap) * LOG2E;
-              const int key = key0 + 16 * u + g + 8 * h, q = pos[n][c];
-              if (key > q || (p.a.window > 0 && key <= q - p.a.window && key >= p.a.keep)) v = -INFINITY;
-              x = fmaxf(x, v);
-            }
-          top[n][c] = x;
-        }
-    }
-    bool moved = false;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) moved |= top[n][c] > m[n][c] + 8.f || (m[n][c] == -INFINITY && top[n][c] > -INFINITY);
-    float ratio = scales.y / unit;
-    const bool other_unit = !begun || ratio > 16.f || ratio < 0.015625f;
-    begun = true;
-    if (__any_sync(0xffffffffu, moved) || other_unit) {
-      float to = 1.f;
-      if (other_unit) {
-        const float next = fmaxf(scales.y, unit * 0x1p-90f);      // (O stays finite)
-        to = unit / next;
-        unit = next;
-        ratio = scales.y / unit;
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float corr[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float x = top[n][c];
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          corr[c] = 1.f;
-          if (x > m[n][c] + 8.f || (m[n][c] == -INFINITY && x > -INFINITY)) {
-            corr[c] = m[n][c] == -INFINITY ? 0.f : exp2f(m[n][c] - x);
-            m[n][c] = x;
-          }
-          l[n][c] *= corr[c];
-          corr[c] *= to;
-        }
-#pragma unroll
-        for (int u = 0; u < MT; ++u) {
-          o[n][u][0] *= corr[0]; o[n][u][2] *= corr[0];
-          o[n][u][1] *= corr[1]; o[n][u][3] *= corr[1];
-        }
-      }
-    }
-    // ---- P, its sums, and P^T as the B operand
-    uint32_t pf[KG][NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
-#pragma unroll
-      for (int u = 0; u < KG; ++u) {
-        const float p0 = exp2_fast(s[u][n][0] - m0), p1 = exp2_fast(s[u][n][1] - m1);
-        const float p2 = exp2_fast(s[u][n][2] - m0), p3 = exp2_fast(s[u][n][3] - m1);
-        l[n][0] += p0 + p2;
-        l[n][1] += p1 + p3;
-        pf[u][n][0] = transposed(pack_half2(p0 * ratio, p1 * ratio));
-        pf[u][n][1] = transposed(pack_half2(p2 * ratio, p3 * ratio));
-      }
-    }
-    // ---- O^T += V^T P^T: of keys 2t, 2t + 1, 2t + 8, 2t + 9 the bytes 2u (row g) and 2u + 1 (row g + 8)
-#pragma unroll
-    for (int u = 0; u < KG; ++u) {
-      uint32_t v[4][VW];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint8_t* src = at + KG * S::K_BYTES + u * S::V_BYTES + k * (S::VB * 32) + lane * S::VB;
-        if constexpr (VW == 4) {
-          const uint4 x = *reinterpret_cast<const uint4*>(src);
-          v[k][0] = x.x; v[k][1] = x.y; v[k][2] = x.z; v[k][3] = x.w;
-        } else {
-          const uint2 x = *reinterpret_cast<const uint2*>(src);
-          v[k][0] = x.x; v[k][1] = x.y;
-        }
-      }
-      if (!whole) {                // a key that no row sees may hold anything: NaN times a weight of zero would stay
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int key = key0 + 16 * u + 2 * t + (k & 1) + (k >> 1) * 8;
-          if (key > w.key_hi || (key < w.key_lo && key >= p.a.keep)) {
-#pragma unroll
-            for (int x = 0; x < VW; ++x) v[k][x] = 0u;
-          }
-        }
-      }
-#pragma unroll
-      for (int x = 0; x < VW; ++x)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const uint32_t ab = __byte_perm(v[0][x], v[1][x], y == 0 ? 0x5140 : 0x7362);
-          const uint32_t cd = __byte_perm(v[2][x], v[3][x], y == 0 ? 0x5140 : 0x7362);
-          const uint32_t a0 = half2_lo(ab), a1 = half2_hi(ab), a2 = half2_lo(cd), a3 = half2_hi(cd);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * x + y], a0, a1, a2, a3, pf[u][n][0], pf[u][n][1]);
-        }
-    }
-  }
-
-  // ---- the four warps, over the ring, which nothing more is copied to
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
-  float* mO = reinterpret_cast<float*>(smem);
-  float* mM = mO + WARPS * ROWS * D;
-  float* mL = mM + WARPS * ROWS;
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float sum = l[n][c];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-      const int row = warp * ROWS + n * 8 + 2 * t + c;
-      if (g == 0) { mM[row] = m[n][c]; mL[row] = sum; }
-#pragma unroll
-      for (int u = 0; u < MT; ++u)
-        *reinterpret_cast<float2*>(mO + row * D + MT * g * 2 + 2 * u) = make_float2(o[n][u][c] * unit, o[n][u][c + 2] * unit);
-    }
-  __syncthreads();
-  sO = reinterpret_cast<float*>(smem + S::MERGE);
-  sM = sO + ROWS * D;
-  sL = sM + ROWS;
-  for (int idx = threadIdx.x; idx < n_rows * D; idx += WARPS * 32) {
-    const int r = idx / D, d = idx % D;
-    float top = -INFINITY;
-#pragma unroll
-    for (int x = 0; x < WARPS; ++x) top = fmaxf(top, mM[x * ROWS + r]);
-    const float use = top == -INFINITY ? 0.f : top;
-    float acc = 0.f, sum = 0.f;
-#pragma unroll
-    for (int x = 0; x < WARPS; ++x) {
-      const float f = exp2f(mM[x * ROWS + r] - use);
-      acc += mO[(x * ROWS + r) * D + d] * f;
-      sum += mL[x * ROWS + r] * f;
-    }
-    sO[idx] = acc;
-    if (d == 0) { sM[r] = top; sL[r] = sum; }
-  }
-  __syncthreads();
-}
-
-template <int D>
-__device__ __forceinline__ void store(const Params& p, const Where& w, int kvh, int r, int d, float o, float l) {
-  p.a.out[((int64_t)(w.tok0 + r / p.G) * p.a.H + kvh * p.G + r % p.G) * D + d] = __float2bfloat16_rn(o / l);
-}
-
-template <int D, int NT>
-__global__ void __launch_bounds__(WARPS * 32) cluster_kernel(Params p) {
-  rb_pdl_launch_dependents();
-  using S = Shape<D, NT>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  Segment seg;
-  seg.tile = blockIdx.x; seg.kvh = blockIdx.y;
-  seg.visited = visited_tiles(p, seg.tile);
-  seg.first = (int)((int64_t)blockIdx.z * seg.visited / p.parts);
-  seg.last = (int)((int64_t)(blockIdx.z + 1) * seg.visited / p.parts);
-  rb_pdl_wait();
-  float *sO, *sM, *sL;
-  work<D, NT>(p, seg, smem, sO, sM, sL);
-  const Where w(p, seg.tile);
-  const int n = w.ntok * p.G * D;
-  if (p.parts == 1) {
-    for (int idx = threadIdx.x; idx < n; idx += WARPS * 32) store<D>(p, w, seg.kvh, idx / D, idx % D, sO[idx], sL[idx / D]);
-    return;
-  }
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  for (int idx = (int)blockIdx.z * WARPS * 32 + threadIdx.x; idx < n; idx += p.parts * WARPS * 32) {
-    const int r = idx / D;
-    float m[16], l[16], o[16];
-#pragma unroll
-    for (int z = 0; z < 16; ++z) {                 // everything is asked for first
-      m[z] = -INFINITY; l[z] = 0.f; o[z] = 0.f;
-      if (z < p.parts) {
-        uint32_t am, al, ao;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(am) : "r"(shared_addr(sM + r)), "r"((uint32_t)z));
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(al) : "r"(shared_addr(sL + r)), "r"((uint32_t)z));
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ao) : "r"(shared_addr(sO + idx)), "r"((uint32_t)z));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(m[z]) : "r"(am));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(l[z]) : "r"(al));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o[z]) : "r"(ao));
-      }
-    }
-    float top = -INFINITY;
-#pragma unroll
-    for (int z = 0; z < 16; ++z) top = fmaxf(top, m[z]);
-    const float use = top == -INFINITY ? 0.f : top;
-    float acc = 0.f, sum = 0.f;
-#pragma unroll
-    for (int z = 0; z < 16; ++z) {
-      const float f = exp2f(m[z] - use);
-      sum += l[z] * f;
-      acc += o[z] * f;
-    }
-    store<D>(p, w, seg.kvh, r, idx % D, acc, sum);
-  }
-  // nobody's shared memory goes away while another part reads it
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// Dealt out: all pairs' tiles of keys in the order (row tile, kv head, tile); a block takes `share` of them, one after the other.
-// What a block leaves for a pair that it shares goes to place block + pair of the scratch: no two blocks' places are the same,
-// and those of one pair follow one another.
-__device__ __forceinline__ int64_t share_of(const Params& p, int64_t total, int blocks) {
-  const int64_t even = (total + blocks - 1) / blocks;
-  return even > p.least ? even : p.least;
-}
-// tiles of keys of the row tiles before `tile`, times the kv heads (and with tile = n_tiles: of all): the whole block, summed in shared memory
-__device__ __forceinline__ int block_count(int v, int* s) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = (blockDim.x + 31) >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if (lane == 0) s[warp] = v;
-  __syncthreads();
-  int sum = 0;
-  for (int x = 0; x < n; ++x) sum += s[x];
-  return sum;
-}
-
-template <int D, int NT>
-__global__ void __launch_bounds__(WARPS * 32) dealt_kernel(Params p) {
-  rb_pdl_launch_dependents();
-  using S = Shape<D, NT>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int counts[WARPS], s_tile, s_before;
-  // positions, slots and page tables were written before the step began: the deal needs no wait
-  int mine = 0;
-  for (int i = threadIdx.x; i < p.n_tiles; i += WARPS * 32) mine += visited_tiles(p, i);
-  const int64_t total = (int64_t)block_count(mine, counts) * p.Kh;
-  const int64_t share = share_of(p, total, gridDim.x);
-  int64_t x = (int64_t)blockIdx.x * share;
-  const int64_t end = x + share < total ? x + share : total;
-  rb_pdl_wait();
-  if (x >= end) return;
-  // the row tile that tile x of all belongs to: the first warp walks over them, 32 at a time
-  if (threadIdx.x < 32) {
-    int before = 0;
-    for (int i0 = 0; i0 < p.n_tiles; i0 += 32) {
-      const int i = i0 + (int)threadIdx.x;
-      const int n = i < p.n_tiles ? visited_tiles(p, i) : 0;
-      int upto = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, upto, o);
-        if ((int)threadIdx.x >= o) upto += y;
-      }
-      const bool here = n > 0 && (int64_t)(before + upto) * p.Kh > x;
-      const uint32_t who = __ballot_sync(0xffffffffu, here);
-      if (who != 0) {
-        if ((int)threadIdx.x == __ffs(who) - 1) { s_tile = i; s_before = before + upto - n; }
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-  }
-  __syncthreads();
-  int tile = s_tile;
-  int64_t base = (int64_t)s_before * p.Kh;         // the first tile of the row tile's pairs
-  while (x < end) {
-    Segment seg;
-    seg.visited = visited_tiles(p, tile);
-    if (x >= base + (int64_t)seg.visited * p.Kh) { base += (int64_t)seg.visited * p.Kh; ++tile; continue; }
-    seg.tile = tile;
-    seg.kvh = (int)((x - base) / seg.visited);
-    const int64_t pair0 = base + (int64_t)seg.kvh * seg.visited;
-    seg.first = (int)(x - pair0);
-    seg.last = (int)(end - pair0 < seg.visited ? end - pair0 : seg.visited);
-    float *sO, *sM, *sL;
-    work<D, NT>(p, seg, smem, sO, sM, sL);
-    const Where w(p, tile);
-    const int n_rows = w.ntok * p.G, n = n_rows * D;
-    if (seg.first == 0 && seg.last == seg.visited) {
-      for (int idx = threadIdx.x; idx < n; idx += WARPS * 32) store<D>(p, w, seg.kvh, idx / D, idx % D, sO[idx], sL[idx / D]);
-    } else {
-      const int64_t place = blockIdx.x + (int64_t)tile * p.Kh + seg.kvh;
-      for (int idx = threadIdx.x; idx < n; idx += WARPS * 32) p.part_o[place * S::ROWS * D + idx] = sO[idx];
-      for (int r = threadIdx.x; r < n_rows; r += WARPS * 32) {
-        p.part_ml[(place * S::ROWS + r) * 2] = sM[r];
-        p.part_ml[(place * S::ROWS + r) * 2 + 1] = sL[r];
-      }
-    }
-    __syncthreads();                               // the shared sums have been read
-    x = pair0 + seg.last;
-  }
-}
-
-// Pairs that several blocks have worked on, one block of threads each: every warp takes every eighth part, joined in shared memory.
-template <int D, int NT>
-__global__ void __launch_bounds__(256) join_kernel(Params p, int blocks) {
-  rb_pdl_launch_dependents();
-  constexpr int ROWS = 8 * NT;
-  extern __shared__ __align__(16) float joined[];  // [ROWS] maxima, [ROWS] sums
-  __shared__ int counts[8];
-  const int tile = blockIdx.x, kvh = blockIdx.y;
-  int mine = 0, ahead = 0;
-  for (int i = threadIdx.x; i < p.n_tiles; i += 256) {
-    const int n = visited_tiles(p, i);
-    mine += n;
-    if (i < tile) ahead += n;
-  }
-  const int64_t total = (int64_t)block_count(mine, counts) * p.Kh;
-  const int64_t base = (int64_t)block_count(ahead, counts) * p.Kh;
-  const int visited = visited_tiles(p, tile);
-  const int64_t share = share_of(p, total, blocks), pair0 = base + (int64_t)kvh * visited;
-  const int first = (int)(pair0 / share), last = (int)((pair0 + visited - 1) / share);
-  rb_pdl_wait();
-  if (first == last) return;
-  const Where w(p, tile);
-  const int n_rows = w.ntok * p.G;
-  const int64_t place0 = first + (int64_t)tile * p.Kh + kvh;
-  const int parts = last - first + 1;
-  const float* ml = p.part_ml + place0 * ROWS * 2;
-  // every row's maximum over the parts, and the sum that belongs to it
-  for (int r = threadIdx.x >> 5; r < n_rows; r += 8) {
-    const int lane = threadIdx.x & 31;
-    float top = -INFINITY, sum = 0.f;
-    for (int z = lane; z < parts; z += 32) top = fmaxf(top, ml[((int64_t)z * ROWS + r) * 2]);
-    top = rb_warp_max(top);
-    const float use = top == -INFINITY ? 0.f : top;
-    for (int z = lane; z < parts; z += 32) sum += ml[((int64_t)z * ROWS + r) * 2 + 1] * exp2f(ml[((int64_t)z * ROWS + r) * 2] - use);
-    sum = rb_warp_sum(sum);
-    if (lane == 0) { joined[r] = use; joined[ROWS + r] = sum; }
-  }
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < n_rows * D; idx += 256) {
-    const int r = idx / D;
-    const float* o = p.part_o + place0 * ROWS * D + idx;
-    float acc = 0.f;
-#pragma unroll 8
-    for (int z = 0; z < parts; ++z) acc += o[(int64_t)z * ROWS * D] * exp2f(ml[((int64_t)z * ROWS + r) * 2] - joined[r]);
-    store<D>(p, w, kvh, r, idx % D, acc, joined[ROWS + r]);
-  }
-}
-
-// blocks of the kernel that an SM holds: by registers at the kernel's bound and by shared memory
-template <int D, int NT> int per_sm() {
-  static int n[RB_MAX_DEVICES] = {0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= RB_MAX_DEVICES) dev = 0;
-  if (n[dev] == 0) {
-    int v = 0;
-    if (cudaFuncSetAttribute(dealt_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D, NT>::BYTES) != cudaSuccess ||
-        cudaFuncSetAttribute(cluster_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D, NT>::BYTES) != cudaSuccess ||
-        cudaFuncSetAttribute(cluster_kernel<D, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, dealt_kernel<D, NT>, WARPS * 32, Shape<D, NT>::BYTES) != cudaSuccess || v < 1)
-      v = 1;
-    (void)cudaGetLastError();
-    n[dev] = v;
-  }
-  return n[dev];
-}
-// the most parts that a cluster may have: 16 where the device runs such clusters of this kernel, else 8 (asked once)
-template <int D, int NT> int cluster_most() {
-  static int answer = 0;
-  if (answer == 0) {
-    per_sm<D, NT>();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1, 1, 16);
-    cfg.blockDim = dim3(WARPS * 32, 1, 1);
-    cfg.dynamicSmemBytes = Shape<D, NT>::BYTES;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 16;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    answer = cudaOccupancyMaxActiveClusters(&n, cluster_kernel<D, NT>, &cfg) == cudaSuccess && n >= 1 ? 16 : 8;
-    (void)cudaGetLastError();
-  }
-  return answer;
-}
-inline int most_parts(int D, int NT) {
-  return D == 64 ? (NT == 1 ? cluster_most<64, 1>() : NT == 2 ? cluster_most<64, 2>() : NT == 3 ? cluster_most<64, 3>() : cluster_most<64, 4>())
-                 : (NT == 1 ? cluster_most<128, 1>() : NT == 2 ? cluster_most<128, 2>() : NT == 3 ? cluster_most<128, 3>() : cluster_most<128, 4>());
-}
-inline int places(int D, int NT) {
-  const int n = D == 64 ? (NT == 1 ? per_sm<64, 1>() : NT == 2 ? per_sm<64, 2>() : NT == 3 ? per_sm<64, 3>() : per_sm<64, 4>())
-                        : (NT == 1 ? per_sm<128, 1>() : NT == 2 ? per_sm<128, 2>() : NT == 3 ? per_sm<128, 3>() : per_sm<128, 4>());
-  return n * rb_sm_count();
-}
-
-template <int D, int NT>
-int launch(const Params& p, int blocks, cudaStream_t stream) {
-  using S = Shape<D, NT>;
-  per_sm<D, NT>();                                 // (sets the kernels' attributes)
-  if (p.parts == 0) {
-    RB_LAUNCH("rb_attention8_rows", (dealt_kernel<D, NT>), blocks, WARPS * 32, S::BYTES, stream, p);
-    RB_LAUNCH("rb_attention8_rows (join)", (join_kernel<D, NT>), dim3(p.n_tiles, p.Kh), 256, S::ROWS * 8, stream, p, blocks);
-    return 0;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.n_tiles, p.Kh, p.parts);
-  cfg.blockDim = dim3(WARPS * 32, 1, 1);
-  cfg.dynamicSmemBytes = S::BYTES;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = p.parts;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = rb_pdl_enabled() ? 2 : 1;
-  RB_CUDA(cudaLaunchKernelEx(&cfg, cluster_kernel<D, NT>, p));
-  return 0;
-}
-template <int D>
-int launch_rows(const Params& p, int NT, int blocks, cudaStream_t stream) {
-  return NT == 1 ? launch<D, 1>(p, blocks, stream) : NT == 2 ? launch<D, 2>(p, blocks, stream)
-       : NT == 3 ? launch<D, 3>(p, blocks, stream) : launch<D, 4>(p, blocks, stream);
-}
-
-}  // namespace rows8
-
 }  // namespace
 
 // out[T, H * D]: attention of q[T, H, D] over the codes; rows of any steps (a row's own position and slot say what it sees).
@@ -861,54 +83,4 @@ RB_EXPORT int rb_attention8_simple(void* out, const void* q, void* cache_k, void
   p.scale = scale; p.window = window; p.keep = opt.keep_first; p.sinks = opt.sinks; p.softcap = opt.softcap;
   RB_LAUNCH("rb_attention8_simple", (attn8_simple_kernel), dim3(T, H), 128, (size_t)2 * D * 4, stream, p);
   return 0;
-}
-
-// Whether the kernel of few rows takes these sizes (a token's heads of one kv head fit its rows, a tile of keys one page).
-RB_EXPORT int rb_attention8_rows_supports(int H, int Kh, int D, int page_size) {
-  if (Kh <= 0 || Kh > 65535 || H % Kh) return 0;
-  return (D == 64 || D == 128) && page_size % rows8::TILE == 0 && H / Kh <= 32;
-}
-
-// How a launch of `n_tiles` row tiles of at most `rows` rows is cut, the longest sequence `context` positions: out4 = parts of a pair that
-// are a cluster (0: dealt out), blocks when dealt out, floats of part_o, floats of part_ml.
-// A cluster where two parts of every pair and more fit the SMs at once and no part is long; else all tiles are dealt out to as many
-// blocks as the SMs hold at once, four tiles to a block at least.
-RB_EXPORT int rb_attention8_rows_plan(int n_tiles, int rows, int Kh, int D, int context, long long* out4) {
-  const int NT = (rows + 7) / 8, places = rows8::places(D, NT), most = rows8::most_parts(D, NT);
-  const int tiles = (context + rows8::TILE - 1) / rows8::TILE;
-  const long long pairs = (long long)n_tiles * Kh;
-  int parts = 1;
-  while (parts * 2 <= tiles && parts < most && pairs * parts * 2 <= places) parts *= 2;
-  out4[0] = parts; out4[1] = out4[2] = out4[3] = 0;
-  if (tiles <= 1 || (parts > 1 && tiles <= 16 * parts)) return 0;
-  long long blocks = (pairs * tiles + 3) / 4;
-  if (blocks > places) blocks = places;
-  out4[0] = 0;
-  out4[1] = blocks;
-  out4[2] = (blocks + pairs) * 8 * NT * D;
-  out4[3] = (blocks + pairs) * 8 * NT * 2;
-  return 0;
-}
-
-// Few rows a sequence: row tile i is the tile_ntok[i] tokens from tile_tok0[i] on, of one sequence (null: row i alone), at most `rows` rows
-// of H / Kh heads each; cut as rb_attention8_rows_plan says, with its scratch.
-RB_EXPORT int rb_attention8_rows(void* out, const void* q, void* cache_k, void* cache_v, const float* k_scale, const float* v_scale,
-                                 const int* page_table, int max_pages, int page_size, const int* tok_pos, const int* tok_slot,
-                                 const int* tile_tok0, const int* tile_ntok, int n_tiles, int rows, int H, int Kh, int D, float scale,
-                                 int window, int parts, int blocks, float* part_o, float* part_ml, cudaStream_t stream) {
-  const RbAttentionOptions opt = rb_attention_take();
-  if (n_tiles == 0) return 0;
-  RB_REQUIRE(rb_attention8_rows_supports(H, Kh, D, page_size) && rows >= H / Kh && rows <= 32,
-             "rb_attention8_rows: sizes H=%d Kh=%d D=%d page=%d, %d rows not supported", H, Kh, D, page_size, rows);
-  RB_REQUIRE(parts >= 0 && parts <= rows8::most_parts(D, (rows + 7) / 8) && (parts > 0 || (blocks > 0 && part_o && part_ml)), "rb_attention8_rows: %d parts, %d blocks", parts, blocks);
-  rows8::Params p;
-  p.a.q = (const __nv_bfloat16*)q; p.a.out = (__nv_bfloat16*)out;
-  p.a.cache = RbPagedLayer{cache_k, cache_v, page_table, max_pages, page_size, Kh, D};
-  p.a.k_scale = k_scale; p.a.v_scale = v_scale; p.a.block = rows8::TILE;
-  p.a.tok_pos = tok_pos; p.a.tok_slot = tok_slot; p.a.H = H;
-  p.a.scale = scale; p.a.window = window; p.a.keep = window > 0 ? opt.keep_first : 0; p.a.sinks = opt.sinks; p.a.softcap = opt.softcap;
-  p.tile_tok0 = tile_tok0; p.tile_ntok = tile_ntok; p.n_tiles = n_tiles; p.Kh = Kh; p.G = H / Kh;
-  p.parts = parts; p.least = 4; p.part_o = part_o; p.part_ml = part_ml;
-  const int NT = (rows + 7) / 8;
-  return D == 64 ? rows8::launch_rows<64>(p, NT, blocks, stream) : rows8::launch_rows<128>(p, NT, blocks, stream);
 }

@@ -578,6 +578,7 @@ int launch_tc(const CUtensorMap& tk, const CUtensorMap& tv, const TcAttnParams& 
 }  // namespace
 
 #include "attention_decode_tma.cuh"
+#include "attention8_rows.cuh"
 
 int rb_attention_combine(void* out, const float* part_o, const float* part_ml, int B, int H, int D, int n_splits,
                          cudaStream_t stream);   // attention_tiled.cu

@@ -119,7 +119,7 @@ _SIGNATURES = {
     "rb_append8": [P, P, L, P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
     "rb_cache8_values": [P, P, P, I, P, P, P, P, P, I, I, I, I, P],
     "rb_attention8_simple": [P, P, P, P, P, P, P, I, I, P, P, I, I, I, I, F, I, P],
-    "rb_attention8_rows": [P, P, P, P, P, P, P, I, I, P, P, P, P, I, I, I, I, I, F, I, I, I, P, P, P],
+    "rb_attention8_rows": [P, P, P, P, P, P, L, P, I, I, P, P, P, P, I, I, I, I, I, F, I, I, I, P, P, P],
     "rb_verify": [P, P, P, L, P, L, P, P, P, P, I, I, I, I, P, P],
     "rb_set_error_flag_for_test": [I],
     "rb_late_copy_for_test": [P, P, L, L, P],
@@ -129,7 +129,7 @@ _SIGNATURES = {
 
 
 #: source files whose kernels address the cache through the checked function (each has its own word)
-CHECKED_FILES = ("elementwise", "gemm_tcgen05", "attention_simple", "attention_tiled", "latent", "prepare", "cache8", "attention8")
+CHECKED_FILES = ("elementwise", "gemm_tcgen05", "attention_simple", "attention_tiled", "latent", "prepare", "cache8", "attention8", "attention8_rows")
 
 
 class KernelError(RuntimeError):

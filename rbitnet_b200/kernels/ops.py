@@ -805,7 +805,7 @@ class CudaOps:
             part_o = torch.empty((n_o,), dtype=torch.float32, device=self.device)
             part_ml = torch.empty((n_ml,), dtype=torch.float32, device=self.device)
         self.lib.call("rb_attention8_rows", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v), _ptr(view.scales[0]), _ptr(view.scales[1]),
-                      _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos), _ptr(meta.tok_slot), _ptr(tok0),
+                      view.k.shape[0], _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos), _ptr(meta.tok_slot), _ptr(tok0),
                       _ptr(ntok), n_tiles, rows, H, Kh, D, float(scale), win, parts, blocks, _ptr(part_o), _ptr(part_ml),
                       self._stream(), launches=2 if parts == 0 else 1)
         return out
