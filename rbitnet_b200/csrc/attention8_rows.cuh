@@ -43,8 +43,8 @@ struct Params {
   int n_tiles, Kh, G;
   int parts;                  // > 0: the parts of a pair are a cluster; 0: the tiles are dealt out to gridDim.x blocks
   int least;                  // dealt out: tiles of a block, at least
-  float* part_o;              // dealt out: [blocks + pairs][8 NT][D], and
-  float* part_ml;             // [blocks + pairs][8 NT][2] (maximum in base-2 units, sum)
+  float4* part_o;             // dealt out: [blocks + pairs][NT][D / 16][lane], what the accumulators of a lane hold, and
+  float2* part_ml;            // [blocks + pairs][8 NT] (maximum in base-2 units, sum)
 };
 
 // two codes (the low 16 bits, or the high ones) as two float16 values
@@ -82,16 +82,28 @@ template <int D, int NT> struct Shape {
   static constexpr int KG = 2;                            // groups of 16 keys of a tile that a warp takes at a time
   static constexpr int CHUNK = KG * 16 * D;               // bytes of their codes, of keys and of values each
   static constexpr int STAGE = 2 * CHUNK;                 // of a warp
-  static constexpr int NS = NT == 1 ? 2 : 3;
+  static constexpr int NS = 3;
   static constexpr int ROWS = 8 * NT;
   static constexpr bool Q_SHARED = NT >= 3;               // the query operands lie in shared memory, not in registers
   static constexpr int Q_BYTES = Q_SHARED ? (D / 16) * NT * 256 : 0;
+  static constexpr int MT = D / 16;                       // accumulators' row tiles
+  static constexpr int QT = MT / WARPS;                   // of them that a warp joins and hands on
   static constexpr int RING = WARPS * NS * STAGE;
-  static constexpr int MERGE = WARPS * ROWS * (D + 2) * 4;        // over the ring: [warp][row][D], then maxima and sums
-  static constexpr int SHOW = ROWS * (D + 2) * 4;                 // behind it: what the cluster's other blocks read
-  static constexpr int OFF_Q = RING > MERGE + SHOW ? RING : MERGE + SHOW;
-  static constexpr int OFF_BAR = OFF_Q + Q_BYTES;
-  static constexpr int BYTES = OFF_BAR + WARPS * NS * 8 + 1024;   // + room to align
+  static constexpr int OFF_Q = RING;
+  static constexpr int OFF_ML = OFF_Q + Q_BYTES;                        // [warp][row] maximum and sum; then of the block, [row]
+  static constexpr int OFF_AT = OFF_ML + (WARPS + 1) * ROWS * 8;        // [warp] the stage that its accumulators begin in
+  static constexpr int OFF_BAR = OFF_AT + 16;
+  static constexpr int BYTES = OFF_BAR + WARPS * NS * 8 + 1024;         // + room to align
+  static constexpr int LEFT = STAGE / (MT * 512);         // eights of rows whose accumulators a stage holds
+  static constexpr int AHEAD = NS - (NT + LEFT - 1) / LEFT;             // stages of the next pair filled while a pair's warps are joined
+  static_assert(AHEAD >= 1, "a warp leaves its accumulators in its own ring");
+  static_assert(NT * MT * 512 <= RING, "what the cluster's other blocks read, over the ring");
+};
+
+// The block's sums of a pair: of every eight rows, row tiles WARP * QT .. of O^T as this lane's accumulators (rows 2t, 2t + 1), maxima and sums.
+template <int D, int NT> struct Joined {
+  float4 o[NT][Shape<D, NT>::QT];
+  float m[NT][2], l[NT][2];
 };
 
 // A warp's ring between two pairs: copies asked for and copies used, whose numbers say the stage and its barrier's phase.
@@ -128,59 +140,74 @@ __device__ __forceinline__ int visited_tiles(const Params& p, int tile) {
   return RbKeyTiles(w.key_lo, w.key_hi, p.a.keep, TILE).n;
 }
 
-// The block's part of a pair: the four warps' sums joined in `smem` (unnormalised [row][D], maxima, sums).
-template <int D, int NT>
-__device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV, const Segment& seg, uint8_t* smem,
-                                     Ring& ring, float*& sO, float*& sM, float*& sL) {
+// A warp's way through a segment: where the sequence lies, the tiles that it asks for next and their pages, scales of the tiles on their way.
+// The positions, slots and page tables were written before the step began: `Job` may be made before the wait, `ask` not.
+template <int D, int NT> struct Job {
   using S = Shape<D, NT>;
-  constexpr int KG = S::KG, KP = D / 64, MT = D / 16, ROWS = S::ROWS, VW = D / 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const Where w(p, seg.tile);
-  const int kvh = seg.kvh, G = p.G, H = p.a.H, n_rows = w.ntok * G;
-  const RbKeyTiles tiles(w.key_lo, w.key_hi, p.a.keep, TILE);
-  // the warp's share of a tile, and of the tiles
-  constexpr int SHARES = TILE / (16 * KG), STEP = WARPS / SHARES;
-  const int in_tile = warp % SHARES * (16 * KG), kt0 = seg.first + warp / SHARES;
-  const int per = p.a.cache.page_size / TILE;      // tiles of a page
-  const int* pages = p.a.cache.page_table + (int64_t)w.slot * p.a.cache.max_pages;
-  uint8_t* stages = smem + warp * S::NS * S::STAGE;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR) + warp * S::NS;
-
-  auto page_of = [&](int kt) -> int {
+  static constexpr int SHARES = TILE / (16 * S::KG), STEP = WARPS / SHARES;      // the warp's share of a tile, and of the tiles
+  Segment seg;
+  Where w;
+  RbKeyTiles tiles;
+  int in_tile, next;               // the warp's first key in a tile; the tile that is asked for next
+  int page[S::NS];                 // pages of tiles next, next + STEP, ...
+  float2 scales[S::NS - 1];        // of the tiles on their way (keys, values)
+  __device__ __forceinline__ Job(const Params& p, const Segment& s)
+      : seg(s), w(p, s.tile), tiles(w.key_lo, w.key_hi, p.a.keep, TILE) {
+    const int warp = threadIdx.x >> 5;
+    in_tile = warp % SHARES * (16 * S::KG);
+    next = seg.first + warp / SHARES;
+#pragma unroll
+    for (int i = 0; i < S::NS; ++i) page[i] = page_of(p, next + i * STEP);
+  }
+  __device__ __forceinline__ int page_of(const Params& p, int kt) const {
     if (kt >= seg.last) return 0;
-    const int tile = tiles.at(kt);
+    const int tile = tiles.at(kt), per = p.a.cache.page_size / TILE;
 #ifdef RB_CHECKED
-    return (int)(rb_page_offset(p.a.cache, w.slot, tile * TILE, kvh) / ((int64_t)p.Kh * p.a.cache.page_size * D));
+    return (int)(rb_page_offset(p.a.cache, w.slot, tile * TILE, seg.kvh) / ((int64_t)p.Kh * p.a.cache.page_size * D));
 #endif
-    return pages[per == 1 ? tile : tile / per];
-  };
-  // The scales of tile kt, and its codes on their way; nothing of a tile that ends before the warp's share.
-  auto request = [&](int kt, int page) -> float2 {
-    if (kt >= seg.last || ring.failed) return make_float2(1.f, 1.f);
+    return p.a.cache.page_table[(int64_t)w.slot * p.a.cache.max_pages + (per == 1 ? tile : tile / per)];
+  }
+  // The next tile's codes on their way, and its scales (place i of the queue); nothing of a tile that ends before the warp's share.
+  __device__ __forceinline__ void ask(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV, uint8_t* stages, uint64_t* full,
+                                      Ring& ring, int i) {
+    const int kt = next, at = page[0];
+    next += STEP;
+#pragma unroll
+    for (int j = 0; j + 1 < S::NS; ++j) page[j] = page[j + 1];
+    page[S::NS - 1] = page_of(p, next + (S::NS - 1) * STEP);
+    scales[i] = make_float2(1.f, 1.f);
+    if (kt >= seg.last || ring.failed) return;
     const int tile = tiles.at(kt);
-    if (tile * TILE + in_tile > w.key_hi) return make_float2(1.f, 1.f);
-    const int unit = (page * p.Kh + kvh) * per + (per == 1 ? 0 : tile % per);      // the block's number in the pool
+    if (tile * TILE + in_tile > w.key_hi) return;
+    const int per = p.a.cache.page_size / TILE;
+    const int unit = (at * p.Kh + seg.kvh) * per + (per == 1 ? 0 : tile % per);     // the block's number in the pool
     const uint32_t s = ring.asked % S::NS;
     if (elect_one()) {
       mbar_expect_tx(&full[s], S::STAGE);
-      const int row = (int)(((int64_t)unit * TILE + in_tile) * D / 128);           // of 128 bytes
+      const int row = (int)(((int64_t)unit * TILE + in_tile) * D / 128);            // of 128 bytes
       tma_load_2d(stages + s * S::STAGE, tmK, 0, row, &full[s]);
       tma_load_2d(stages + s * S::STAGE + S::CHUNK, tmV, 0, row, &full[s]);
     }
     __syncwarp();
     ++ring.asked;
-    return make_float2(p.a.k_scale[unit], p.a.v_scale[unit]);
-  };
-  int next_page;
-  float2 scales_of[S::NS];           // of the tiles on their way
-  {
-    int first[S::NS];
-#pragma unroll
-    for (int i = 0; i < S::NS; ++i) first[i] = page_of(kt0 + i * STEP);
-#pragma unroll
-    for (int i = 0; i < S::NS - 1; ++i) scales_of[i] = request(kt0 + i * STEP, first[i]);
-    next_page = first[S::NS - 1];
+    scales[i] = make_float2(p.a.k_scale[unit], p.a.v_scale[unit]);
   }
+};
+
+// The block's part of a pair, whose first S::AHEAD tiles have been asked for; `then(ahead)` asks for those of the pair after it.
+template <int D, int NT, typename F>
+__device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV, Job<D, NT>& job, uint8_t* smem,
+                                     Ring& ring, Joined<D, NT>& joined, F then) {
+  using S = Shape<D, NT>;
+  constexpr int KG = S::KG, KP = D / 64, MT = D / 16, ROWS = S::ROWS, VW = D / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const Where w = job.w;
+  const Segment seg = job.seg;
+  const int kvh = seg.kvh, G = p.G, H = p.a.H, n_rows = w.ntok * G, in_tile = job.in_tile;
+  uint8_t* stages = smem + warp * S::NS * S::STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR) + warp * S::NS;
+#pragma unroll
+  for (int i = S::AHEAD; i < S::NS - 1; ++i) job.ask(p, tmK, tmV, stages, full, ring, i);
 
   // ---- the query rows as B operands: of row g of every eight, values 64 j + 16 t + 4 i + (0, 1) and (2, 3)
   uint32_t qf[S::Q_SHARED ? 1 : MT][S::Q_SHARED ? 1 : NT][2];
@@ -255,16 +282,12 @@ __device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, co
   }
 
   bool begun = false;
-  for (int kt = kt0; kt < seg.last && !ring.failed; kt += STEP) {
-    const float2 scales = scales_of[0];
-    {
-      const int ahead = kt + (S::NS - 1) * STEP, after = page_of(ahead + STEP);
+  for (int kt = seg.first + warp / Job<D, NT>::SHARES; kt < seg.last && !ring.failed; kt += Job<D, NT>::STEP) {
+    const float2 scales = job.scales[0];
 #pragma unroll
-      for (int i = 0; i + 2 < S::NS; ++i) scales_of[i] = scales_of[i + 1];
-      scales_of[S::NS - 2] = request(ahead, next_page);
-      next_page = after;
-    }
-    const int key0 = tiles.at(kt) * TILE + in_tile;
+    for (int i = 0; i + 2 < S::NS; ++i) job.scales[i] = job.scales[i + 1];
+    job.ask(p, tmK, tmV, stages, full, ring, S::NS - 2);
+    const int key0 = job.tiles.at(kt) * TILE + in_tile;
     if (key0 > w.key_hi) continue;
     const uint32_t stage = ring.used % S::NS;
     if (!mbar_wait_warp(&full[stage], (ring.used / S::NS) & 1, 15)) {
@@ -442,51 +465,106 @@ __device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, co
     __syncwarp();                    // everybody has left this stage: it may be filled again
   }
 
-  // ---- the four warps, over the ring: every copy has been waited for
-  __syncthreads();
-  float* mO = reinterpret_cast<float*>(smem);
-  float* mM = mO + WARPS * ROWS * D;
-  float* mL = mM + WARPS * ROWS;
+  // ---- the next pair's first tiles, which arrive meanwhile; then the four warps: each leaves its accumulators, as its lanes hold them,
+  // in those stages of its own ring that are not being filled, and takes a quarter of the row tiles from all
+  const uint32_t beside = ring.asked + S::AHEAD;
+  then(stages, full);
+  float2* ml = reinterpret_cast<float2*>(smem + S::OFF_ML);
+  uint32_t* places = reinterpret_cast<uint32_t*>(smem + S::OFF_AT);
+  // (of warp x, the accumulators of the n-th eight)
+  auto left = [&](int x, uint32_t from, int n) {
+    return reinterpret_cast<float4*>(smem + (x * S::NS + (from + n / S::LEFT) % S::NS) * S::STAGE) + n % S::LEFT * (MT * 32) + lane;
+  };
+  if (lane == 0) places[warp] = beside;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int n = 0; n < NT; ++n) {
+    float4* to = left(warp, beside, n);
+#pragma unroll
+    for (int u = 0; u < MT; ++u) to[u * 32] = make_float4(o[n][u][0] * unit, o[n][u][1] * unit, o[n][u][2] * unit, o[n][u][3] * unit);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       float sum = l[n][c];
       sum += __shfl_xor_sync(0xffffffffu, sum, 4);
       sum += __shfl_xor_sync(0xffffffffu, sum, 8);
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-      const int row = warp * ROWS + n * 8 + 2 * t + c;
-      if (g == 0) { mM[row] = m[n][c]; mL[row] = sum; }
-#pragma unroll
-      for (int u = 0; u < MT; ++u)
-        *reinterpret_cast<float2*>(mO + row * D + MT * g * 2 + 2 * u) = make_float2(o[n][u][c] * unit, o[n][u][c + 2] * unit);
+      if (g == 0) ml[warp * ROWS + n * 8 + 2 * t + c] = make_float2(m[n][c], sum);
     }
-  __syncthreads();
-  sO = reinterpret_cast<float*>(smem + S::MERGE);
-  sM = sO + ROWS * D;
-  sL = sM + ROWS;
-  for (int idx = threadIdx.x; idx < n_rows * D; idx += WARPS * 32) {
-    const int r = idx / D, d = idx % D;
-    float top = -INFINITY;
-#pragma unroll
-    for (int x = 0; x < WARPS; ++x) top = fmaxf(top, mM[x * ROWS + r]);
-    const float use = top == -INFINITY ? 0.f : top;
-    float acc = 0.f, sum = 0.f;
-#pragma unroll
-    for (int x = 0; x < WARPS; ++x) {
-      const float f = exp2f(mM[x * ROWS + r] - use);
-      acc += mO[(x * ROWS + r) * D + d] * f;
-      sum += mL[x * ROWS + r] * f;
-    }
-    sO[idx] = acc;
-    if (d == 0) { sM[r] = top; sL[r] = sum; }
   }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float f[WARPS][2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float2 of[WARPS];
+      float top = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < WARPS; ++x) {
+        of[x] = ml[x * ROWS + n * 8 + 2 * t + c];
+        top = fmaxf(top, of[x].x);
+      }
+      const float use = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < WARPS; ++x) {
+        f[x][c] = exp2_fast(of[x].x - use);
+        sum += of[x].y * f[x][c];
+      }
+      joined.m[n][c] = top;
+      joined.l[n][c] = sum;
+    }
+#pragma unroll
+    for (int u = 0; u < S::QT; ++u) {
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int x = 0; x < WARPS; ++x) {
+        const float4 v = left(x, places[x], n)[(warp * S::QT + u) * 32];
+        acc.x += v.x * f[x][0]; acc.y += v.y * f[x][1];
+        acc.z += v.z * f[x][0]; acc.w += v.w * f[x][1];
+      }
+      joined.o[n][u] = acc;
+    }
+  }
+  fence_async_shared();              // (the ring is filled by copies again, after the block's next barrier)
   __syncthreads();
 }
 
+// Values d, d + 1 of rows 2t, 2t + 1 of the n-th eight, unnormalised, with the rows' sums: d = D/8 g + 2u for row tile u of O^T.
 template <int D>
-__device__ __forceinline__ void store(const Params& p, const Where& w, int kvh, int r, int d, float o, float l) {
-  p.a.out[((int64_t)(w.tok0 + r / p.G) * p.a.H + kvh * p.G + r % p.G) * D + d] = __float2bfloat16_rn(o / l);
+__device__ __forceinline__ void store(const Params& p, const Where& w, int kvh, int n, int u, int lane, const float4& o, const float (&l)[2]) {
+  const int d = D / 8 * (lane >> 2) + 2 * u;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int r = n * 8 + 2 * (lane & 3) + c;
+    if (r < w.ntok * p.G) {
+      const float inv = 1.0f / l[c];
+      __nv_bfloat16* dst = p.a.out + ((int64_t)(w.tok0 + r / p.G) * p.a.H + kvh * p.G + r % p.G) * D + d;
+      *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn((c ? o.y : o.x) * inv, (c ? o.w : o.z) * inv);
+    }
+  }
+}
+template <int D, int NT>
+__device__ __forceinline__ void store(const Params& p, const Where& w, int kvh, const Joined<D, NT>& j) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int u = 0; u < Shape<D, NT>::QT; ++u) store<D>(p, w, kvh, n, warp * Shape<D, NT>::QT + u, lane, j.o[n][u], j.l[n]);
+}
+
+// Another part joins the sums so far of rows 2t, 2t + 1 (`of`: its maximum and sum for both).
+__device__ __forceinline__ void add_part(float4& acc, float (&m)[2], float (&l)[2], const float4& o, const float4& of) {
+  float f[2], k[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const float mz = c ? of.z : of.x, top = fmaxf(m[c], mz), use = top == -INFINITY ? 0.f : top;
+    k[c] = exp2_fast(m[c] - use);
+    f[c] = exp2_fast(mz - use);
+    l[c] = l[c] * k[c] + (c ? of.w : of.y) * f[c];
+    m[c] = top;
+  }
+  acc.x = acc.x * k[0] + o.x * f[0]; acc.y = acc.y * k[1] + o.y * f[1];
+  acc.z = acc.z * k[0] + o.z * f[0]; acc.w = acc.w * k[1] + o.w * f[1];
 }
 
 // The warps' barriers; what follows is ordered by the caller's or the first barrier of the block.
@@ -513,54 +591,70 @@ __global__ void __launch_bounds__(WARPS * 32) cluster_kernel(const __grid_consta
   seg.visited = visited_tiles(p, seg.tile);
   seg.first = (int)((int64_t)blockIdx.z * seg.visited / p.parts);
   seg.last = (int)((int64_t)(blockIdx.z + 1) * seg.visited / p.parts);
+  Job<D, NT> job(p, seg);
   rb_pdl_wait();
-  float *sO, *sM, *sL;
-  work<D, NT>(p, &tmK, &tmV, seg, smem, ring, sO, sM, sL);
-  const Where w(p, seg.tile);
-  const int n = w.ntok * p.G * D;
+  {
+    uint8_t* stages = smem + (threadIdx.x >> 5) * S::NS * S::STAGE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR) + (threadIdx.x >> 5) * S::NS;
+#pragma unroll
+    for (int i = 0; i < S::AHEAD; ++i) job.ask(p, &tmK, &tmV, stages, full, ring, i);
+  }
+  Joined<D, NT> mine;
+  work<D, NT>(p, &tmK, &tmV, job, smem, ring, mine, [](uint8_t*, uint64_t*) {});
+  const Where& w = job.w;
   if (p.parts == 1) {
-    for (int idx = threadIdx.x; idx < n; idx += WARPS * 32) store<D>(p, w, seg.kvh, idx / D, idx % D, sO[idx], sL[idx / D]);
+    store<D, NT>(p, w, seg.kvh, mine);
     return;
+  }
+  // what the cluster's other blocks read, over the ring
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float4* sO = reinterpret_cast<float4*>(smem);
+  float2* sML = reinterpret_cast<float2*>(smem + S::OFF_ML) + WARPS * S::ROWS;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int u = 0; u < S::QT; ++u) sO[(n * S::MT + warp * S::QT + u) * 32 + lane] = mine.o[n][u];
+    if (warp == 0 && lane < 4) {
+      sML[n * 8 + 2 * lane] = make_float2(mine.m[n][0], mine.l[n][0]);
+      sML[n * 8 + 2 * lane + 1] = make_float2(mine.m[n][1], mine.l[n][1]);
+    }
   }
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  for (int idx = (int)blockIdx.z * WARPS * 32 + threadIdx.x; idx < n; idx += p.parts * WARPS * 32) {
-    const int r = idx / D;
-    float m[16], l[16], o[16];
+  // every block finishes a share of the lanes' accumulators from all parts, in part order
+  for (int idx = (int)blockIdx.z * WARPS * 32 + threadIdx.x; idx < NT * S::MT * 32; idx += p.parts * WARPS * 32) {
+    const int n = idx / (S::MT * 32), u = idx / 32 % S::MT, row = n * 8 + 2 * (idx & 3);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int z0 = 0; z0 < p.parts; z0 += 4) {
+      float4 o[4], of[4];            // (of: maximum and sum of both rows)
 #pragma unroll
-    for (int z = 0; z < 16; ++z) {                 // everything is asked for first
-      m[z] = -INFINITY; l[z] = 0.f; o[z] = 0.f;
-      if (z < p.parts) {
-        uint32_t am, al, ao;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(am) : "r"(smem_u32(sM + r)), "r"((uint32_t)z));
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(al) : "r"(smem_u32(sL + r)), "r"((uint32_t)z));
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ao) : "r"(smem_u32(sO + idx)), "r"((uint32_t)z));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(m[z]) : "r"(am));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(l[z]) : "r"(al));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o[z]) : "r"(ao));
+      for (int z = 0; z < 4; ++z) {
+        o[z] = make_float4(0.f, 0.f, 0.f, 0.f);
+        of[z] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+        if (z0 + z < p.parts) {
+          uint32_t ao, am;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ao) : "r"(smem_u32(sO + idx)), "r"((uint32_t)(z0 + z)));
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(am) : "r"(smem_u32(sML + row)), "r"((uint32_t)(z0 + z)));
+          asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(o[z].x), "=f"(o[z].y), "=f"(o[z].z), "=f"(o[z].w) : "r"(ao));
+          asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(of[z].x), "=f"(of[z].y), "=f"(of[z].z), "=f"(of[z].w) : "r"(am));
+        }
       }
-    }
-    float top = -INFINITY;
 #pragma unroll
-    for (int z = 0; z < 16; ++z) top = fmaxf(top, m[z]);
-    const float use = top == -INFINITY ? 0.f : top;
-    float acc = 0.f, sum = 0.f;
-#pragma unroll
-    for (int z = 0; z < 16; ++z) {
-      const float f = exp2f(m[z] - use);
-      sum += l[z] * f;
-      acc += o[z] * f;
+      for (int z = 0; z < 4; ++z) add_part(acc, m, l, o[z], of[z]);
     }
-    store<D>(p, w, seg.kvh, r, idx % D, acc, sum);
+    store<D>(p, w, seg.kvh, n, u, idx & 31, acc, l);
   }
   // nobody's shared memory goes away while another part reads it
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Dealt out: all pairs' tiles of keys in the order (row tile, kv head, tile); a block takes `share` of them, one after the other.
+// Dealt out: all pairs' tiles of keys in the order (row tile, kv head, tile); a block takes `share` of them, one after the other.  To begin
+// and to end a pair costs as much as BEGIN tiles, which are dealt out with the others, ahead of the pair's own.
 // What a block leaves for a pair that it shares goes to place block + pair of the scratch: no two blocks' places are the same,
 // and those of one pair follow one another.
+constexpr int BEGIN = 10;
 __device__ __forceinline__ int64_t share_of(const Params& p, int64_t total, int blocks) {
   const int64_t even = (total + blocks - 1) / blocks;
   return even > p.least ? even : p.least;
@@ -589,19 +683,18 @@ __global__ void __launch_bounds__(WARPS * 32) dealt_kernel(const __grid_constant
   __shared__ int counts[WARPS], s_tile, s_before;
   // positions, slots and page tables were written before the step began: the deal needs no wait
   int mine = 0;
-  for (int i = threadIdx.x; i < p.n_tiles; i += WARPS * 32) mine += visited_tiles(p, i);
+  for (int i = threadIdx.x; i < p.n_tiles; i += WARPS * 32) mine += visited_tiles(p, i) + BEGIN;
   const int64_t total = (int64_t)block_count(mine, counts) * p.Kh;
   const int64_t share = share_of(p, total, gridDim.x);
   int64_t x = (int64_t)blockIdx.x * share;
   const int64_t end = x + share < total ? x + share : total;
-  rb_pdl_wait();
   if (x >= end) return;
   // the row tile that tile x of all belongs to: the first warp walks over them, 32 at a time
   if (threadIdx.x < 32) {
     int before = 0;
     for (int i0 = 0; i0 < p.n_tiles; i0 += 32) {
       const int i = i0 + (int)threadIdx.x;
-      const int n = i < p.n_tiles ? visited_tiles(p, i) : 0;
+      const int n = i < p.n_tiles ? visited_tiles(p, i) + BEGIN : 0;
       int upto = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -620,80 +713,102 @@ __global__ void __launch_bounds__(WARPS * 32) dealt_kernel(const __grid_constant
   __syncthreads();
   int tile = s_tile;
   int64_t base = (int64_t)s_before * p.Kh;         // the first tile of the row tile's pairs
-  while (x < end) {
-    Segment seg;
-    seg.visited = visited_tiles(p, tile);
-    if (x >= base + (int64_t)seg.visited * p.Kh) { base += (int64_t)seg.visited * p.Kh; ++tile; continue; }
-    seg.tile = tile;
-    seg.kvh = (int)((x - base) / seg.visited);
-    const int64_t pair0 = base + (int64_t)seg.kvh * seg.visited;
-    seg.first = (int)(x - pair0);
-    seg.last = (int)(end - pair0 < seg.visited ? end - pair0 : seg.visited);
-    float *sO, *sM, *sL;
-    work<D, NT>(p, &tmK, &tmV, seg, smem, ring, sO, sM, sL);
-    const Where w(p, tile);
-    const int n_rows = w.ntok * p.G, n = n_rows * D;
-    if (seg.first == 0 && seg.last == seg.visited) {
-      for (int idx = threadIdx.x; idx < n; idx += WARPS * 32) store<D>(p, w, seg.kvh, idx / D, idx % D, sO[idx], sL[idx / D]);
-    } else {
-      const int64_t place = blockIdx.x + (int64_t)tile * p.Kh + seg.kvh;
-      for (int idx = threadIdx.x; idx < n; idx += WARPS * 32) p.part_o[place * S::ROWS * D + idx] = sO[idx];
-      for (int r = threadIdx.x; r < n_rows; r += WARPS * 32) {
-        p.part_ml[(place * S::ROWS + r) * 2] = sM[r];
-        p.part_ml[(place * S::ROWS + r) * 2 + 1] = sL[r];
-      }
+  // the block's next segment (tile < 0: none is left)
+  auto next_segment = [&]() -> Segment {
+    while (x < end) {
+      Segment seg;
+      seg.visited = visited_tiles(p, tile);
+      const int length = seg.visited + BEGIN;
+      if (x >= base + (int64_t)length * p.Kh) { base += (int64_t)length * p.Kh; ++tile; continue; }
+      seg.tile = tile;
+      seg.kvh = (int)((x - base) / length);
+      const int64_t pair0 = base + (int64_t)seg.kvh * length;
+      seg.first = max((int)(x - pair0) - BEGIN, 0);
+      seg.last = (int)(end - pair0 < length ? end - pair0 : length) - BEGIN;
+      x = pair0 + length;
+      if (seg.last > seg.first) return seg;        // (else the range ends with what the pair's beginning costs)
     }
-    __syncthreads();                               // the shared sums have been read
-    x = pair0 + seg.last;
+    return Segment{-1, 0, 0, 0, 0};
+  };
+  Segment seg = next_segment();
+  if (seg.tile < 0) return;
+  Job<D, NT> job(p, seg);
+  rb_pdl_wait();
+  {
+    uint8_t* stages = smem + (threadIdx.x >> 5) * S::NS * S::STAGE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR) + (threadIdx.x >> 5) * S::NS;
+#pragma unroll
+    for (int i = 0; i < S::AHEAD; ++i) job.ask(p, &tmK, &tmV, stages, full, ring, i);
+  }
+  while (seg.tile >= 0) {
+    const Segment now = seg;
+    const Where w = job.w;
+    Joined<D, NT> mine;
+    work<D, NT>(p, &tmK, &tmV, job, smem, ring, mine, [&](uint8_t* stages, uint64_t* full) {
+      seg = next_segment();
+      if (seg.tile < 0) return;
+      job = Job<D, NT>(p, seg);
+#pragma unroll
+      for (int i = 0; i < S::AHEAD; ++i) job.ask(p, &tmK, &tmV, stages, full, ring, i);
+    });
+    if (now.first == 0 && now.last == now.visited) {
+      store<D, NT>(p, w, now.kvh, mine);
+      continue;
+    }
+    const int64_t place = blockIdx.x + (int64_t)now.tile * p.Kh + now.kvh;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int u = 0; u < S::QT; ++u) p.part_o[((place * NT + n) * S::MT + warp * S::QT + u) * 32 + lane] = mine.o[n][u];
+      if (warp == 0 && lane < 4)
+        *reinterpret_cast<float4*>(p.part_ml + place * S::ROWS + n * 8 + 2 * lane) = make_float4(mine.m[n][0], mine.l[n][0], mine.m[n][1], mine.l[n][1]);
+    }
   }
 }
 
-// Pairs that several blocks have worked on, one block of threads each: every warp takes every eighth part, joined in shared memory.
+// Pairs that several blocks have worked on: a block of threads per pair and 8 rows, a thread for what one lane's accumulators of a row tile hold.
 template <int D, int NT>
-__global__ void __launch_bounds__(256) join_kernel(Params p, int blocks) {
+__global__ void __launch_bounds__(D * 2) join_kernel(Params p, int blocks) {
   rb_pdl_launch_dependents();
-  constexpr int ROWS = 8 * NT;
-  extern __shared__ __align__(16) float joined[];  // [ROWS] maxima, [ROWS] sums
-  __shared__ int counts[8];
-  const int tile = blockIdx.x, kvh = blockIdx.y;
-  int mine = 0, ahead = 0;
-  for (int i = threadIdx.x; i < p.n_tiles; i += 256) {
-    const int n = visited_tiles(p, i);
-    mine += n;
-    if (i < tile) ahead += n;
+  constexpr int MT = D / 16;
+  __shared__ int counts[D / 16];
+  const int tile = blockIdx.x, kvh = blockIdx.y, n = blockIdx.z;
+  int all = 0, ahead = 0;
+  for (int i = threadIdx.x; i < p.n_tiles; i += D * 2) {
+    const int v = visited_tiles(p, i) + BEGIN;
+    all += v;
+    if (i < tile) ahead += v;
   }
-  const int64_t total = (int64_t)block_count(mine, counts) * p.Kh;
+  const int64_t total = (int64_t)block_count(all, counts) * p.Kh;
   const int64_t base = (int64_t)block_count(ahead, counts) * p.Kh;
-  const int visited = visited_tiles(p, tile);
-  const int64_t share = share_of(p, total, blocks), pair0 = base + (int64_t)kvh * visited;
-  const int first = (int)(pair0 / share), last = (int)((pair0 + visited - 1) / share);
-  rb_pdl_wait();
-  if (first == last) return;
   const Where w(p, tile);
-  const int n_rows = w.ntok * p.G;
-  const int64_t place0 = first + (int64_t)tile * p.Kh + kvh;
-  const int parts = last - first + 1;
-  const float* ml = p.part_ml + place0 * ROWS * 2;
-  // every row's maximum over the parts, and the sum that belongs to it
-  for (int r = threadIdx.x >> 5; r < n_rows; r += 8) {
-    const int lane = threadIdx.x & 31;
-    float top = -INFINITY, sum = 0.f;
-    for (int z = lane; z < parts; z += 32) top = fmaxf(top, ml[((int64_t)z * ROWS + r) * 2]);
-    top = rb_warp_max(top);
-    const float use = top == -INFINITY ? 0.f : top;
-    for (int z = lane; z < parts; z += 32) sum += ml[((int64_t)z * ROWS + r) * 2 + 1] * exp2f(ml[((int64_t)z * ROWS + r) * 2] - use);
-    sum = rb_warp_sum(sum);
-    if (lane == 0) { joined[r] = use; joined[ROWS + r] = sum; }
+  const int length = RbKeyTiles(w.key_lo, w.key_hi, p.a.keep, TILE).n + BEGIN;
+  const int64_t share = share_of(p, total, blocks), pair0 = base + (int64_t)kvh * length;
+  const int64_t first = (pair0 + BEGIN) / share, last = (pair0 + length - 1) / share;
+  rb_pdl_wait();
+  if (first == last || n * 8 >= w.ntok * p.G) return;
+  const int64_t place = first + (int64_t)tile * p.Kh + kvh;
+  const int parts = (int)(last - first) + 1, lane = threadIdx.x & 31;
+  const float4* po = p.part_o + (place * NT + n) * MT * 32 + threadIdx.x;
+  const float2* pm = p.part_ml + place * 8 * NT + n * 8 + 2 * (lane & 3);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  for (int z0 = 0; z0 < parts; z0 += 4) {
+    float4 o[4], of[4];
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      o[z] = make_float4(0.f, 0.f, 0.f, 0.f);
+      of[z] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+      if (z0 + z < parts) {
+        o[z] = po[(int64_t)(z0 + z) * NT * MT * 32];
+        of[z] = *reinterpret_cast<const float4*>(pm + (int64_t)(z0 + z) * 8 * NT);
+      }
+    }
+#pragma unroll
+    for (int z = 0; z < 4; ++z) add_part(acc, m, l, o[z], of[z]);
   }
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < n_rows * D; idx += 256) {
-    const int r = idx / D;
-    const float* o = p.part_o + place0 * ROWS * D + idx;
-    float acc = 0.f;
-#pragma unroll 8
-    for (int z = 0; z < parts; ++z) acc += o[(int64_t)z * ROWS * D] * exp2f(ml[((int64_t)z * ROWS + r) * 2] - joined[r]);
-    store<D>(p, w, kvh, r, idx % D, acc, joined[ROWS + r]);
-  }
+  store<D>(p, w, kvh, n, (int)threadIdx.x >> 5, lane, acc, l);
 }
 
 // blocks of the kernel that an SM holds: by registers at the kernel's bound and by shared memory
@@ -751,7 +866,7 @@ int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, int bl
   per_sm<D, NT>();                                 // (sets the kernels' attributes)
   if (p.parts == 0) {
     RB_LAUNCH("rb_attention8_rows", (dealt_kernel<D, NT>), blocks, WARPS * 32, S::BYTES, stream, tk, tv, p);
-    RB_LAUNCH("rb_attention8_rows (join)", (join_kernel<D, NT>), dim3(p.n_tiles, p.Kh), 256, S::ROWS * 8, stream, p, blocks);
+    RB_LAUNCH("rb_attention8_rows (join)", (join_kernel<D, NT>), dim3(p.n_tiles, p.Kh, NT), D * 2, 0, stream, p, blocks);
     return 0;
   }
   cudaLaunchConfig_t cfg = {};
@@ -793,6 +908,7 @@ RB_EXPORT int rb_attention8_rows_plan(int n_tiles, int rows, int Kh, int D, int 
   const int NT = (rows + 7) / 8, places = rows8::places(D, NT), most = rows8::most_parts(D, NT);
   const int tiles = (context + rows8::TILE - 1) / rows8::TILE;
   const long long pairs = (long long)n_tiles * Kh;
+  RB_REQUIRE(n_tiles > 0 && Kh > 0 && rows > 0 && rows <= 32, "rb_attention8_rows_plan: %d tiles of %d rows, %d kv heads", n_tiles, rows, Kh);
   int parts = 1;
   while (parts * 2 <= tiles && parts < most && pairs * parts * 2 <= places) parts *= 2;
   out4[0] = parts; out4[1] = out4[2] = out4[3] = 0;
@@ -826,7 +942,7 @@ RB_EXPORT int rb_attention8_rows(void* out, const void* q, void* cache_k, void* 
   p.a.tok_pos = tok_pos; p.a.tok_slot = tok_slot; p.a.H = H;
   p.a.scale = scale; p.a.window = window; p.a.keep = window > 0 ? opt.keep_first : 0; p.a.sinks = opt.sinks; p.a.softcap = opt.softcap;
   p.tile_tok0 = tile_tok0; p.tile_ntok = tile_ntok; p.n_tiles = n_tiles; p.Kh = Kh; p.G = H / Kh;
-  p.parts = parts; p.least = 4; p.part_o = part_o; p.part_ml = part_ml;
+  p.parts = parts; p.least = 4; p.part_o = (float4*)part_o; p.part_ml = (float2*)part_ml;
   CUtensorMap tk, tv;                                // rows of 128 bytes, a warp's 32 positions a box
   const long long rows128 = n_pages * Kh * page_size * D / 128;
   if (rb_get_tensor_map(&tk, cache_k, rows128, 64, 64, 32 * D / 128) != 0) return -1;
