@@ -9,15 +9,24 @@
 // that is the token taken.  A logit that is NaN counts as -inf; a draft outside the vocabulary is not accepted and takes
 // nothing from p; where p - q leaves nothing, the token is drawn from p.
 //
-// Exponentials and sums are float64: the running sum over 100,000 tokens decides on a single token, and in float32 it would
-// move by more than the smallest probabilities, another way for every way of cutting the sum.
+// What decides on a single token is float64: the running sum over 100,000 tokens would move by more than the smallest
+// probabilities in float32, another way for every way of cutting it.  But that sum is taken over ONE row a sequence, the row whose
+// token is taken; whether a draft is accepted hangs on a row's whole sum, and float32 decides that too unless u q S lies within
+// 2^-14 of p S.  So:
+//   rows    every row's maximum and float32 sum, a block of threads per 8,192 logits: one pass, 16-byte loads, each logit read once
+//   pick    a cluster per sequence.  The drafts in turn (a row whose float32 sum leaves it open is summed again in float64); then
+//           the float64 sums of max(p - q, 0) over the blocks' and their warps' shares of the row taken, and the walk into one of them.
+// The float32 sum S' is off by less than 2^-14 of itself: a term e^x is off by 2^-22 and by what rounding x = (z - max) / T does,
+// 2^-23 |x|, which a term of a weight worth counting (|x| < 40) turns into 2^-17 of it; the sum adds 2^-19 at most (64 terms a thread).
+// Bounded by memory: 64 sequences of 4 drafts over 128,256 logits are 164 MB.
 #include "rb_common.cuh"
 
 namespace {
 
-constexpr int CHUNK = 4096, THREADS = 256, PICK_THREADS = 1024;
+constexpr int CHUNK = 8192, THREADS = 256, PICK_WARPS = 16, PICK_THREADS = PICK_WARPS * 32;
+constexpr double OPEN = 1.0 / 16384;             // float32 decides outside this share of the two sides
 
-struct Stat { double sum; float max; int arg; };
+struct Stat { float max, sum; int arg, unused; };
 
 struct Verify {
   int* accepted;               // [B]
@@ -35,154 +44,318 @@ struct Verify {
 };
 
 __device__ __forceinline__ float clean(float v) { return v != v ? -INFINITY : v; }
-// exp((z - m) / T), 1 at the maximum itself (also where that is infinite)
-__device__ __forceinline__ double weight(float z, float m, double inv_t) {
-  return z == m ? 1.0 : exp(((double)z - (double)m) * inv_t);
+
+// exp((z - m) / T) with c = log2(e) / T, 1 at the maximum itself (also where that is infinite): float32 and float64
+__device__ __forceinline__ float weight_f32(float z, float m, float c) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((z - m) * c));
+  return z == m ? 1.f : y;
+}
+// 2^x for x <= 0: the nearest whole number goes to the exponent, Taylor's series of e^(r ln 2) for the rest, |r| <= 1/2 (the first
+// term left out is 4e-18)
+__device__ __forceinline__ double weight(float z, float m, double c) {
+  if (z == m) return 1.0;
+  const double x = ((double)z - (double)m) * c;
+  if (!(x > -1021.0)) return 0.0;
+  const double whole = x + 6755399441055744.0;   // 1.5 * 2^52: rounds to whole numbers, which are its low bits
+  const double t = (x - (whole - 6755399441055744.0)) * 0.69314718055994530942;
+  double e = 1.0 / 6227020800.0;
+  e = fma(e, t, 1.0 / 479001600.0);
+  e = fma(e, t, 1.0 / 39916800.0);
+  e = fma(e, t, 1.0 / 3628800.0);
+  e = fma(e, t, 1.0 / 362880.0);
+  e = fma(e, t, 1.0 / 40320.0);
+  e = fma(e, t, 1.0 / 5040.0);
+  e = fma(e, t, 1.0 / 720.0);
+  e = fma(e, t, 1.0 / 120.0);
+  e = fma(e, t, 1.0 / 24.0);
+  e = fma(e, t, 1.0 / 6.0);
+  e = fma(e, t, 0.5);
+  e = fma(e, t, 1.0);
+  e = fma(e, t, 1.0);
+  return __hiloint2double(__double2hiint(e) + (__double2loint(whole) << 20), __double2loint(e));
+}
+__device__ __forceinline__ double inverse_temperature(float temp) { return 1.4426950408889634074 / (double)temp; }
+
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
-__global__ void __launch_bounds__(THREADS) verify_stats_kernel(Verify p) {
+// VEC: rows begin on 16 bytes.
+template <bool VEC>
+__global__ void __launch_bounds__(THREADS) verify_rows_kernel(Verify p) {
   rb_pdl_launch_dependents();
+  constexpr int PER = CHUNK / THREADS;
+  __shared__ float s_max[THREADS / 32], s_sum[THREADS / 32];
+  __shared__ int s_arg[THREADS / 32];
+  const int r = blockIdx.x, lo = blockIdx.y * CHUNK, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   rb_pdl_wait();
-  __shared__ float scratch[33];
-  __shared__ double sums[THREADS / 32];
-  __shared__ int s_arg;
-  const int r = blockIdx.x, c = blockIdx.y;
+  const float* z = p.logits + (int64_t)r * p.stride + lo;
+  const int n = min(p.V - lo, CHUNK);
+  float v[PER];
+#pragma unroll
+  for (int i = 0; i < PER / 4; ++i) {
+    const int at = (i * THREADS + threadIdx.x) * 4;
+    if (VEC && at + 4 <= n) {
+      const float4 x = *reinterpret_cast<const float4*>(z + at);
+      v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[4 * i + j] = at + j < n ? z[at + j] : -INFINITY;
+    }
+  }
+  // the row's sequence: the last that begins at or before it
   int seq = 0;
-  while (seq + 1 < p.B && p.first_row[seq + 1] <= r) ++seq;
-  const float temp = p.temperature[seq];
-  const float* z = p.logits + (int64_t)r * p.stride;
-  const int lo = c * CHUNK, hi = min(p.V, lo + CHUNK);
-  float m = -INFINITY;
-  for (int i = lo + threadIdx.x; i < hi; i += THREADS) m = fmaxf(m, clean(z[i]));
-  m = rb_block_max(m, scratch);
-  if (threadIdx.x == 0) s_arg = hi;
-  __syncthreads();
-  for (int i = lo + threadIdx.x; i < hi; i += THREADS)
-    if (clean(z[i]) == m) { atomicMin(&s_arg, i); break; }
-  double sum = 0.0;
-  if (temp > 0.f && m > -INFINITY) {
-    const double inv_t = 1.0 / (double)temp;
-    for (int i = lo + threadIdx.x; i < hi; i += THREADS) sum += weight(clean(z[i]), m, inv_t);
+  for (int a = 0, b = p.B; a < b;) {
+    const int mid = (a + b) >> 1;
+    if (p.first_row[mid] <= r) { seq = mid; a = mid + 1; } else { b = mid; }
   }
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
+  const float temp = p.temperature[seq];
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    v[i] = clean(v[i]);
+    m = fmaxf(m, v[i]);
+  }
+  m = rb_warp_max(m);
+  if (lane == 0) s_max[warp] = m;
+  __syncthreads();
+  m = s_max[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 32; ++w) m = fmaxf(m, s_max[w]);
+  float sum = 0.f;
+  int arg = p.V;
+  if (temp > 0.f) {
+    if (m > -INFINITY) {
+      const float c = (float)inverse_temperature(temp);
+      float four[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < PER; ++i) four[i & 3] += weight_f32(v[i], m, c);
+      sum = (four[0] + four[1]) + (four[2] + four[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = PER - 1; i >= 0; --i)
+      if (v[i] == m) arg = lo + ((i >> 2) * THREADS + (int)threadIdx.x) * 4 + (i & 3);
+    arg = __reduce_min_sync(0xffffffffu, arg);
+  }
+  sum = rb_warp_sum(sum);
+  if (lane == 0) { s_sum[warp] = sum; s_arg[warp] = arg; }
   __syncthreads();
   if (threadIdx.x == 0) {
-    double all = 0.0;
-    for (int w = 0; w < THREADS / 32; ++w) all += sums[w];
-    p.stats[(int64_t)r * p.chunks + c] = Stat{all, m, s_arg};
+    for (int w = 1; w < THREADS / 32; ++w) { sum += s_sum[w]; arg = min(arg, s_arg[w]); }
+    p.stats[(int64_t)r * p.chunks + blockIdx.y] = Stat{m, sum, arg, 0};
   }
 }
 
-__global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p) {
-  rb_pdl_launch_dependents();
-  rb_pdl_wait();
-  __shared__ double part[PICK_THREADS];
-  __shared__ double s_total, s_before;
-  __shared__ float s_max;
-  __shared__ int s_row, s_arg, s_owner, s_count, s_last;
-  // (rows outside the logits, which only a wrong first_row can name, are left out)
-  const int b = blockIdx.x, r0 = min(max(p.first_row[b], 0), p.R), r1 = min(p.first_row[b + 1], p.R);
-  const float temp = p.temperature[b];
-  const double inv_t = 1.0 / (double)temp;
-  int* tokens = p.tokens + (int64_t)b * (p.most + 1);
-  for (int j = threadIdx.x; j <= p.most; j += PICK_THREADS) tokens[j] = -1;
+// The block's sum of a value per thread, the same in all of them (sums in a fixed order).
+__device__ __forceinline__ double block_sum(double v, double* s) {
+  v = warp_sum(v);
   __syncthreads();
-  if (threadIdx.x == 0) {
-    s_row = -1;
-    int n = 0;
-    for (int r = r0; r < r1; ++r) {
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double all = 0.0;
+#pragma unroll
+  for (int w = 0; w < PICK_WARPS; ++w) all += s[w];
+  return all;
+}
+
+// The first of n values (a lane has the lane-th) at which the running sum after `before` exceeds `goal`, else the last above zero (else -1);
+// `before` becomes the sum ahead of it.  All lanes get both.
+__device__ __forceinline__ int first_over(double v, int n, double goal, double& before) {
+  const int lane = threadIdx.x & 31;
+  double run = before;
+  int found = -1, last = -1;
+  double ahead = before, ahead_of_last = before;
+  for (int i = 0; i < n; ++i) {
+    const double x = __shfl_sync(0xffffffffu, v, i);
+    if (x > 0.0) { last = i; ahead_of_last = run; }
+    if (found < 0 && run + x > goal) { found = i; ahead = run; }
+    run += x;
+  }
+  (void)lane;
+  before = found >= 0 ? ahead : ahead_of_last;
+  return found >= 0 ? found : last;
+}
+
+// A cluster per sequence: block c has logits c * share .. of the row whose token is taken, a warp a PICK_WARPS-th of those.
+__global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int blocks) {
+  rb_pdl_launch_dependents();
+  __shared__ double s_sums[PICK_WARPS];          // what the block's warps have
+  __shared__ double s_shown[2];                  // what the cluster's blocks read
+  __shared__ int s_found[PICK_WARPS], s_args[PICK_WARPS];
+  __shared__ float s_maxima[PICK_WARPS];
+  __shared__ int s_n, s_row, s_arg;
+  __shared__ float s_m;
+  const int rank = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  rb_pdl_wait();
+  // (rows outside the logits, which only a wrong first_row can name, are left out)
+  const int r0 = min(max(p.first_row[b], 0), p.R), r1 = min(p.first_row[b + 1], p.R);
+  const float temp = p.temperature[b];
+  const double c = inverse_temperature(temp);
+  int* tokens = p.tokens + (int64_t)b * (p.most + 1);
+  if (threadIdx.x == 0) { s_n = 0; s_row = -1; s_arg = -1; }
+  if (rank == 0)
+    for (int j = threadIdx.x; j <= p.most; j += PICK_THREADS) tokens[j] = -1;
+  __syncthreads();
+  auto total_of = [&](int r, float m) {          // a row's float64 sum, by the whole block
+    const float* z = p.logits + (int64_t)r * p.stride;
+    double mine = 0.0;
+    for (int i = threadIdx.x; i < p.V; i += PICK_THREADS) mine += weight(clean(z[i]), m, c);
+    return block_sum(mine, s_sums);
+  };
+  // ---- the drafts, PICK_WARPS rows at a time, a warp each: 1 accepted, 0 not, 2 open
+  for (int at = r0; at < r1; at += PICK_WARPS) {
+    const int r = at + warp;
+    int found = 0, arg = p.V;
+    float m = -INFINITY;
+    if (r < r1) {
       const Stat* st = p.stats + (int64_t)r * p.chunks;
-      float m = -INFINITY;
-      int arg = 0;
-      for (int c = 0; c < p.chunks; ++c)
-        if (st[c].max > m) { m = st[c].max; arg = st[c].arg; }      // chunks ascend: the lowest of equals
+      for (int i = lane; i < p.chunks; i += 32) m = fmaxf(m, st[i].max);
+      m = rb_warp_max(m);
       const bool greedy = !(temp > 0.f && m > -INFINITY);
-      double total = 1.0;
-      if (!greedy) {
-        total = 0.0;
-        for (int c = 0; c < p.chunks; ++c)
-          if (st[c].max > -INFINITY) total += st[c].sum * weight(st[c].max, m, inv_t);
-      }
-      const int d = p.drafts[r];
-      if (r + 1 < r1 && n < p.most && d >= 0 && d < p.V) {
-        const double q = p.probs ? (double)p.probs[(int64_t)r * p.probs_stride + d] : 1.0;
-        const double w = greedy ? (d == arg ? 1.0 : 0.0) : weight(clean(p.logits[(int64_t)r * p.stride + d]), m, inv_t);
-        if ((double)p.uniforms[2 * (int64_t)r] * q * total < w) {
-          tokens[n++] = d;
-          continue;
+      double total = 0.0;
+      for (int i = lane; i < p.chunks; i += 32) {
+        const Stat one = st[i];
+        if (greedy) {
+          if (one.max == m) arg = min(arg, temp > 0.f ? 0 : one.arg);
+        } else if (one.max > -INFINITY) {
+          total += (double)one.sum * weight(one.max, m, c);
         }
       }
-      s_row = r; s_total = total; s_max = m; s_arg = greedy ? arg : -1;
-      break;
+      total = warp_sum(total);
+      arg = greedy ? __reduce_min_sync(0xffffffffu, arg) : -1;
+      const int d = p.drafts[r];
+      if (r + 1 < r1 && r - r0 < p.most && d >= 0 && d < p.V) {
+        const double q = p.probs ? (double)p.probs[(int64_t)r * p.probs_stride + d] : 1.0;
+        const double left = (double)p.uniforms[2 * (int64_t)r] * q;
+        if (greedy) {
+          found = left < (d == arg ? 1.0 : 0.0) ? 1 : 0;
+        } else {
+          const double w = weight(clean(p.logits[(int64_t)r * p.stride + d]), m, c), side = left * total;
+          found = side * (1.0 + OPEN) < w ? 1 : (side * (1.0 - OPEN) >= w ? 0 : 2);
+        }
+      }
     }
-    p.accepted[b] = n;
-    s_count = n;
+    if (lane == 0) { s_found[warp] = found; s_args[warp] = arg; s_maxima[warp] = m; }
+    __syncthreads();
+    int n = 0;
+    for (; n < PICK_WARPS && at + n < r1; ++n) {
+      int f = s_found[n];
+      if (f == 2) {                              // (the same in all threads, and in all blocks of the cluster)
+        const int row = at + n, d = p.drafts[row];
+        const double q = p.probs ? (double)p.probs[(int64_t)row * p.probs_stride + d] : 1.0;
+        const double total = total_of(row, s_maxima[n]);
+        f = (double)p.uniforms[2 * (int64_t)row] * q * total < weight(clean(p.logits[(int64_t)row * p.stride + d]), s_maxima[n], c) ? 1 : 0;
+      }
+      if (f == 0) break;
+      if (threadIdx.x == 0) {
+        if (rank == 0) tokens[at - r0 + n] = p.drafts[at + n];
+        ++s_n;
+      }
+    }
+    const bool here = n < PICK_WARPS && at + n < r1;
+    if (here && threadIdx.x == 0) { s_row = at + n; s_arg = s_args[n]; s_m = s_maxima[n]; }
+    __syncthreads();
+    if (here) break;
   }
-  __syncthreads();
-  const int r = s_row;
-  if (r < 0) return;                             // a sequence without rows
-  if (s_arg >= 0) {
-    if (threadIdx.x == 0) tokens[s_count] = s_arg;
+  const int r = s_row, taken = s_n;
+  if (rank == 0 && threadIdx.x == 0) p.accepted[b] = taken;
+  if (r < 0) return;                             // a sequence without rows: all blocks of the cluster
+  if (s_arg >= 0) {                              // nothing is drawn
+    if (rank == 0 && threadIdx.x == 0) tokens[taken] = s_arg;
     return;
   }
+  // ---- the token: sums over the blocks' and the warps' shares
   const float* z = p.logits + (int64_t)r * p.stride;
   const int d = r + 1 < r1 ? p.drafts[r] : -1;
   const bool judged = d >= 0 && d < p.V;
   const float* q = judged && p.probs ? p.probs + (int64_t)r * p.probs_stride : nullptr;
-  const double total = s_total;
-  const float m = s_max;
-  const int per = (p.V + PICK_THREADS - 1) / PICK_THREADS;
-  const int lo = min(p.V, (int)threadIdx.x * per), hi = min(p.V, lo + per);
+  const float m = s_m;
+  const int per_warp = ((p.V + blocks - 1) / blocks + PICK_THREADS - 1) / PICK_THREADS * 32;       // a multiple of 32
+  const int lo = min((int64_t)p.V, ((int64_t)rank * PICK_WARPS + warp) * per_warp), hi = min(p.V, lo + per_warp);
+  int turn = 0;
+  // the cluster's sum of a block's values, and of those ahead of this block
+  auto over_cluster = [&](double v, double& ahead) {
+    if (threadIdx.x == 0) s_shown[turn & 1] = v;
+    __syncthreads();
+    double all = v;
+    ahead = 0.0;
+    if (blocks > 1) {
+      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+      all = 0.0;
+      for (int x = 0; x < blocks; ++x) {
+        uint32_t at;
+        double one;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&s_shown[turn & 1])), "r"(x));
+        asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(one) : "r"(at));
+        if (x == rank) ahead = all;
+        all += one;
+      }
+    }
+    ++turn;
+    return all;
+  };
+  double total = 1.0, ahead = 0.0;
+  if (q) {
+    double mine = 0.0;
+#pragma unroll 4
+    for (int i = lo + lane; i < hi; i += 32) mine += weight(clean(z[i]), m, c);
+    total = over_cluster(block_sum(mine, s_sums), ahead);
+  }
   // whole: from p itself, where p - q has nothing left
   for (int whole = judged ? 0 : 1; whole < 2; ++whole) {
+    // (p - q) times the sum of the weights: without q nothing is divided, so that equal logits are equal steps exactly
     auto left = [&](int i) -> double {
-      // (p - q) times the sum of the weights: without q nothing is divided, so that equal logits are equal steps exactly
-      const double w = weight(clean(z[i]), m, inv_t);
+      const double w = weight(clean(z[i]), m, c);
       if (whole) return w;
       if (q) return fmax(w - (double)q[i] * total, 0.0);
       return i == d ? 0.0 : w;
     };
     double mine = 0.0;
-    for (int i = lo; i < hi; ++i) mine += left(i);
-    part[threadIdx.x] = mine;
-    if (threadIdx.x == 0) s_last = -1;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      double all = 0.0;
-      for (int t = 0; t < PICK_THREADS; ++t) all += part[t];
-      const double goal = (double)p.uniforms[2 * (int64_t)r + 1] * all;
-      double before = 0.0;
-      int owner = -1;
-      for (int t = 0; t < PICK_THREADS && owner < 0; ++t) {
-        if (before + part[t] > goal) owner = t;
-        else before += part[t];
-      }
-      if (owner < 0)                             // rounding left the goal at the end: the last that has something
-        for (int t = PICK_THREADS - 1; t >= 0 && owner < 0; --t)
-          if (part[t] > 0.0) { owner = t; before = -1.0; }
-      s_owner = owner;
-      s_before = before;
-      s_total = goal;
-    }
-    __syncthreads();
-    if (s_owner >= 0) {
-      if ((int)threadIdx.x == s_owner) {
-        double run = s_before;
+#pragma unroll 4
+    for (int i = lo + lane; i < hi; i += 32) mine += left(i);
+    const double block = block_sum(mine, s_sums);
+    const double all = over_cluster(block, ahead);
+    if (!(all > 0.0) && whole == 0) continue;
+    const double goal = (double)p.uniforms[2 * (int64_t)r + 1] * all;
+    // the block whose share the goal falls into: the sums ahead of the blocks ascend (rounding cannot leave it out: the last block with
+    // something ends at `all`, which is above the goal; a number that is not below 1 takes that block too)
+    const bool mine_holds = block > 0.0 && ahead + block > goal && !(ahead > goal);
+    const bool last_holds = !(all > goal) && block > 0.0 && !(ahead + block < all);
+    if (mine_holds || last_holds) {
+      double before = ahead;
+      const int w = first_over(lane < PICK_WARPS ? s_sums[lane] : 0.0, PICK_WARPS, goal, before);
+      if (warp == w) {
+        // 32 pieces of the warp's share, a lane each; then the elements of one piece
+        const int piece = per_warp / 32;
+        const int a = min(hi, lo + lane * piece), e = min(hi, a + piece);
+        double sum = 0.0;
+        for (int i = a; i < e; ++i) sum += left(i);
+        const int x = first_over(sum, 32, goal, before);
         int pick = -1;
-        for (int i = lo; i < hi; ++i) {
-          const double w = left(i);
-          if (w > 0.0) pick = i;
-          if (s_before >= 0.0) {
-            run += w;
-            if (run > s_total) break;
-          }
+        const int from = min(hi, lo + x * piece), to = min(hi, from + piece);
+        for (int i0 = from; i0 < to && x >= 0; i0 += 32) {
+          const double v = i0 + lane < to ? left(i0 + lane) : 0.0;
+          double upto = before;
+          const int y = first_over(v, 32, goal, upto);
+          const double one = __shfl_sync(0xffffffffu, v, y < 0 ? 0 : y);
+          if (y >= 0) pick = i0 + y;
+          if (y >= 0 && upto + one > goal) break;
+          double run = before;                   // (all 32, in order)
+          for (int k = 0; k < 32; ++k) run += __shfl_sync(0xffffffffu, v, k);
+          before = run;
         }
-        tokens[s_count] = pick;
+        if (lane == 0) tokens[taken] = pick;
       }
-      return;
     }
-    __syncthreads();
+    break;
+  }
+  if (blocks > 1) {                              // nobody's shared memory goes away while another block reads it
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
 }
 
@@ -197,12 +370,32 @@ RB_EXPORT int rb_verify(int* accepted, int* tokens, const float* logits, int64_t
                         const int* first_row, const int* drafts, const float* temperature, const float* uniforms, int B, int R, int V,
                         int most, void* scratch, cudaStream_t stream) {
   if (B == 0) return 0;
-  RB_REQUIRE(V > 0 && R >= 0 && most >= 0, "rb_verify: %d rows of %d logits, %d drafts", R, V, most);
+  RB_REQUIRE(V > 0 && R >= 0 && most >= 0 && B <= 65535, "rb_verify: %d sequences, %d rows of %d logits, %d drafts", B, R, V, most);
   Verify p;
   p.accepted = accepted; p.tokens = tokens; p.logits = logits; p.stride = stride; p.probs = probs; p.probs_stride = probs_stride;
   p.first_row = first_row; p.drafts = drafts; p.temperature = temperature; p.uniforms = uniforms; p.stats = (Stat*)scratch;
   p.B = B; p.R = R; p.V = V; p.most = most; p.chunks = (V + CHUNK - 1) / CHUNK;
-  if (R > 0) RB_LAUNCH("rb_verify (rows)", (verify_stats_kernel), dim3(R, p.chunks), THREADS, 0, stream, p);
-  RB_LAUNCH("rb_verify (pick)", (verify_pick_kernel), B, PICK_THREADS, 0, stream, p);
+  if (R > 0) {
+    const bool vec = stride % 4 == 0 && ((uintptr_t)logits & 15) == 0;
+    if (vec) RB_LAUNCH("rb_verify (rows)", (verify_rows_kernel<true>), dim3(R, p.chunks), THREADS, 0, stream, p);
+    else RB_LAUNCH("rb_verify (rows)", (verify_rows_kernel<false>), dim3(R, p.chunks), THREADS, 0, stream, p);
+  }
+  // blocks of a cluster: about 16,384 logits each, 8 at most
+  int blocks = 1;
+  while (blocks < 8 && V > 16384 * blocks) blocks *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks, B, 1);
+  cfg.blockDim = dim3(PICK_THREADS, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = rb_pdl_enabled() ? 2 : 1;
+  RB_CUDA(cudaLaunchKernelEx(&cfg, verify_pick_kernel, p, blocks));
   return 0;
 }
