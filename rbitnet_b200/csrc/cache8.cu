@@ -33,6 +33,51 @@ __device__ __forceinline__ float of_code(uint8_t c) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
 }
 
+// Sixteen codes (16 bytes) times a scale as sixteen bfloat16 values (32 bytes); exact: a code has four binary digits.
+__device__ __forceinline__ void values16(const uint4& codes, float scale, uint4 (&out)[2]) {
+  const uint32_t in[4] = {codes.x, codes.y, codes.z, codes.w};
+  uint32_t to[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(in[i >> 1] >> (i & 1) * 16), __NV_E4M3);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * scale, f.y * scale);
+    to[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  out[0] = make_uint4(to[0], to[1], to[2], to[3]);
+  out[1] = make_uint4(to[4], to[5], to[6], to[7]);
+}
+// Eight values times a power of two as codes (8 bytes).
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float inv) {
+  uint32_t out[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * inv, v[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * inv, v[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+    out[i] = lo | hi << 16;
+  }
+  return make_uint2(out[0], out[1]);
+}
+// Codes of `count` values brought to another scale by `n` threads: count is a multiple of 16, the address of 16 bytes.
+__device__ __forceinline__ void rescale16(uint8_t* codes, int count, float ratio, int me, int n) {
+  for (int i = me; i < count / 16; i += n) {
+    uint4 c = reinterpret_cast<uint4*>(codes)[i];
+    uint32_t* w = reinterpret_cast<uint32_t*>(&c);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      uint32_t two[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[x] >> h * 16), __NV_E4M3);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+        two[h] = __nv_cvt_float2_to_fp8x2(make_float2(f.x * ratio, f.y * ratio), __NV_SATFINITE, __NV_E4M3);
+      }
+      w[x] = two[0] | two[1] << 16;
+    }
+    reinterpret_cast<uint4*>(codes)[i] = c;
+  }
+}
+
 struct Append8 {
   __nv_bfloat16* q_out;          // [T, H, D]
   const __nv_bfloat16* qkv;      // [T, (H + 2 Kh) D], rows qkv_stride apart (H D without writing)
@@ -113,6 +158,209 @@ __global__ void __launch_bounds__(256) append8_kernel(Append8 p) {
   }
 }
 
+// Eight pairs of a row: where their first and second values lie (two 16-byte pieces), and the rotation of them.
+__device__ __forceinline__ int piece_a(const Append8& p, int e) { return p.interleaved ? 16 * e : 8 * e; }
+__device__ __forceinline__ int piece_b(const Append8& p, int e) { return p.interleaved ? 16 * e + 8 : p.cache.head_dim / 2 + 8 * e; }
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// sc: the token's (sine, cosine) of pairs 8e .. 8e + 7
+__device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const float2* sc, int interleaved) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 t = sc[i];
+    // interleaved: pair i is (2i, 2i + 1) of the sixteen values
+    float& x = interleaved ? (i < 4 ? a[2 * i] : b[2 * i - 8]) : a[i];
+    float& y = interleaved ? (i < 4 ? a[2 * i + 1] : b[2 * i - 7]) : b[i];
+    const float x0 = x, x1 = y;
+    x = x0 * t.y - x1 * t.x;
+    y = x0 * t.x + x1 * t.y;
+  }
+}
+__device__ __forceinline__ float largest8(const float (&a)[8], const float (&b)[8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fabsf(a[i]), fabsf(b[i])));
+  return m;
+}
+
+// Heads of a multiple of 16 values (up to 128 SPAN), turned whole, rows on 16 bytes: a block of threads per (tile, kv head) as above, but a
+// thread takes eight pairs at a time (16-byte loads and stores), a token's sines and cosines are made once for the query heads
+// and the key, and the tile's keys and values stay in registers between the largest value and the codes.
+// A tile of 64 tokens reads 64 (G + 2) D values; 8,192 tokens of 32 heads on 8 kv heads of 128 are 1,024 blocks.
+template <int SPAN>
+__global__ void __launch_bounds__(256) append8_tiles_kernel(Append8 p) {
+  rb_pdl_launch_dependents();
+  extern __shared__ float2 turns[];              // [tokens of the tile][D / 2] (sine, cosine)
+  __shared__ float tops[2][8];
+  const int D = p.cache.head_dim, Kh = p.cache.n_kv_heads, G = p.H / Kh, half = D / 2, pieces = D / 16;
+  const int kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tok0 = p.tile_tok0[blockIdx.x], n = p.tile_ntok[blockIdx.x];
+  const int slot = p.tok_slot[tok0], pos0 = p.tok_pos[tok0];
+  rb_pdl_wait();
+  const __nv_bfloat16* rows = p.qkv + (int64_t)tok0 * p.qkv_stride;
+  // the keys and values are asked for first
+  uint4 kv[2][SPAN][2];
+  if (p.write_kv) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < SPAN; ++i) {
+        const int item = i * 256 + threadIdx.x, tok = item / pieces, e = item % pieces;
+        kv[s][i][0] = kv[s][i][1] = make_uint4(0, 0, 0, 0);
+        if (tok < n) {
+          const __nv_bfloat16* src = rows + (int64_t)tok * p.qkv_stride + (int64_t)(p.H + s * Kh + kvh) * D;
+          kv[s][i][0] = *reinterpret_cast<const uint4*>(src + piece_a(p, e));
+          kv[s][i][1] = *reinterpret_cast<const uint4*>(src + piece_b(p, e));
+        }
+      }
+  }
+  for (int i = threadIdx.x; p.rot_dim && i < n * half; i += 256) {
+    float sn, cs;
+    angle_sincos(pos0 + i / half, (double)p.inv_freq[i % half], 1.0f, &sn, &cs);
+    turns[i] = make_float2(sn, cs);
+  }
+  __syncthreads();
+  float2 top = make_float2(0.f, 0.f);
+  if (p.write_kv) {
+#pragma unroll
+    for (int i = 0; i < SPAN; ++i) {
+      const int item = i * 256 + threadIdx.x, tok = item / pieces, e = item % pieces;
+      float a[8], b[8];
+      unpack8(kv[1][i][0], a); unpack8(kv[1][i][1], b);
+      top.y = fmaxf(top.y, largest8(a, b));
+      if (tok < n) {
+        unpack8(kv[0][i][0], a); unpack8(kv[0][i][1], b);
+        if (p.rot_dim) turn8(a, b, turns + tok * half + 8 * e, p.interleaved);
+        top.x = fmaxf(top.x, largest8(a, b));
+      }
+    }
+    top.x = rb_warp_max(top.x);
+    top.y = rb_warp_max(top.y);
+    if (lane == 0) { tops[0][warp] = top.x; tops[1][warp] = top.y; }
+  }
+  // the query heads, while the largest values meet
+  for (int item = threadIdx.x; item < n * G * pieces; item += 256) {
+    const int e = item % pieces, th = item / pieces, tok = th / G, head = kvh * G + th % G;
+    const __nv_bfloat16* src = rows + (int64_t)tok * p.qkv_stride + (int64_t)head * D;
+    __nv_bfloat16* dst = p.q_out + ((int64_t)(tok0 + tok) * p.H + head) * D;
+    float a[8], b[8];
+    unpack8(*reinterpret_cast<const uint4*>(src + piece_a(p, e)), a);
+    unpack8(*reinterpret_cast<const uint4*>(src + piece_b(p, e)), b);
+    if (p.rot_dim) turn8(a, b, turns + tok * half + 8 * e, p.interleaved);
+    *reinterpret_cast<uint4*>(dst + piece_a(p, e)) = pack8(a);
+    *reinterpret_cast<uint4*>(dst + piece_b(p, e)) = pack8(b);
+  }
+  if (!p.write_kv) return;
+  const int before = pos0 % p.block;             // positions that the block holds already
+  const int64_t at = rb_page_offset(p.cache, slot, pos0, kvh) - (int64_t)before * D;       // of the block's first code
+  const int64_t unit = at / ((int64_t)p.block * D);
+  const float old_k = before > 0 ? p.k_scale[unit] : 0.f, old_v = before > 0 ? p.v_scale[unit] : 0.f;
+  __syncthreads();                               // (everybody has the old scales, too)
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    float amax = tops[s][0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) amax = fmaxf(amax, tops[s][w]);
+    const float old = s ? old_v : old_k, now = fmaxf(old, scale_for(amax)), inv = 1.0f / now;
+    uint8_t* codes = (uint8_t*)(s ? p.cache.v : p.cache.k) + at;
+    if (old < now) rescale16(codes, before * D, old * inv, threadIdx.x, 256);
+#pragma unroll
+    for (int i = 0; i < SPAN; ++i) {
+      const int item = i * 256 + threadIdx.x, tok = item / pieces, e = item % pieces;
+      if (tok < n) {
+        float a[8], b[8];
+        unpack8(kv[s][i][0], a); unpack8(kv[s][i][1], b);
+        if (s == 0 && p.rot_dim) turn8(a, b, turns + tok * half + 8 * e, p.interleaved);
+        uint8_t* to = codes + (before + tok) * D;
+        *reinterpret_cast<uint2*>(to + piece_a(p, e)) = codes8(a, inv);
+        *reinterpret_cast<uint2*>(to + piece_b(p, e)) = codes8(b, inv);
+      }
+    }
+    if (threadIdx.x == 0) (s ? p.v_scale : p.k_scale)[unit] = now;
+  }
+}
+
+// The same for one token a tile (a decode step): a warp per (row, kv head), up to 8 kv heads a block; the sines and cosines once a block.
+// What bounds it is latency: a wait, the row, the old scales, the codes.
+__global__ void __launch_bounds__(256) append8_step_kernel(Append8 p) {
+  rb_pdl_launch_dependents();
+  extern __shared__ float2 turns[];              // [D / 2]
+  const int D = p.cache.head_dim, Kh = p.cache.n_kv_heads, G = p.H / Kh, half = D / 2, pieces = D / 16;
+  const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y * (blockDim.x >> 5) + warp;
+  const int slot = p.tok_slot[row], pos = p.tok_pos[row];
+  for (int i = threadIdx.x; p.rot_dim && i < half; i += blockDim.x) {       // (positions and frequencies: not written by the kernel before)
+    float sn, cs;
+    angle_sincos(pos, (double)p.inv_freq[i], 1.0f, &sn, &cs);
+    turns[i] = make_float2(sn, cs);
+  }
+  const bool mine = kvh < Kh;
+  int64_t at = 0, unit = 0;
+  const int before = pos % p.block;
+  if (mine && p.write_kv) {
+    at = rb_page_offset(p.cache, slot, pos, kvh) - (int64_t)before * D;
+    unit = at / ((int64_t)p.block * D);
+  }
+  rb_pdl_wait();
+  const __nv_bfloat16* src = p.qkv + (int64_t)row * p.qkv_stride;
+  // items: the key's pieces, the value's, then the query heads'; the first two streams lie in the first turn (D <= 256)
+  const int items = (p.write_kv ? 2 * pieces : 0) + G * pieces;
+  const int ahead = p.write_kv ? 2 * pieces : 0;
+  float old_k = 0.f, old_v = 0.f;
+  if (mine && p.write_kv && before > 0) { old_k = p.k_scale[unit]; old_v = p.v_scale[unit]; }
+  __syncthreads();
+  if (!mine) return;
+  for (int base = 0; base < items; base += 32) {
+    const int item = base + lane;
+    const bool is_k = item < ahead && item < pieces, is_v = item < ahead && !is_k, on = item < items;
+    const int e = item % pieces;
+    const int64_t head = is_k ? p.H + kvh : is_v ? p.H + Kh + kvh : kvh * G + (item - ahead) / pieces;
+    float a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+    if (on) {
+      unpack8(*reinterpret_cast<const uint4*>(src + head * D + piece_a(p, e)), a);
+      unpack8(*reinterpret_cast<const uint4*>(src + head * D + piece_b(p, e)), b);
+      if (!is_v && p.rot_dim) turn8(a, b, turns + 8 * e, p.interleaved);
+    }
+    if (on && !is_k && !is_v) {
+      __nv_bfloat16* dst = p.q_out + ((int64_t)row * p.H + head) * D;
+      *reinterpret_cast<uint4*>(dst + piece_a(p, e)) = pack8(a);
+      *reinterpret_cast<uint4*>(dst + piece_b(p, e)) = pack8(b);
+    }
+    if (base == 0 && p.write_kv) {
+      const float big = largest8(a, b);
+      const float top_k = rb_warp_max(is_k ? big : 0.f), top_v = rb_warp_max(is_v ? big : 0.f);
+      const float now_k = fmaxf(old_k, scale_for(top_k)), now_v = fmaxf(old_v, scale_for(top_v));
+      uint8_t* k = (uint8_t*)p.cache.k + at;
+      uint8_t* v = (uint8_t*)p.cache.v + at;
+      if (old_k < now_k) rescale16(k, before * D, old_k / now_k, lane, 32);
+      if (old_v < now_v) rescale16(v, before * D, old_v / now_v, lane, 32);
+      if (is_k || is_v) {
+        const float inv = 1.0f / (is_k ? now_k : now_v);
+        uint8_t* to = (is_k ? k : v) + before * D;
+        *reinterpret_cast<uint2*>(to + piece_a(p, e)) = codes8(a, inv);
+        *reinterpret_cast<uint2*>(to + piece_b(p, e)) = codes8(b, inv);
+      }
+      if (lane == 0) { p.k_scale[unit] = now_k; p.v_scale[unit] = now_v; }
+    }
+  }
+}
+
 // The values of whole pages: item i is (slot, page of the sequence, positions in use); what lies behind those is zero.
 __global__ void __launch_bounds__(256) cache8_values_kernel(__nv_bfloat16* k_out, __nv_bfloat16* v_out, RbPagedLayer c, const float* k_scale,
                                                            const float* v_scale, const int* items, int block) {
@@ -129,6 +377,27 @@ __global__ void __launch_bounds__(256) cache8_values_kernel(__nv_bfloat16* k_out
     const bool in = pos < used;
     k_out[to + idx] = __float2bfloat16_rn(in ? of_code(k[idx]) * k_scale[s + pos / block] : 0.f);
     v_out[to + idx] = __float2bfloat16_rn(in ? of_code(v[idx]) * v_scale[s + pos / block] : 0.f);
+  }
+}
+
+// The same for heads of a multiple of 16 values: a thread turns 16 codes at a time.
+__global__ void __launch_bounds__(256) cache8_values16_kernel(__nv_bfloat16* k_out, __nv_bfloat16* v_out, RbPagedLayer c, const float* k_scale,
+                                                             const float* v_scale, const int* items, int block) {
+  rb_pdl_launch_dependents();
+  const int i = blockIdx.x, kvh = blockIdx.y, D = c.head_dim, n = c.page_size * D;
+  const int slot = items[3 * i], page = items[3 * i + 1], used = items[3 * i + 2];
+  rb_pdl_wait();
+  const int64_t at = rb_page_offset(c, slot, page * c.page_size, kvh), to = ((int64_t)i * c.n_kv_heads + kvh) * n;
+  const uint8_t* in = (const uint8_t*)(blockIdx.z ? c.v : c.k) + at;
+  const float* scale = (blockIdx.z ? v_scale : k_scale) + at / ((int64_t)block * D);
+  __nv_bfloat16* out = (blockIdx.z ? v_out : k_out) + to;
+#pragma unroll 2
+  for (int idx = threadIdx.x * 16; idx < n; idx += 256 * 16) {
+    const int pos = idx / D;
+    uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (pos < used) values16(*reinterpret_cast<const uint4*>(in + idx), scale[block == c.page_size ? 0 : pos / block], v);
+    *reinterpret_cast<uint4*>(out + idx) = v[0];
+    *reinterpret_cast<uint4*>(out + idx + 8) = v[1];
   }
 }
 
@@ -159,6 +428,25 @@ RB_EXPORT int rb_append8(void* q_out, const void* qkv, int64_t qkv_stride, const
   p.cache = RbPagedLayer{cache_k, cache_v, page_table, max_pages, page_size, Kh, D};
   p.k_scale = k_scale; p.v_scale = v_scale;
   p.block = block; p.H = H; p.write_kv = write_kv; p.interleaved = interleaved; p.rot_dim = rot_dim;
+  const uintptr_t bases = (uintptr_t)q_out | (uintptr_t)qkv | (uintptr_t)cache_k | (uintptr_t)cache_v;
+  if (D % 16 == 0 && D <= 256 && (rot_dim == D || rot_dim == 0) && qkv_stride % 8 == 0 && (bases & 15) == 0) {
+    if (!tile_tok0) {
+      const int warps = Kh < 8 ? Kh : 8;
+      RB_LAUNCH("rb_append8 (step)", (append8_step_kernel), dim3(n_tiles, (Kh + warps - 1) / warps), warps * 32, (size_t)D / 2 * 8, stream, p);
+      return 0;
+    }
+    static RbOncePerDevice tiled;
+    if (tiled.first()) {
+      RB_CUDA(cudaFuncSetAttribute(append8_tiles_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_BLOCK * 32 * 8));
+      RB_CUDA(cudaFuncSetAttribute(append8_tiles_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_BLOCK * 64 * 8));
+      RB_CUDA(cudaFuncSetAttribute(append8_tiles_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_BLOCK * 128 * 8));
+    }
+    const size_t turns = (size_t)block * D / 2 * 8;
+    if (D <= 64) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<1>), dim3(n_tiles, Kh), 256, turns, stream, p);
+    else if (D <= 128) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<2>), dim3(n_tiles, Kh), 256, turns, stream, p);
+    else RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<4>), dim3(n_tiles, Kh), 256, turns, stream, p);
+    return 0;
+  }
   static RbOncePerDevice configured;
   if (configured.first())
     RB_CUDA(cudaFuncSetAttribute(append8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_BLOCK * 512 * 4));
@@ -175,6 +463,11 @@ RB_EXPORT int rb_cache8_values(void* k_out, void* v_out, const int* items, int n
   const int block = rb_cache8_block(page_size);
   RB_REQUIRE(block > 0 && Kh > 0 && Kh <= 65535 && D > 0, "rb_cache8_values: bad sizes page=%d Kh=%d D=%d", page_size, Kh, D);
   RbPagedLayer c{cache_k, cache_v, page_table, max_pages, page_size, Kh, D};
+  if (D % 16 == 0 && (((uintptr_t)k_out | (uintptr_t)v_out | (uintptr_t)cache_k | (uintptr_t)cache_v) & 15) == 0) {
+    RB_LAUNCH("rb_cache8_values", (cache8_values16_kernel), dim3(n, Kh, 2), 256, 0, stream, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, c, k_scale,
+              v_scale, items, block);
+    return 0;
+  }
   RB_LAUNCH("rb_cache8_values", (cache8_values_kernel), dim3(n, Kh), 256, 0, stream, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, c, k_scale, v_scale,
             items, block);
   return 0;

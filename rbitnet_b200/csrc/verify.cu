@@ -51,29 +51,26 @@ __device__ __forceinline__ float weight_f32(float z, float m, float c) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((z - m) * c));
   return z == m ? 1.f : y;
 }
-// 2^x for x <= 0: the nearest whole number goes to the exponent, Taylor's series of e^(r ln 2) for the rest, |r| <= 1/2 (the first
-// term left out is 4e-18)
-__device__ __forceinline__ double weight(float z, float m, double c) {
+// In float64 2^x, x = (z - m) c <= 0, is 2^k times 2^(j / 64) from a table (64 values a block, exp2's) times the first six terms of
+// the series of 2^r, |r| <= 1/128 (the first term left out is 4e-17 of the result): a third of the multiply-adds of a series alone,
+// and float64 is the slow unit here.
+__device__ __forceinline__ double weight(float z, float m, double c, const double* table) {
   if (z == m) return 1.0;
   const double x = ((double)z - (double)m) * c;
   if (!(x > -1021.0)) return 0.0;
-  const double whole = x + 6755399441055744.0;   // 1.5 * 2^52: rounds to whole numbers, which are its low bits
-  const double t = (x - (whole - 6755399441055744.0)) * 0.69314718055994530942;
-  double e = 1.0 / 6227020800.0;
-  e = fma(e, t, 1.0 / 479001600.0);
-  e = fma(e, t, 1.0 / 39916800.0);
-  e = fma(e, t, 1.0 / 3628800.0);
-  e = fma(e, t, 1.0 / 362880.0);
-  e = fma(e, t, 1.0 / 40320.0);
-  e = fma(e, t, 1.0 / 5040.0);
-  e = fma(e, t, 1.0 / 720.0);
-  e = fma(e, t, 1.0 / 120.0);
+  const double whole = x + 105553116266496.0;    // 1.5 * 2^46: rounds to 64ths, whose number is the low bits
+  const double t = (x - (whole - 105553116266496.0)) * 0.69314718055994530942;
+  const int n = __double2loint(whole);
+  double e = 1.0 / 120.0;
   e = fma(e, t, 1.0 / 24.0);
   e = fma(e, t, 1.0 / 6.0);
   e = fma(e, t, 0.5);
   e = fma(e, t, 1.0);
-  e = fma(e, t, 1.0);
-  return __hiloint2double(__double2hiint(e) + (__double2loint(whole) << 20), __double2loint(e));
+  e = fma(e * t, table[n & 63], table[n & 63]);
+  return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
+}
+__device__ __forceinline__ void make_table(double* table) {
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
 }
 __device__ __forceinline__ double inverse_temperature(float temp) { return 1.4426950408889634074 / (double)temp; }
 
@@ -162,27 +159,30 @@ __device__ __forceinline__ double block_sum(double v, double* s) {
   return all;
 }
 
-// The first of n values (a lane has the lane-th) at which the running sum after `before` exceeds `goal`, else the last above zero (else -1);
-// `before` becomes the sum ahead of it.  All lanes get both.
-__device__ __forceinline__ int first_over(double v, int n, double goal, double& before) {
+// The first of the lanes' values at which the running sum after `before` exceeds `goal`, else the last above zero (else -1); `before` becomes
+// the sum ahead of it, and `over` whether it exceeds.  All lanes get the same.
+__device__ __forceinline__ int first_over(double v, double goal, double& before, bool& over) {
   const int lane = threadIdx.x & 31;
-  double run = before;
-  int found = -1, last = -1;
-  double ahead = before, ahead_of_last = before;
-  for (int i = 0; i < n; ++i) {
-    const double x = __shfl_sync(0xffffffffu, v, i);
-    if (x > 0.0) { last = i; ahead_of_last = run; }
-    if (found < 0 && run + x > goal) { found = i; ahead = run; }
-    run += x;
+  double upto = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
   }
-  (void)lane;
-  before = found >= 0 ? ahead : ahead_of_last;
-  return found >= 0 ? found : last;
+  const uint32_t past = __ballot_sync(0xffffffffu, before + upto > goal && v > 0.0), some = __ballot_sync(0xffffffffu, v > 0.0);
+  over = past != 0;
+  const int at = over ? __ffs(past) - 1 : 31 - __clz(some);
+  if (at < 0) return -1;
+  before += __shfl_sync(0xffffffffu, upto - v, at);
+  return at;
 }
 
-// A cluster per sequence: block c has logits c * share .. of the row whose token is taken, a warp a PICK_WARPS-th of those.
+// A cluster per sequence: block c has logits c * share .. of the row whose token is taken, a warp a PICK_WARPS-th of those, `items` times 32.
+// ITEMS > 0: that many at most, and their weights stay in registers between the sums and the walk; 0: any number, made again.
+template <int ITEMS>
 __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int blocks) {
   rb_pdl_launch_dependents();
+  __shared__ double table[64];
   __shared__ double s_sums[PICK_WARPS];          // what the block's warps have
   __shared__ double s_shown[2];                  // what the cluster's blocks read
   __shared__ int s_found[PICK_WARPS], s_args[PICK_WARPS];
@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int
   __shared__ int s_n, s_row, s_arg;
   __shared__ float s_m;
   const int rank = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  make_table(table);
   rb_pdl_wait();
   // (rows outside the logits, which only a wrong first_row can name, are left out)
   const int r0 = min(max(p.first_row[b], 0), p.R), r1 = min(p.first_row[b + 1], p.R);
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int
   auto total_of = [&](int r, float m) {          // a row's float64 sum, by the whole block
     const float* z = p.logits + (int64_t)r * p.stride;
     double mine = 0.0;
-    for (int i = threadIdx.x; i < p.V; i += PICK_THREADS) mine += weight(clean(z[i]), m, c);
+    for (int i = threadIdx.x; i < p.V; i += PICK_THREADS) mine += weight(clean(z[i]), m, c, table);
     return block_sum(mine, s_sums);
   };
   // ---- the drafts, PICK_WARPS rows at a time, a warp each: 1 accepted, 0 not, 2 open
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int
         if (greedy) {
           if (one.max == m) arg = min(arg, temp > 0.f ? 0 : one.arg);
         } else if (one.max > -INFINITY) {
-          total += (double)one.sum * weight(one.max, m, c);
+          total += (double)one.sum * weight(one.max, m, c, table);
         }
       }
       total = warp_sum(total);
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int
         if (greedy) {
           found = left < (d == arg ? 1.0 : 0.0) ? 1 : 0;
         } else {
-          const double w = weight(clean(p.logits[(int64_t)r * p.stride + d]), m, c), side = left * total;
+          const double w = weight(clean(p.logits[(int64_t)r * p.stride + d]), m, c, table), side = left * total;
           found = side * (1.0 + OPEN) < w ? 1 : (side * (1.0 - OPEN) >= w ? 0 : 2);
         }
       }
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int
         const int row = at + n, d = p.drafts[row];
         const double q = p.probs ? (double)p.probs[(int64_t)row * p.probs_stride + d] : 1.0;
         const double total = total_of(row, s_maxima[n]);
-        f = (double)p.uniforms[2 * (int64_t)row] * q * total < weight(clean(p.logits[(int64_t)row * p.stride + d]), s_maxima[n], c) ? 1 : 0;
+        f = (double)p.uniforms[2 * (int64_t)row] * q * total < weight(clean(p.logits[(int64_t)row * p.stride + d]), s_maxima[n], c, table) ? 1 : 0;
       }
       if (f == 0) break;
       if (threadIdx.x == 0) {
@@ -298,25 +299,47 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int
     ++turn;
     return all;
   };
-  double total = 1.0, ahead = 0.0;
+  const int items = per_warp / 32;
+  double total = 1.0, ahead = 0.0, kept[ITEMS > 0 ? ITEMS : 1];
+  auto made = [&](int i) -> double {             // the weight of the lane's i-th logit
+    const int at = lo + i * 32 + lane;
+    return at < hi ? weight(clean(z[at]), m, c, table) : 0.0;
+  };
+  if (ITEMS > 0) {
+    float zs[ITEMS > 0 ? ITEMS : 1];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) zs[i] = lo + i * 32 + lane < hi ? clean(z[lo + i * 32 + lane]) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) kept[i] = weight(zs[i], m, c, table);
+  }
   if (q) {
     double mine = 0.0;
+    if (ITEMS > 0) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) mine += kept[i];
+    } else {
 #pragma unroll 4
-    for (int i = lo + lane; i < hi; i += 32) mine += weight(clean(z[i]), m, c);
+      for (int i = 0; i < items; ++i) mine += made(i);
+    }
     total = over_cluster(block_sum(mine, s_sums), ahead);
   }
   // whole: from p itself, where p - q has nothing left
   for (int whole = judged ? 0 : 1; whole < 2; ++whole) {
     // (p - q) times the sum of the weights: without q nothing is divided, so that equal logits are equal steps exactly
-    auto left = [&](int i) -> double {
-      const double w = weight(clean(z[i]), m, c);
-      if (whole) return w;
-      if (q) return fmax(w - (double)q[i] * total, 0.0);
-      return i == d ? 0.0 : w;
+    auto left = [&](double w, int i) -> double {
+      const int at = lo + i * 32 + lane;
+      if (whole || at >= hi) return w;
+      if (q) return fmax(w - (double)q[at] * total, 0.0);
+      return at == d ? 0.0 : w;
     };
     double mine = 0.0;
+    if (ITEMS > 0) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) mine += left(kept[i], i);
+    } else {
 #pragma unroll 4
-    for (int i = lo + lane; i < hi; i += 32) mine += left(i);
+      for (int i = 0; i < items; ++i) mine += left(made(i), i);
+    }
     const double block = block_sum(mine, s_sums);
     const double all = over_cluster(block, ahead);
     if (!(all > 0.0) && whole == 0) continue;
@@ -327,26 +350,31 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int
     const bool last_holds = !(all > goal) && block > 0.0 && !(ahead + block < all);
     if (mine_holds || last_holds) {
       double before = ahead;
-      const int w = first_over(lane < PICK_WARPS ? s_sums[lane] : 0.0, PICK_WARPS, goal, before);
+      bool over;
+      const int w = first_over(lane < PICK_WARPS ? s_sums[lane] : 0.0, goal, before, over);
       if (warp == w) {
-        // 32 pieces of the warp's share, a lane each; then the elements of one piece
-        const int piece = per_warp / 32;
-        const int a = min(hi, lo + lane * piece), e = min(hi, a + piece);
-        double sum = 0.0;
-        for (int i = a; i < e; ++i) sum += left(i);
-        const int x = first_over(sum, 32, goal, before);
+        // rows of 32 logits in turn: the one that the goal falls into, and in it the token (else the last that has something)
         int pick = -1;
-        const int from = min(hi, lo + x * piece), to = min(hi, from + piece);
-        for (int i0 = from; i0 < to && x >= 0; i0 += 32) {
-          const double v = i0 + lane < to ? left(i0 + lane) : 0.0;
-          double upto = before;
-          const int y = first_over(v, 32, goal, upto);
-          const double one = __shfl_sync(0xffffffffu, v, y < 0 ? 0 : y);
-          if (y >= 0) pick = i0 + y;
-          if (y >= 0 && upto + one > goal) break;
-          double run = before;                   // (all 32, in order)
-          for (int k = 0; k < 32; ++k) run += __shfl_sync(0xffffffffu, v, k);
-          before = run;
+        bool done = false;
+        auto row = [&](double v, int i) {
+          if (done) return;
+          const uint32_t some = __ballot_sync(0xffffffffu, v > 0.0);
+          if (some == 0) return;
+          pick = lo + i * 32 + 31 - __clz(some);
+          const double sum = warp_sum(v);
+          if (before + sum > goal) {
+            double upto = before;
+            bool found;
+            const int y = first_over(v, goal, upto, found);
+            if (found) { pick = lo + i * 32 + y; done = true; }
+          }
+          before += sum;
+        };
+        if (ITEMS > 0) {
+#pragma unroll
+          for (int i = 0; i < ITEMS; ++i) row(left(kept[i], i), i);
+        } else {
+          for (int i = 0; i < items; ++i) row(left(made(i), i), i);
         }
         if (lane == 0) tokens[taken] = pick;
       }
@@ -380,9 +408,10 @@ RB_EXPORT int rb_verify(int* accepted, int* tokens, const float* logits, int64_t
     if (vec) RB_LAUNCH("rb_verify (rows)", (verify_rows_kernel<true>), dim3(R, p.chunks), THREADS, 0, stream, p);
     else RB_LAUNCH("rb_verify (rows)", (verify_rows_kernel<false>), dim3(R, p.chunks), THREADS, 0, stream, p);
   }
-  // blocks of a cluster: about 16,384 logits each, 8 at most
+  // blocks of a cluster: 8 logits a thread or more, 8 blocks at most; up to 32 a thread stay in registers
   int blocks = 1;
-  while (blocks < 8 && V > 16384 * blocks) blocks *= 2;
+  while (blocks < 8 && V > 8 * PICK_THREADS * blocks) blocks *= 2;
+  const int items = ((V + blocks - 1) / blocks + PICK_THREADS - 1) / PICK_THREADS;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks, B, 1);
   cfg.blockDim = dim3(PICK_THREADS, 1, 1);
@@ -396,6 +425,7 @@ RB_EXPORT int rb_verify(int* accepted, int* tokens, const float* logits, int64_t
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = rb_pdl_enabled() ? 2 : 1;
-  RB_CUDA(cudaLaunchKernelEx(&cfg, verify_pick_kernel, p, blocks));
+  auto kernel = items <= 8 ? verify_pick_kernel<8> : items <= 16 ? verify_pick_kernel<16> : items <= 32 ? verify_pick_kernel<32> : verify_pick_kernel<0>;
+  RB_CUDA(cudaLaunchKernelEx(&cfg, kernel, p, blocks));
   return 0;
 }
