@@ -23,7 +23,7 @@
 
 namespace {
 
-constexpr int CHUNK = 8192, THREADS = 256, PICK_WARPS = 16, PICK_THREADS = PICK_WARPS * 32;
+constexpr int CHUNK = 8192, THREADS = 256, PICK_WARPS = 16, PICK_THREADS = PICK_WARPS * 32, MOST_ITEMS = 512;
 constexpr double OPEN = 1.0 / 16384;             // float32 decides outside this share of the two sides
 
 struct Stat { float max, sum; int arg, unused; };
@@ -51,26 +51,26 @@ __device__ __forceinline__ float weight_f32(float z, float m, float c) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((z - m) * c));
   return z == m ? 1.f : y;
 }
-// In float64 2^x, x = (z - m) c <= 0, is 2^k times 2^(j / 64) from a table (64 values a block, exp2's) times the first six terms of
-// the series of 2^r, |r| <= 1/128 (the first term left out is 4e-17 of the result): a third of the multiply-adds of a series alone,
-// and float64 is the slow unit here.
+// In float64 2^x, x = (z - m) c <= 0, is 2^k times 2^(j / 256) from a table (exp2's values, made by every block) times the first
+// five terms of the series of e^(r ln 2), |r| <= 1/512 (the first left out is 4e-17 of the result): ten float64 operations.
+constexpr int TABLE = 256;
 __device__ __forceinline__ double weight(float z, float m, double c, const double* table) {
-  if (z == m) return 1.0;
-  const double x = ((double)z - (double)m) * c;
-  if (!(x > -1021.0)) return 0.0;
-  const double whole = x + 105553116266496.0;    // 1.5 * 2^46: rounds to 64ths, whose number is the low bits
-  const double t = (x - (whole - 105553116266496.0)) * 0.69314718055994530942;
+  const double x = ((double)z - (double)m) * c;  // (no branch: several of these run side by side)
+  const double whole = x + 26388279066624.0;     // 1.5 * 2^44: rounds to 256ths, whose number is the low bits
+  const double r = x - (whole - 26388279066624.0);
   const int n = __double2loint(whole);
-  double e = 1.0 / 120.0;
-  e = fma(e, t, 1.0 / 24.0);
-  e = fma(e, t, 1.0 / 6.0);
-  e = fma(e, t, 0.5);
-  e = fma(e, t, 1.0);
-  e = fma(e * t, table[n & 63], table[n & 63]);
-  return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
+  // ln 2 and its powers over the factorials
+  double e = fma(r, 0.00961812910762847716, 0.05550410866482157995);
+  e = fma(e, r, 0.24022650695910071233);
+  e = fma(e, r, 0.69314718055994530942);
+  const double t = table[n & (TABLE - 1)];
+  e = fma(e * r, t, t);
+  e = __hiloint2double(__double2hiint(e) + ((n >> 8) << 20), __double2loint(e));
+  e = x > -1021.0 ? e : 0.0;                     // (also where x is no number)
+  return z == m ? 1.0 : e;
 }
 __device__ __forceinline__ void make_table(double* table) {
-  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
+  for (int i = threadIdx.x; i < TABLE; i += blockDim.x) table[i] = exp2((double)i / TABLE);
 }
 __device__ __forceinline__ double inverse_temperature(float temp) { return 1.4426950408889634074 / (double)temp; }
 
@@ -177,12 +177,13 @@ __device__ __forceinline__ int first_over(double v, double goal, double& before,
   return at;
 }
 
-// A cluster per sequence: block c has logits c * share .. of the row whose token is taken, a warp a PICK_WARPS-th of those, `items` times 32.
-// ITEMS > 0: that many at most, and their weights stay in registers between the sums and the walk; 0: any number, made again.
-template <int ITEMS>
+// A cluster per sequence: block c has logits c * share .. of the row whose token is taken, a warp a PICK_WARPS-th of those, `items` rows of 32.
+// The weights are made again for every sum: kept in registers (32 a thread) they make the kernel a straight line of thousands of
+// instructions that each run once a warp, and fetching those took 200 us of 64 sequences over 128,256 logits.
 __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int blocks) {
   rb_pdl_launch_dependents();
-  __shared__ double table[64];
+  __shared__ double table[TABLE];
+  __shared__ double s_rows[MOST_ITEMS];           // sums of the rows of 32 logits of the warp's share that the token lies in
   __shared__ double s_sums[PICK_WARPS];          // what the block's warps have
   __shared__ double s_shown[2];                  // what the cluster's blocks read
   __shared__ int s_found[PICK_WARPS], s_args[PICK_WARPS];
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int
   const float* q = judged && p.probs ? p.probs + (int64_t)r * p.probs_stride : nullptr;
   const float m = s_m;
   const int per_warp = ((p.V + blocks - 1) / blocks + PICK_THREADS - 1) / PICK_THREADS * 32;       // a multiple of 32
-  const int lo = min((int64_t)p.V, ((int64_t)rank * PICK_WARPS + warp) * per_warp), hi = min(p.V, lo + per_warp);
+  const int lo = (int)min((int64_t)p.V, ((int64_t)rank * PICK_WARPS + warp) * per_warp);
   int turn = 0;
   // the cluster's sum of a block's values, and of those ahead of this block
   auto over_cluster = [&](double v, double& ahead) {
@@ -300,46 +301,48 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int
     return all;
   };
   const int items = per_warp / 32;
-  double total = 1.0, ahead = 0.0, kept[ITEMS > 0 ? ITEMS : 1];
-  auto made = [&](int i) -> double {             // the weight of the lane's i-th logit
-    const int at = lo + i * 32 + lane;
-    return at < hi ? weight(clean(z[at]), m, c, table) : 0.0;
+  double total = 0.0, ahead = 0.0;
+  // (p - q) times the sum of the weights: without q nothing is divided, so that equal logits are equal steps exactly.  `gone`: the token
+  // that is certain and was not accepted, or -1.  (A logit that is no number has the weight 0, as minus infinity has.)
+  auto left = [&](float zi, float qi, double less) -> double {
+    const double v = weight(zi, m, c, table) - (double)qi * less;
+    return v > 0.0 ? v : 0.0;
   };
-  if (ITEMS > 0) {
-    float zs[ITEMS > 0 ? ITEMS : 1];
+  auto logit = [&](int64_t at, int gone) -> float { return at < p.V && at != gone ? z[at] : -INFINITY; };
+  // the sum over the warp's share, a lane's part of it: eight rows of 32 are asked for together
+  auto share_sum = [&](int gone) -> double {
+    double sum = 0.0;
+    for (int i0 = 0; i0 < items; i0 += 8) {
+      float zi[8];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) zs[i] = lo + i * 32 + lane < hi ? clean(z[lo + i * 32 + lane]) : -INFINITY;
+      for (int i = 0; i < 8; ++i) zi[i] = i0 + i < items ? logit(lo + (i0 + i) * 32 + lane, gone) : -INFINITY;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) kept[i] = weight(zs[i], m, c, table);
-  }
-  if (q) {
-    double mine = 0.0;
-    if (ITEMS > 0) {
-#pragma unroll
-      for (int i = 0; i < ITEMS; ++i) mine += kept[i];
-    } else {
-#pragma unroll 4
-      for (int i = 0; i < items; ++i) mine += made(i);
+      for (int i = 0; i < 8; ++i) sum += weight(zi[i], m, c, table);
     }
-    total = over_cluster(block_sum(mine, s_sums), ahead);
-  }
+    return sum;
+  };
+  auto share_left = [&](double less) -> double {
+    double sum = 0.0;
+    for (int i0 = 0; i0 < items; i0 += 8) {
+      float zi[8], qi[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = lo + (i0 + i) * 32 + lane;
+        zi[i] = i0 + i < items ? logit(at, -1) : -INFINITY;
+        qi[i] = i0 + i < items && at < p.V ? q[at] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += left(zi[i], qi[i], less);
+    }
+    return sum;
+  };
+  if (q) total = over_cluster(block_sum(share_sum(-1), s_sums), ahead);
   // whole: from p itself, where p - q has nothing left
   for (int whole = judged ? 0 : 1; whole < 2; ++whole) {
-    // (p - q) times the sum of the weights: without q nothing is divided, so that equal logits are equal steps exactly
-    auto left = [&](double w, int i) -> double {
-      const int at = lo + i * 32 + lane;
-      if (whole || at >= hi) return w;
-      if (q) return fmax(w - (double)q[at] * total, 0.0);
-      return at == d ? 0.0 : w;
-    };
-    double mine = 0.0;
-    if (ITEMS > 0) {
-#pragma unroll
-      for (int i = 0; i < ITEMS; ++i) mine += left(kept[i], i);
-    } else {
-#pragma unroll 4
-      for (int i = 0; i < items; ++i) mine += left(made(i), i);
-    }
+    const float* qs = whole ? nullptr : q;
+    const double less = whole ? 0.0 : total;
+    const int gone = whole || q ? -1 : d;
+    const double mine = qs ? share_left(total) : share_sum(gone);
     const double block = block_sum(mine, s_sums);
     const double all = over_cluster(block, ahead);
     if (!(all > 0.0) && whole == 0) continue;
@@ -351,32 +354,29 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int
     if (mine_holds || last_holds) {
       double before = ahead;
       bool over;
+      // (every warp for itself) the warp whose share holds the goal; then all warps sum that share's rows of 32, and the first finds the
+      // row and the token
       const int w = first_over(lane < PICK_WARPS ? s_sums[lane] : 0.0, goal, before, over);
-      if (warp == w) {
-        // rows of 32 logits in turn: the one that the goal falls into, and in it the token (else the last that has something)
-        int pick = -1;
-        bool done = false;
-        auto row = [&](double v, int i) {
-          if (done) return;
-          const uint32_t some = __ballot_sync(0xffffffffu, v > 0.0);
-          if (some == 0) return;
-          pick = lo + i * 32 + 31 - __clz(some);
-          const double sum = warp_sum(v);
-          if (before + sum > goal) {
-            double upto = before;
-            bool found;
-            const int y = first_over(v, goal, upto, found);
-            if (found) { pick = lo + i * 32 + y; done = true; }
-          }
-          before += sum;
-        };
-        if (ITEMS > 0) {
-#pragma unroll
-          for (int i = 0; i < ITEMS; ++i) row(left(kept[i], i), i);
-        } else {
-          for (int i = 0; i < items; ++i) row(left(made(i), i), i);
+      const int64_t from = ((int64_t)rank * PICK_WARPS + w) * per_warp;
+      for (int i = warp; i < items; i += PICK_WARPS) {
+        const int64_t at = from + i * 32 + lane;
+        const double sum = warp_sum(left(logit(at, gone), qs && at < p.V ? qs[at] : 0.f, less));
+        if (lane == 0) s_rows[i] = sum;
+      }
+      __syncthreads();
+      if (warp == 0) {
+        int row = -1;
+        for (int i0 = 0; i0 < items; i0 += 32) {
+          double upto = before;
+          const double v = i0 + lane < items ? s_rows[i0 + lane] : 0.0;
+          const int y = first_over(v, goal, upto, over);
+          if (y >= 0) { row = i0 + y; ahead = upto; }
+          if (over) break;
+          before += warp_sum(v);
         }
-        if (lane == 0) tokens[taken] = pick;
+        const int64_t at = from + row * 32;
+        const int y = row >= 0 ? first_over(left(logit(at + lane, gone), qs && at + lane < p.V ? qs[at + lane] : 0.f, less), goal, ahead, over) : -1;
+        if (lane == 0) tokens[taken] = y >= 0 ? (int)at + y : -1;
       }
     }
     break;
@@ -398,6 +398,7 @@ RB_EXPORT int rb_verify(int* accepted, int* tokens, const float* logits, int64_t
                         const int* first_row, const int* drafts, const float* temperature, const float* uniforms, int B, int R, int V,
                         int most, void* scratch, cudaStream_t stream) {
   if (B == 0) return 0;
+  RB_REQUIRE(V <= 8 * PICK_THREADS * MOST_ITEMS, "rb_verify: %d logits a row, %d at most", V, 8 * PICK_THREADS * MOST_ITEMS);
   RB_REQUIRE(V > 0 && R >= 0 && most >= 0 && B <= 65535, "rb_verify: %d sequences, %d rows of %d logits, %d drafts", B, R, V, most);
   Verify p;
   p.accepted = accepted; p.tokens = tokens; p.logits = logits; p.stride = stride; p.probs = probs; p.probs_stride = probs_stride;
@@ -408,10 +409,9 @@ RB_EXPORT int rb_verify(int* accepted, int* tokens, const float* logits, int64_t
     if (vec) RB_LAUNCH("rb_verify (rows)", (verify_rows_kernel<true>), dim3(R, p.chunks), THREADS, 0, stream, p);
     else RB_LAUNCH("rb_verify (rows)", (verify_rows_kernel<false>), dim3(R, p.chunks), THREADS, 0, stream, p);
   }
-  // blocks of a cluster: 8 logits a thread or more, 8 blocks at most; up to 32 a thread stay in registers
+  // blocks of a cluster: 8 logits a thread or more, 8 blocks at most
   int blocks = 1;
   while (blocks < 8 && V > 8 * PICK_THREADS * blocks) blocks *= 2;
-  const int items = ((V + blocks - 1) / blocks + PICK_THREADS - 1) / PICK_THREADS;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks, B, 1);
   cfg.blockDim = dim3(PICK_THREADS, 1, 1);
@@ -425,7 +425,6 @@ RB_EXPORT int rb_verify(int* accepted, int* tokens, const float* logits, int64_t
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = rb_pdl_enabled() ? 2 : 1;
-  auto kernel = items <= 8 ? verify_pick_kernel<8> : items <= 16 ? verify_pick_kernel<16> : items <= 32 ? verify_pick_kernel<32> : verify_pick_kernel<0>;
-  RB_CUDA(cudaLaunchKernelEx(&cfg, kernel, p, blocks));
+  RB_CUDA(cudaLaunchKernelEx(&cfg, verify_pick_kernel, p, blocks));
   return 0;
 }
