@@ -8,6 +8,10 @@ A head's page is one contiguous [page_size, width] tile.  ``table[slot][i]`` is 
 that holds the slot's positions i*page_size .. (i+1)*page_size-1; the streams of a group
 share the table.
 
+A cache may be held in 8 bits (``dtype`` float8_e4m3fn): the pools hold codes, and beside each lies a tensor of float32 scales
+``[layer in group][page][head][block in page]``, one per block of positions (a whole page of up to 64, else 64); what they
+mean is said in csrc/cache8.cu.
+
 State area: for every schedule entry whose mixer declares a ``StateNeed``, a
 tensor [n_slots, *shape]; a slot's rows are zeroed when the slot is given out.
 The Llama decoder needs none, so the area is empty for it.
@@ -43,23 +47,34 @@ class CacheLayerView:
     scales: tuple = ()         # a cache held in 8 bits: per stream, float32 [n_pages, kv heads, blocks of a page]
 
 
+def scale_block(page_size: int) -> int:
+    """Positions that share a scale in pages of ``page_size`` of a cache held in 8 bits (-1: such pages are not taken)."""
+    return page_size if 0 < page_size <= 64 else (64 if page_size % 64 == 0 and page_size > 0 else -1)
+
+
 class CacheGroup:
     def __init__(self, need: CacheNeed, entries: List[int], n_pages: int, n_slots: int, max_pages: int,
                  page_size: int, dtype, device):
         self.need, self.entries = need, entries
         self.n_pages = n_pages
+        self.block = scale_block(page_size) if dtype == torch.float8_e4m3fn else 0
+        if self.block < 0:
+            raise ValueError(f"a cache held in 8 bits has pages of up to 64 positions or of a multiple of 64, not of {page_size}")
         self.pools = [torch.zeros((len(entries), n_pages, heads, page_size, width), dtype=dtype, device=device)
                       for heads, width in need.stream_shapes()]
+        self.scales = [torch.zeros((len(entries), n_pages, heads, page_size // self.block), dtype=torch.float32, device=device)
+                       for heads, _ in need.stream_shapes()] if self.block else []
         self.table_host = np.zeros((n_slots, max_pages), dtype=np.int32)
         self.table = torch.zeros((n_slots, max_pages), dtype=torch.int32, device=device)
         self.dirty = set()
 
     def bytes(self) -> int:
-        return sum(p.numel() * p.element_size() for p in self.pools)
+        return sum(p.numel() * p.element_size() for p in self.pools + self.scales)
 
     def bytes_per_position(self) -> int:
-        """What one cached position of one sequence holds in this group, over its layers."""
-        return sum(h * w for h, w in self.need.stream_shapes()) * self.pools[0].element_size() * len(self.entries)
+        """What one cached position of one sequence holds in this group, over its layers (its share of the scales rounded up)."""
+        codes = sum(h * w for h, w in self.need.stream_shapes()) * self.pools[0].element_size() * len(self.entries)
+        return codes + (-(-sum(4 * h for h, _ in self.need.stream_shapes()) * len(self.entries) // self.block) if self.block else 0)
 
 
 class SequenceCache:
@@ -211,7 +226,8 @@ class SequenceCache:
         grp = self.groups[g]
         streams = tuple(p[i] for p in grp.pools)
         return CacheLayerView(streams[0], streams[1] if len(streams) > 1 else None, grp.table, self.max_pages,
-                              self.page_size, grp.need.n_kv_heads, grp.need.head_dim, writes, g, streams)
+                              self.page_size, grp.need.n_kv_heads, grp.need.head_dim, writes, g, streams,
+                              tuple(x[i] for x in grp.scales))
 
     def state(self, entry: int):
         """The state area of a schedule entry: a tensor [n_slots, *shape], a dict name -> tensor for a

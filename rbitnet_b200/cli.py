@@ -30,6 +30,8 @@ def _add_engine_args(ap):
     ap.add_argument("--max-seq", type=int, default=None, help="longest sequence (default: the model's)")
     ap.add_argument("--cache-tokens", type=int, default=None, help="cache size in positions over all live sequences")
     ap.add_argument("--max-batch", type=int, default=64, help="most sequences generated together")
+    ap.add_argument("--cache-dtype", choices=["float8_e4m3"], default=None,
+                    help="hold keys and values in 8 bits (default: the compute dtype)")
 
 
 def _engine(args):
@@ -38,7 +40,7 @@ def _engine(args):
         raise SystemExit("no model: give --model DIR or set RBITNET_MODEL")
     kw = {"ops": args.ops} if getattr(args, "ops", None) is not None else {}
     return Engine.load_path(args.model, dtype=args.dtype, max_seq=args.max_seq, max_tokens=args.cache_tokens,
-                            max_batch=args.max_batch, verbose=True, **kw)
+                            max_batch=args.max_batch, cache_dtype=args.cache_dtype, verbose=True, **kw)
 
 
 def cmd_generate(args) -> int:
@@ -59,7 +61,7 @@ def cmd_generate(args) -> int:
         raise SystemExit("nothing to generate from: give --prompt TEXT or --prompt-ids '1 2 3' (or a file, one prompt a line)")
     stop = args.stop_id if args.stop_id else None
     results = eng.generate(prompts, max_tokens=args.max_tokens, temperature=args.temperature, seed=args.sample_seed,
-                           stop_ids=stop)
+                           stop_ids=stop, draft_tokens=args.draft_tokens)
     for r in results:
         print(json.dumps({"tokens": r.tokens, "finish_reason": r.finish_reason, "prompt_tokens": r.prompt_tokens}))
     return 0
@@ -110,6 +112,8 @@ def main(argv=None, ops=None) -> int:
     g.add_argument("--temperature", type=float, default=0.7, help="<= 0: greedy (reference server default 0.7)")
     g.add_argument("--sample-seed", type=int, default=0, help="seed of the sampling draws")
     g.add_argument("--stop-id", type=int, action="append", help="stop token id (default: config.json's eos_token_id)")
+    g.add_argument("--draft-tokens", type=int, default=0,
+                   help="check up to so many tokens a step that followed the last ones where they stood before (token ids only)")
     g.set_defaults(fn=cmd_generate)
     i = sub.add_parser("inspect", help="summary and tensor table of a model folder")
     i.add_argument("model")

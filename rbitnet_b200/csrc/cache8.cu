@@ -10,7 +10,7 @@
 //
 // A block that begins with the first new position takes its scale from the new values alone: what it held before (another
 // sequence's, or tokens that were dropped) has no part in it.  Otherwise scale = max(old, needed).
-#include "rb_rotary.cuh"
+#include "rb_common.cuh"
 
 #include <cuda_fp8.h>
 
@@ -78,6 +78,16 @@ __device__ __forceinline__ void rescale16(uint8_t* codes, int count, float ratio
   }
 }
 
+// Sine and cosine of position * frequency: the turns in float64, their fraction in (-1/2, 1/2] in float32, so that far positions
+// lose nothing.
+__device__ __forceinline__ float2 turn_of(int pos, float freq) {
+  const double turns = (double)pos * ((double)freq * 0.15915494309189533577);
+  float sn, cs;
+  const double whole = turns + 6755399441055744.0;         // 1.5 * 2^52: rounds to whole numbers
+  sincospif((float)(turns - (whole - 6755399441055744.0)) * 2.0f, &sn, &cs);
+  return make_float2(sn, cs);
+}
+
 struct Append8 {
   __nv_bfloat16* q_out;          // [T, H, D]
   const __nv_bfloat16* qkv;      // [T, (H + 2 Kh) D], rows qkv_stride apart (H D without writing)
@@ -118,10 +128,9 @@ __global__ void __launch_bounds__(256) append8_kernel(Append8 p) {
     a = p.interleaved ? 2 * i : i;
     b = p.interleaved ? 2 * i + 1 : i + rhalf;
     const float x0 = __bfloat162float(src[a]), x1 = __bfloat162float(src[b]);
-    float sn, cs;
-    angle_sincos(pos0 + tok, (double)p.inv_freq[i], 1.0f, &sn, &cs);
-    ya = x0 * cs - x1 * sn;
-    yb = x0 * sn + x1 * cs;
+    const float2 t = turn_of(pos0 + tok, p.inv_freq[i]);
+    ya = x0 * t.y - x1 * t.x;
+    yb = x0 * t.x + x1 * t.y;
   };
   int a, b;
   float ya, yb;
@@ -134,7 +143,7 @@ __global__ void __launch_bounds__(256) append8_kernel(Append8 p) {
   }
   if (!p.write_kv) return;
   const int before = pos0 % p.block;             // positions that the block holds already
-  const int64_t at = rb_page_offset(p.cache, slot, pos0, kvh) - (int64_t)before * D;       // of the block's first code
+  const int64_t at = rb_page_offset(p.cache, slot, pos0 - before, kvh);       // of the block's first code
   for (int stream = 0; stream < 2; ++stream) {
     uint8_t* codes = (uint8_t*)(stream == 0 ? p.cache.k : p.cache.v) + at;
     float* scale = (stream == 0 ? p.k_scale : p.v_scale) + at / ((int64_t)p.block * D);
@@ -178,17 +187,30 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// sc: the token's (sine, cosine) of pairs 8e .. 8e + 7
-__device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const float2* sc, int interleaved) {
+// Sines and cosines of pairs 8e .. 8e + 7 at a position.
+__device__ __forceinline__ void turns8(const Append8& p, int pos, int e, float2 (&sc)[8]) {
+  const float4 lo = *reinterpret_cast<const float4*>(p.inv_freq + 8 * e), hi = *reinterpret_cast<const float4*>(p.inv_freq + 8 * e + 4);
+  const float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sc[i] = turn_of(pos, f[i]);
+}
+__device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const float2 (&sc)[8], int interleaved) {
+  if (interleaved) {                             // pair i is (2i, 2i + 1) of the sixteen values
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float& x = i < 4 ? a[2 * i] : b[2 * i - 8];
+      float& y = i < 4 ? a[2 * i + 1] : b[2 * i - 7];
+      const float x0 = x, x1 = y;
+      x = x0 * sc[i].y - x1 * sc[i].x;
+      y = x0 * sc[i].x + x1 * sc[i].y;
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float2 t = sc[i];
-    // interleaved: pair i is (2i, 2i + 1) of the sixteen values
-    float& x = interleaved ? (i < 4 ? a[2 * i] : b[2 * i - 8]) : a[i];
-    float& y = interleaved ? (i < 4 ? a[2 * i + 1] : b[2 * i - 7]) : b[i];
-    const float x0 = x, x1 = y;
-    x = x0 * t.y - x1 * t.x;
-    y = x0 * t.x + x1 * t.y;
+    const float x0 = a[i], x1 = b[i];
+    a[i] = x0 * sc[i].y - x1 * sc[i].x;
+    b[i] = x0 * sc[i].x + x1 * sc[i].y;
   }
 }
 __device__ __forceinline__ float largest8(const float (&a)[8], const float (&b)[8]) {
@@ -198,98 +220,102 @@ __device__ __forceinline__ float largest8(const float (&a)[8], const float (&b)[
   return m;
 }
 
-// Heads of a multiple of 16 values (up to 128 SPAN), turned whole, rows on 16 bytes: a block of threads per (tile, kv head) as above, but a
-// thread takes eight pairs at a time (16-byte loads and stores), a token's sines and cosines are made once for the query heads
-// and the key, and the tile's keys and values stay in registers between the largest value and the codes.
-// A tile of 64 tokens reads 64 (G + 2) D values; 8,192 tokens of 32 heads on 8 kv heads of 128 are 1,024 blocks.
-template <int SPAN>
-__global__ void __launch_bounds__(256) append8_tiles_kernel(Append8 p) {
+// Heads of a multiple of 16 values, turned whole, rows on 16 bytes: a block of threads per (tile, kv head).  A thread takes one piece of
+// eight pairs of one token (SPAN of them where a head is long), and of that piece everything: it makes the sines and cosines once, in
+// registers, turns the key's piece and those of the G query heads with them, and keeps the key's and the value's pieces until the
+// block's largest values have met.  16-byte loads and stores; the blocks of a tile's kv heads run side by side, so that rows are read whole.
+// What bounds it is the chain of waits of a block (tile, positions, rows, the largest values), hidden behind the blocks beside it.
+template <int THREADS, int SPAN>
+__global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append8_tiles_kernel(Append8 p) {
   rb_pdl_launch_dependents();
-  extern __shared__ float2 turns[];              // [tokens of the tile][D / 2] (sine, cosine)
-  __shared__ float tops[2][8];
-  const int D = p.cache.head_dim, Kh = p.cache.n_kv_heads, G = p.H / Kh, half = D / 2, pieces = D / 16;
-  const int kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tok0 = p.tile_tok0[blockIdx.x], n = p.tile_ntok[blockIdx.x];
+  __shared__ float tops[2][THREADS / 32];
+  const int D = p.cache.head_dim, Kh = p.cache.n_kv_heads, G = p.H / Kh, pieces = D / 16;
+  const int tile = blockIdx.y, kvh = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tok0 = p.tile_tok0[tile], n = p.tile_ntok[tile];
   const int slot = p.tok_slot[tok0], pos0 = p.tok_pos[tok0];
+  const int before = pos0 % p.block;             // positions that the block holds already
+  int64_t at = 0, unit = 0;
+  if (p.write_kv) {
+    at = rb_page_offset(p.cache, slot, pos0 - before, kvh);                   // of the block's first code
+    unit = at / ((int64_t)p.block * D);
+  }
+  int tok[SPAN], e[SPAN];
+  float2 sc[SPAN][8];
+#pragma unroll
+  for (int i = 0; i < SPAN; ++i) {
+    const int item = i * THREADS + threadIdx.x;
+    tok[i] = item / pieces;
+    e[i] = item % pieces;
+    if (p.rot_dim && tok[i] < n) turns8(p, pos0 + tok[i], e[i], sc[i]);        // (frequencies and positions need no wait)
+  }
   rb_pdl_wait();
   const __nv_bfloat16* rows = p.qkv + (int64_t)tok0 * p.qkv_stride;
-  // the keys and values are asked for first
-  uint4 kv[2][SPAN][2];
+  uint4 raw[2][SPAN][2];
+  float old[2] = {0.f, 0.f};
   if (p.write_kv) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int i = 0; i < SPAN; ++i) {
-        const int item = i * 256 + threadIdx.x, tok = item / pieces, e = item % pieces;
-        kv[s][i][0] = kv[s][i][1] = make_uint4(0, 0, 0, 0);
-        if (tok < n) {
-          const __nv_bfloat16* src = rows + (int64_t)tok * p.qkv_stride + (int64_t)(p.H + s * Kh + kvh) * D;
-          kv[s][i][0] = *reinterpret_cast<const uint4*>(src + piece_a(p, e));
-          kv[s][i][1] = *reinterpret_cast<const uint4*>(src + piece_b(p, e));
+        raw[s][i][0] = raw[s][i][1] = make_uint4(0, 0, 0, 0);
+        if (tok[i] < n) {
+          const __nv_bfloat16* src = rows + (int64_t)tok[i] * p.qkv_stride + (int64_t)(p.H + s * Kh + kvh) * D;
+          raw[s][i][0] = *reinterpret_cast<const uint4*>(src + piece_a(p, e[i]));
+          raw[s][i][1] = *reinterpret_cast<const uint4*>(src + piece_b(p, e[i]));
         }
       }
+    if (before > 0) { old[0] = p.k_scale[unit]; old[1] = p.v_scale[unit]; }
   }
-  for (int i = threadIdx.x; p.rot_dim && i < n * half; i += 256) {
-    float sn, cs;
-    angle_sincos(pos0 + i / half, (double)p.inv_freq[i % half], 1.0f, &sn, &cs);
-    turns[i] = make_float2(sn, cs);
-  }
-  __syncthreads();
-  float2 top = make_float2(0.f, 0.f);
-  if (p.write_kv) {
+  // the query heads
 #pragma unroll
-    for (int i = 0; i < SPAN; ++i) {
-      const int item = i * 256 + threadIdx.x, tok = item / pieces, e = item % pieces;
+  for (int i = 0; i < SPAN; ++i) {
+    if (tok[i] >= n) continue;
+    const __nv_bfloat16* src = rows + (int64_t)tok[i] * p.qkv_stride + (int64_t)kvh * G * D;
+    __nv_bfloat16* dst = p.q_out + ((int64_t)(tok0 + tok[i]) * p.H + kvh * G) * D;
+#pragma unroll 4
+    for (int g = 0; g < G; ++g) {
+      const uint4 qa = *reinterpret_cast<const uint4*>(src + g * D + piece_a(p, e[i])), qb = *reinterpret_cast<const uint4*>(src + g * D + piece_b(p, e[i]));
       float a[8], b[8];
-      unpack8(kv[1][i][0], a); unpack8(kv[1][i][1], b);
-      top.y = fmaxf(top.y, largest8(a, b));
-      if (tok < n) {
-        unpack8(kv[0][i][0], a); unpack8(kv[0][i][1], b);
-        if (p.rot_dim) turn8(a, b, turns + tok * half + 8 * e, p.interleaved);
-        top.x = fmaxf(top.x, largest8(a, b));
-      }
+      unpack8(qa, a);
+      unpack8(qb, b);
+      if (p.rot_dim) turn8(a, b, sc[i], p.interleaved);
+      *reinterpret_cast<uint4*>(dst + g * D + piece_a(p, e[i])) = pack8(a);
+      *reinterpret_cast<uint4*>(dst + g * D + piece_b(p, e[i])) = pack8(b);
     }
-    top.x = rb_warp_max(top.x);
-    top.y = rb_warp_max(top.y);
-    if (lane == 0) { tops[0][warp] = top.x; tops[1][warp] = top.y; }
-  }
-  // the query heads, while the largest values meet
-  for (int item = threadIdx.x; item < n * G * pieces; item += 256) {
-    const int e = item % pieces, th = item / pieces, tok = th / G, head = kvh * G + th % G;
-    const __nv_bfloat16* src = rows + (int64_t)tok * p.qkv_stride + (int64_t)head * D;
-    __nv_bfloat16* dst = p.q_out + ((int64_t)(tok0 + tok) * p.H + head) * D;
-    float a[8], b[8];
-    unpack8(*reinterpret_cast<const uint4*>(src + piece_a(p, e)), a);
-    unpack8(*reinterpret_cast<const uint4*>(src + piece_b(p, e)), b);
-    if (p.rot_dim) turn8(a, b, turns + tok * half + 8 * e, p.interleaved);
-    *reinterpret_cast<uint4*>(dst + piece_a(p, e)) = pack8(a);
-    *reinterpret_cast<uint4*>(dst + piece_b(p, e)) = pack8(b);
   }
   if (!p.write_kv) return;
-  const int before = pos0 % p.block;             // positions that the block holds already
-  const int64_t at = rb_page_offset(p.cache, slot, pos0, kvh) - (int64_t)before * D;       // of the block's first code
-  const int64_t unit = at / ((int64_t)p.block * D);
-  const float old_k = before > 0 ? p.k_scale[unit] : 0.f, old_v = before > 0 ? p.v_scale[unit] : 0.f;
+  float ka[SPAN][8], kb[SPAN][8], top[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < SPAN; ++i) {
+    float a[8], b[8];
+    unpack8(raw[1][i][0], a); unpack8(raw[1][i][1], b);
+    top[1] = fmaxf(top[1], largest8(a, b));
+    unpack8(raw[0][i][0], ka[i]); unpack8(raw[0][i][1], kb[i]);
+    if (p.rot_dim && tok[i] < n) turn8(ka[i], kb[i], sc[i], p.interleaved);
+    top[0] = fmaxf(top[0], largest8(ka[i], kb[i]));
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    top[s] = rb_warp_max(top[s]);
+    if (lane == 0) tops[s][warp] = top[s];
+  }
   __syncthreads();                               // (everybody has the old scales, too)
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     float amax = tops[s][0];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) amax = fmaxf(amax, tops[s][w]);
-    const float old = s ? old_v : old_k, now = fmaxf(old, scale_for(amax)), inv = 1.0f / now;
+    for (int w = 1; w < THREADS / 32; ++w) amax = fmaxf(amax, tops[s][w]);
+    const float now = fmaxf(old[s], scale_for(amax)), inv = 1.0f / now;
     uint8_t* codes = (uint8_t*)(s ? p.cache.v : p.cache.k) + at;
-    if (old < now) rescale16(codes, before * D, old * inv, threadIdx.x, 256);
+    if (old[s] < now) rescale16(codes, before * D, old[s] * inv, threadIdx.x, THREADS);
 #pragma unroll
     for (int i = 0; i < SPAN; ++i) {
-      const int item = i * 256 + threadIdx.x, tok = item / pieces, e = item % pieces;
-      if (tok < n) {
-        float a[8], b[8];
-        unpack8(kv[s][i][0], a); unpack8(kv[s][i][1], b);
-        if (s == 0 && p.rot_dim) turn8(a, b, turns + tok * half + 8 * e, p.interleaved);
-        uint8_t* to = codes + (before + tok) * D;
-        *reinterpret_cast<uint2*>(to + piece_a(p, e)) = codes8(a, inv);
-        *reinterpret_cast<uint2*>(to + piece_b(p, e)) = codes8(b, inv);
-      }
+      if (tok[i] >= n) continue;
+      uint8_t* to = codes + (before + tok[i]) * D;
+      float a[8], b[8];
+      if (s) { unpack8(raw[1][i][0], a); unpack8(raw[1][i][1], b); }
+      *reinterpret_cast<uint2*>(to + piece_a(p, e[i])) = codes8(s ? a : ka[i], inv);
+      *reinterpret_cast<uint2*>(to + piece_b(p, e[i])) = codes8(s ? b : kb[i], inv);
     }
     if (threadIdx.x == 0) (s ? p.v_scale : p.k_scale)[unit] = now;
   }
@@ -303,16 +329,13 @@ __global__ void __launch_bounds__(256) append8_step_kernel(Append8 p) {
   const int D = p.cache.head_dim, Kh = p.cache.n_kv_heads, G = p.H / Kh, half = D / 2, pieces = D / 16;
   const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y * (blockDim.x >> 5) + warp;
   const int slot = p.tok_slot[row], pos = p.tok_pos[row];
-  for (int i = threadIdx.x; p.rot_dim && i < half; i += blockDim.x) {       // (positions and frequencies: not written by the kernel before)
-    float sn, cs;
-    angle_sincos(pos, (double)p.inv_freq[i], 1.0f, &sn, &cs);
-    turns[i] = make_float2(sn, cs);
-  }
+  for (int i = threadIdx.x; p.rot_dim && i < half; i += blockDim.x)         // (positions and frequencies: not written by the kernel before)
+    turns[i] = turn_of(pos, p.inv_freq[i]);
   const bool mine = kvh < Kh;
   int64_t at = 0, unit = 0;
   const int before = pos % p.block;
   if (mine && p.write_kv) {
-    at = rb_page_offset(p.cache, slot, pos, kvh) - (int64_t)before * D;
+    at = rb_page_offset(p.cache, slot, pos - before, kvh);
     unit = at / ((int64_t)p.block * D);
   }
   rb_pdl_wait();
@@ -335,7 +358,12 @@ __global__ void __launch_bounds__(256) append8_step_kernel(Append8 p) {
     if (on) {
       unpack8(*reinterpret_cast<const uint4*>(src + head * D + piece_a(p, e)), a);
       unpack8(*reinterpret_cast<const uint4*>(src + head * D + piece_b(p, e)), b);
-      if (!is_v && p.rot_dim) turn8(a, b, turns + 8 * e, p.interleaved);
+      if (!is_v && p.rot_dim) {
+        float2 sc[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sc[i] = turns[8 * e + i];
+        turn8(a, b, sc, p.interleaved);
+      }
     }
     if (on && !is_k && !is_v) {
       __nv_bfloat16* dst = p.q_out + ((int64_t)row * p.H + head) * D;
@@ -420,6 +448,7 @@ RB_EXPORT int rb_append8(void* q_out, const void* qkv, int64_t qkv_stride, const
   RB_REQUIRE(D > 0 && D % 2 == 0 && D <= 512, "rb_append8: head_dim %d must be even, and 512 at most", D);
   RB_REQUIRE(rot_dim >= 0 && rot_dim <= D && rot_dim % 2 == 0, "rb_append8: the rotated prefix %d must be even and at most %d", rot_dim, D);
   RB_REQUIRE(H > 0 && Kh > 0 && H % Kh == 0 && Kh <= 65535, "rb_append8: %d heads on %d kv heads", H, Kh);
+  RB_REQUIRE(!tile_tok0 || n_tiles <= 65535, "rb_append8: %d tiles in one launch", n_tiles);
   const int block = rb_cache8_block(page_size);
   RB_REQUIRE(block > 0, "rb_append8: a page of %d positions must be 64 at most, or a multiple of 64", page_size);
   Append8 p;
@@ -428,23 +457,16 @@ RB_EXPORT int rb_append8(void* q_out, const void* qkv, int64_t qkv_stride, const
   p.cache = RbPagedLayer{cache_k, cache_v, page_table, max_pages, page_size, Kh, D};
   p.k_scale = k_scale; p.v_scale = v_scale;
   p.block = block; p.H = H; p.write_kv = write_kv; p.interleaved = interleaved; p.rot_dim = rot_dim;
-  const uintptr_t bases = (uintptr_t)q_out | (uintptr_t)qkv | (uintptr_t)cache_k | (uintptr_t)cache_v;
+  const uintptr_t bases = (uintptr_t)inv_freq | (uintptr_t)q_out | (uintptr_t)qkv | (uintptr_t)cache_k | (uintptr_t)cache_v;
   if (D % 16 == 0 && D <= 256 && (rot_dim == D || rot_dim == 0) && qkv_stride % 8 == 0 && (bases & 15) == 0) {
     if (!tile_tok0) {
       const int warps = Kh < 8 ? Kh : 8;
       RB_LAUNCH("rb_append8 (step)", (append8_step_kernel), dim3(n_tiles, (Kh + warps - 1) / warps), warps * 32, (size_t)D / 2 * 8, stream, p);
       return 0;
     }
-    static RbOncePerDevice tiled;
-    if (tiled.first()) {
-      RB_CUDA(cudaFuncSetAttribute(append8_tiles_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_BLOCK * 32 * 8));
-      RB_CUDA(cudaFuncSetAttribute(append8_tiles_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_BLOCK * 64 * 8));
-      RB_CUDA(cudaFuncSetAttribute(append8_tiles_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_BLOCK * 128 * 8));
-    }
-    const size_t turns = (size_t)block * D / 2 * 8;
-    if (D <= 64) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<1>), dim3(n_tiles, Kh), 256, turns, stream, p);
-    else if (D <= 128) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<2>), dim3(n_tiles, Kh), 256, turns, stream, p);
-    else RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<4>), dim3(n_tiles, Kh), 256, turns, stream, p);
+    if (D <= 64) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<256, 1>), dim3(Kh, n_tiles), 256, 0, stream, p);
+    else if (D <= 128) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<512, 1>), dim3(Kh, n_tiles), 512, 0, stream, p);
+    else RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<512, 2>), dim3(Kh, n_tiles), 512, 0, stream, p);
     return 0;
   }
   static RbOncePerDevice configured;

@@ -43,6 +43,16 @@ def _dtype(d):
     return _DTYPES[d]
 
 
+def _cache_dtype(d, compute):
+    if d is None or d == compute:
+        return compute
+    if d not in ("float8_e4m3", "fp8", torch.float8_e4m3fn):
+        raise ValueError(f"cache_dtype must be None or 'float8_e4m3', found {d!r}")
+    if compute != torch.bfloat16:
+        raise ValueError("a cache held in 8 bits goes with the bfloat16 mode; float32 has no reduced precision anywhere")
+    return torch.float8_e4m3fn
+
+
 def _no_parent_components(path) -> None:
     # crates/bitnet-core/src/inference.rs:44-53
     if ".." in Path(path).parts:
@@ -54,10 +64,12 @@ class Engine:
                  device="cuda:0", max_tokens: Optional[int] = None, max_seq: Optional[int] = None,
                  max_batch: int = 64, page_size: int = PAGE_SIZE, max_batch_tokens: int = 8192,
                  ops=None, model_path: Optional[Path] = None, verbose: bool = False,
-                 use_graphs: bool = True):
+                 use_graphs: bool = True, cache_dtype=None):
         """max_seq: longest sequence (default: the configuration's max positions).
         max_tokens: cache size in positions over all live sequences, each rounded up to
-        whole pages (default: max_batch sequences of max_seq)."""
+        whole pages (default: max_batch sequences of max_seq).
+        cache_dtype: None (keys and values in the compute dtype), or "float8_e4m3": codes of 8 bits with a scale per block of
+        positions and kv head, half the bytes.  For the bfloat16 mode and layers of plain attention (``Mixer.cache_in_8_bits``)."""
         from ..kernels.ops import CudaOps
         self.config = config
         self.model_path = model_path
@@ -77,13 +89,19 @@ class Engine:
         #: decode steps run as captured CUDA graphs (one per batch size)
         self.use_graphs = use_graphs and ops is None
         cache_needs, reads, state_needs = self.model.cache_plan()
+        self.cache_dtype = _cache_dtype(cache_dtype, self.dtype)
+        if self.cache_dtype != self.dtype:
+            for entry in sorted(set(cache_needs) | set(reads)):
+                layer = self.spec.schedule[entry].layer
+                if not self.model.mixer(layer).cache_in_8_bits:
+                    raise ValueError(f"cache_dtype {cache_dtype!r}: layer {layer} keeps its cache in the compute dtype only")
         # The captured step of a batch size between two graphs is filled up with rows of a padding
         # sequence.  It gets a slot and a page of its own, beyond what the caller asked for, here and
         # now: taken at its first use it could take a page that a running batch was promised.
         n_pages = max(1, -(-max_tokens // page_size))
         extra = 1 if self.use_graphs else 0
         self.cache = SequenceCache(cache_needs, reads, state_needs, (n_pages + extra) * page_size, self.max_seq,
-                                   self.dtype, self.ops.device, page_size=page_size, n_slots=n_pages + extra)
+                                   self.cache_dtype, self.ops.device, page_size=page_size, n_slots=n_pages + extra)
         self._pad_slot = None
         if self.use_graphs:
             self._pad_slot = self.cache.alloc()
@@ -277,18 +295,48 @@ class Engine:
     # ------------------------------------------------------------------ generation
     def generate(self, prompts: Sequence[Sequence[int]], max_tokens: int = 256, temperature: float = 0.7,
                  seed: int = 0, stop_ids: Optional[Sequence[int]] = None,
-                 max_batch: Optional[int] = None, on_token=None) -> List[GenerationResult]:
+                 max_batch: Optional[int] = None, on_token=None, draft_tokens: int = 0) -> List[GenerationResult]:
         """Token-id prompts in, generated ids out, one result per prompt in order.
         temperature <= 0 is greedy.  Defaults are the reference server's
         (crates/bitnet-server/src/lib.rs:317, :358).  ``on_token(request index, token id)`` is
-        called for every emitted token as soon as the host has it."""
+        called for every emitted token as soon as the host has it.
+        ``draft_tokens`` > 0: a step checks up to so many tokens that followed the sequence's last ones where they stood before
+        (``generate.Lookup``), and takes one of its own behind the accepted ones; the tokens are distributed as without it
+        (greedy: the same, up to rounding).  Needs sequences that can take a step back: no windows, no recurrent state."""
         loop = GenerationLoop(self._step_sample, self.cache, max_batch or self.max_batch,
                               decoder=self if self.use_graphs else None)
-        out = loop.run(prompts, max_tokens, temperature, seed,
-                       self.stop_ids if stop_ids is None else stop_ids, on_token=on_token)
+        stop = self.stop_ids if stop_ids is None else stop_ids
+        if draft_tokens > 0:
+            if self.cache.states or self.cache.book.has_windows:
+                raise ValueError("draft_tokens: this model's sequences keep recurrent state or windows, which cannot take a step back")
+            out = loop.run_drafted(prompts, max_tokens, temperature, seed, stop, int(draft_tokens), self._verify_step, on_token=on_token)
+        elif draft_tokens < 0:
+            raise ValueError(f"draft_tokens {draft_tokens} is negative")
+        else:
+            out = loop.run(prompts, max_tokens, temperature, seed, stop, on_token=on_token)
         self.last_stats = {"steps": loop.steps, "prefill_tokens": loop.prefill_tokens,
-                           "decode_tokens": loop.decode_tokens}
+                           "decode_tokens": loop.decode_tokens, "drafted_tokens": loop.drafted_tokens}
         return out
+
+    def _verify_step(self, feed, temperatures, uniforms) -> List[List[int]]:
+        """One step over (slot, last token and drafts) pairs; per sequence the accepted drafts and the token taken behind them.
+        ``uniforms``: two numbers per row.  A sequence moves on by what was accepted; what the step wrote behind that is written over
+        by the next one."""
+        logits = self.stepper.step([StepEntry(slot, toks, list(range(len(toks)))) for slot, toks in feed], advance=False)
+        counts = [len(toks) for _, toks in feed]
+        drafts = [t for _, toks in feed for t in list(toks[1:]) + [-1]]
+        most = max(counts) - 1
+        ints = upload(np.asarray(np.concatenate([np.cumsum([0] + counts), drafts]), dtype=np.int32), self.ops.device)
+        floats = upload(np.concatenate([np.asarray(temperatures, dtype=np.float32), np.asarray(uniforms, dtype=np.float32).reshape(-1)]),
+                        self.ops.device)
+        B = len(feed)
+        accepted, tokens = self.ops.verify_drafts(logits, ints[:B + 1], ints[B + 1:], floats[:B], floats[B:].view(-1, 2), most)
+        both = torch.cat([accepted[:, None], tokens], dim=1).tolist()
+        if hasattr(self.ops, "check_errors"):
+            self.ops.check_errors()
+        for (slot, _), row in zip(feed, both):
+            self.cache.advance(slot, row[0] + 1)
+        return [row[1:row[0] + 2] for row in both]
 
     def _load_tokenizer(self):
         if self._tokenizer is None:

@@ -28,6 +28,9 @@ from typing import Callable, List, Optional, Sequence
 
 from ..sampling.rng import uniforms
 
+#: the numbers that drafts are accepted with are of another seed than those that tokens are drawn with
+ACCEPT_SEED = 0x5EED0D12AF7
+
 
 @dataclass
 class GenerationResult:
@@ -42,6 +45,34 @@ class _Live:
     slot: int
     last: int
     out: List[int] = field(default_factory=list)
+
+
+class Lookup:
+    """Drafts for a sequence from the sequence itself: what followed the last earlier occurrence of its last three tokens (else of the
+    last two, else of the last one)."""
+
+    LONGEST = 3
+
+    def __init__(self, tokens: Sequence[int]):
+        self.tokens: List[int] = []
+        self._after = [{} for _ in range(self.LONGEST)]     # per length: the tokens -> the place behind their last earlier occurrence
+        self.extend(tokens)
+
+    def extend(self, tokens: Sequence[int]) -> None:
+        for t in tokens:
+            # the runs that ended before this token are earlier occurrences from now on
+            n = len(self.tokens)
+            for k in range(1, min(self.LONGEST, n) + 1):
+                self._after[k - 1][tuple(self.tokens[n - k:])] = n
+            self.tokens.append(int(t))
+
+    def propose(self, most: int) -> List[int]:
+        n = len(self.tokens)
+        for k in range(min(self.LONGEST, n), 0, -1):
+            at = self._after[k - 1].get(tuple(self.tokens[n - k:]))
+            if at is not None:
+                return self.tokens[at:at + most]
+        return []
 
 
 class GenerationLoop:
@@ -60,6 +91,7 @@ class GenerationLoop:
         self.steps = 0
         self.prefill_tokens = 0
         self.decode_tokens = 0
+        self.drafted_tokens = 0       # drafts that were checked
 
     def _take_batch(self, pending: List[int], prompts, max_tokens: int) -> List[int]:
         batch: List[int] = []
@@ -171,6 +203,79 @@ class GenerationLoop:
                     live = take(live, sampled)
                     feed = [(s.slot, [s.last]) for s in live]
                     self.decode_tokens += len(live)
+            finally:
+                for s in live:
+                    if s.slot >= 0:
+                        self.cache.free(s.slot)
+        return results  # type: ignore[return-value]
+
+    def run_drafted(self, prompts: Sequence[Sequence[int]], max_tokens: int, temperature: float, seed: int, stop_ids: Sequence[int],
+                    most: int, verify_step: Callable, on_token: Optional[Callable[[int, int], None]] = None) -> List[GenerationResult]:
+        """``run`` with steps that check up to ``most`` drafted tokens a sequence (``Lookup``): ``verify_step(entries, temperatures,
+        uniforms)`` runs one step over ``(slot, last token and drafts)`` pairs, moves each sequence on by what it accepted, and
+        returns per sequence the accepted drafts and the token taken behind them; ``uniforms`` has two numbers a row."""
+        stop = set(int(s) for s in stop_ids)
+        results: List[Optional[GenerationResult]] = [None] * len(prompts)
+        pending = []
+        for r, p in enumerate(prompts):
+            if len(p) == 0:
+                results[r] = GenerationResult([], "empty", 0)
+            elif max_tokens <= 0:
+                results[r] = GenerationResult([], "length", len(p))
+            else:
+                pending.append(r)
+
+        def emit(s: _Live, tokens: Sequence[int], lookup: Lookup) -> bool:
+            """Books a sequence's new tokens; whether it goes on."""
+            for tok in tokens:
+                tok = int(tok)
+                reason = "stop" if tok in stop else None
+                if reason is None:
+                    s.out.append(tok)
+                    s.last = tok
+                    lookup.extend([tok])
+                    if on_token is not None:
+                        on_token(s.request, tok)
+                    if len(s.out) >= max_tokens or len(prompts[s.request]) + len(s.out) > self.cache.max_seq:
+                        reason = "length"        # (or no room to feed this token back)
+                if reason is not None:
+                    results[s.request] = GenerationResult(s.out, reason, len(prompts[s.request]))
+                    self.cache.free(s.slot)
+                    s.slot = -1
+                    return False
+            return True
+
+        def numbers(s: _Live, rows: int) -> List[List[float]]:
+            if temperature <= 0:
+                return [[0.0, 0.0]] * rows
+            steps = [len(s.out) + j for j in range(rows)]
+            return list(map(list, zip(uniforms(seed ^ ACCEPT_SEED, [s.request] * rows, steps).tolist(),
+                                      uniforms(seed, [s.request] * rows, steps).tolist())))
+
+        while pending:
+            batch = self._take_batch(pending, prompts, max_tokens)
+            pending = pending[len(batch):]
+            live = [_Live(r, self.cache.alloc(), -1) for r in batch]
+            lookups = {s.request: Lookup(prompts[s.request]) for s in live}
+            try:
+                feed = [(s.slot, list(prompts[s.request])) for s in live]
+                self.prefill_tokens += sum(len(t) for _, t in feed)
+                draws = [numbers(s, 1)[0][1] for s in live]
+                sampled = self.step_sample(feed, [temperature] * len(live), draws)
+                self.steps += 1
+                live = [s for s, tok in zip(live, sampled) if emit(s, [tok], lookups[s.request])]
+                while live:
+                    feed, draws = [], []
+                    for s in live:
+                        # as many drafts as tokens can still be emitted beside the one that is taken, and as the cache has room for
+                        room = min(most, max_tokens - len(s.out) - 1, self.cache.max_seq - self.cache.length(s.slot) - 1)
+                        feed.append((s.slot, [s.last] + lookups[s.request].propose(max(room, 0))))
+                        draws.extend(numbers(s, len(feed[-1][1])))
+                    self.drafted_tokens += sum(len(t) - 1 for _, t in feed)
+                    got = verify_step(feed, [temperature] * len(live), draws)
+                    self.steps += 1
+                    self.decode_tokens += sum(len(t) for t in got)
+                    live = [s for s, tokens in zip(live, got) if emit(s, tokens, lookups[s.request])]
             finally:
                 for s in live:
                     if s.slot >= 0:

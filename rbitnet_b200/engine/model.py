@@ -73,6 +73,10 @@ class Model:
                              "mixer, so give each mixer a layer of its own")
         return mixers[0] if mixers else None
 
+    def mixer(self, layer: int):
+        """The mixer of a layer (None if it has none)."""
+        return self._mixer_of(self.blocks[layer], layer)
+
     # what the cache has to provide
     def cache_plan(self):
         from ..parts.base import Mixer

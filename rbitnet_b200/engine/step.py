@@ -91,9 +91,11 @@ class Stepper:
         self.model, self.cache, self.ops = model, cache, ops
         self.max_batch_tokens = max_batch_tokens
 
-    def step(self, entries: Sequence[StepEntry]) -> Optional[torch.Tensor]:
+    def step(self, entries: Sequence[StepEntry], advance: bool = True) -> Optional[torch.Tensor]:
         """Returns float32 logits [number of wanted places, vocab] on the device, in the
-        order of the entries and of each entry's ``want``; None if nothing is wanted."""
+        order of the entries and of each entry's ``want``; None if nothing is wanted.
+        ``advance`` False: the sequences' lengths stay, for a caller that moves them on by as many of the tokens as
+        count (``cache.advance``); the next step writes over the others."""
         V = self.model.vocab_size
         seen = set()
         arrays = []
@@ -150,7 +152,7 @@ class Stepper:
                 rows += n
                 done += n
         flush()
-        for e in entries:
+        for e in entries if advance else ():
             self.cache.advance(e.slot, len(e.tokens))
         if not outputs:
             return None

@@ -61,6 +61,15 @@ def memory_chunks_pay(longest: int, tokens: int, chunks: int, heads: int, dim: i
     return in_chunks < by_token
 
 
+def _address(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _cache8(view):
+    """Addresses of a cache held in 8 bits: keys, values, their scales, the page table."""
+    return (view.k.data_ptr(), view.v.data_ptr(), view.scales[0].data_ptr(), view.scales[1].data_ptr(), view.page_table.data_ptr())
+
+
 @dataclass
 class LinearWeight:
     """A weight matrix [out, in] made ready for ``linear``."""
@@ -685,20 +694,24 @@ class CudaOps:
     # ------------------------------------------------------------------ the cache held in 8 bits
     def _check_cache8(self, view, what: str) -> int:
         """Refuses what the 8-bit kernels do not take; returns the positions of a block."""
+        (k, v), (ks, vs), table, page = (view.k, view.v), view.scales, view.page_table, view.page_size
+        block = page if 0 < page <= 64 else (64 if page > 0 and page % 64 == 0 else 0)
+        shape = k.shape
+        if (self.dtype == torch.bfloat16 and block and k.dtype == v.dtype == torch.float8_e4m3fn and k.is_cuda and table.dtype == torch.int32
+                and ks.dtype == vs.dtype == torch.float32 and k.device == v.device == ks.device == vs.device == table.device
+                and shape == v.shape == (shape[0], view.n_kv_heads, page, view.head_dim)
+                and ks.shape == vs.shape == (shape[0], view.n_kv_heads, page // block)
+                and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and table.is_contiguous()
+                and table.dim() == 2 and table.shape[1] == view.max_pages):
+            return block
         if self.dtype != torch.bfloat16:
             raise KernelError(f"{what}: a cache held in 8 bits goes with the bfloat16 mode, not with {self.dtype}")
-        block = self.lib.raw("rb_cache8_block")(view.page_size)
-        if block <= 0:
-            raise KernelError(f"{what}: a page of {view.page_size} positions must be 64 at most, or a multiple of 64")
-        pool = (view.k.shape[0], view.n_kv_heads, view.page_size, view.head_dim)
-        scales = (view.k.shape[0], view.n_kv_heads, view.page_size // block)
-        for name, t, s in (("keys", view.k, view.scales[0]), ("values", view.v, view.scales[1])):
-            self._check(t, torch.float8_e4m3fn, f"{what}: {name}")
-            self._check(s, torch.float32, f"{what}: the scales of the {name}")
-            if tuple(t.shape) != pool or tuple(s.shape) != scales:
-                raise KernelError(f"{what}: {name} {tuple(t.shape)} with scales {tuple(s.shape)}, expected {pool} and {scales}")
-        self._check(view.page_table, torch.int32, f"{what}: page table")
-        return block
+        if not block:
+            raise KernelError(f"{what}: a page of {page} positions must be 64 at most, or a multiple of 64")
+        found = ", ".join(f"{t.dtype} {tuple(t.shape)} on {t.device}, contiguous={t.is_contiguous()}" for t in (k, v, ks, vs, table))
+        raise KernelError(f"{what}: expected contiguous float8_e4m3fn pools [pages, {view.n_kv_heads}, {page}, {view.head_dim}], float32 scales "
+                          f"[pages, {view.n_kv_heads}, {page // block}] and an int32 page table [slots, {view.max_pages}] on one CUDA device; "
+                          f"found {found}")
 
     def _block_tiles(self, meta, block: int):
         """(first row, rows, count) of the tiles of a step's rows that lie in one block of one sequence, made once per step;
@@ -732,10 +745,9 @@ class CudaOps:
         inv_freq, interleaved, rot_dim = (self._zeros_freq(D), False, 0) if rotary is None else rotary
         tok0, ntok, n_tiles = self._block_tiles(meta, block)
         q = torch.empty((T, n_heads, D), dtype=self.dtype, device=self.device)
-        self.lib.call("rb_append8", _ptr(q), _ptr(qkv), qkv.stride(0), _ptr(inv_freq), _ptr(meta.tok_pos), _ptr(meta.tok_slot),
-                      _ptr(tok0), _ptr(ntok), n_tiles, _ptr(view.k), _ptr(view.v), _ptr(view.scales[0]), _ptr(view.scales[1]),
-                      _ptr(view.page_table), view.max_pages, view.page_size, n_heads, Kh, D, 1 if view.writes else 0, rot_dim,
-                      1 if interleaved else 0, self._stream())
+        self.lib.call("rb_append8", q.data_ptr(), qkv.data_ptr(), qkv.stride(0), inv_freq.data_ptr(), meta.tok_pos.data_ptr(),
+                      meta.tok_slot.data_ptr(), _address(tok0), _address(ntok), n_tiles, *_cache8(view), view.max_pages, view.page_size,
+                      n_heads, Kh, D, 1 if view.writes else 0, rot_dim, 1 if interleaved else 0, self._stream())
         return q
 
     def cache_ranges(self, view, ranges) -> CacheRanges:
@@ -758,11 +770,9 @@ class CudaOps:
         if not view.scales:
             raise KernelError("cache_values: the cache holds its values in the compute dtype")
         self._check_cache8(view, "cache_values")
-        shape = (ranges.count, view.n_kv_heads, view.page_size, view.head_dim)
-        k, v = (torch.empty(shape, dtype=torch.bfloat16, device=self.device) for _ in range(2))
-        self.lib.call("rb_cache8_values", _ptr(k), _ptr(v), _ptr(ranges.items), ranges.count, _ptr(view.k), _ptr(view.v),
-                      _ptr(view.scales[0]), _ptr(view.scales[1]), _ptr(view.page_table), view.max_pages, view.page_size, view.n_kv_heads,
-                      view.head_dim, self._stream())
+        k, v = torch.empty((2, ranges.count, view.n_kv_heads, view.page_size, view.head_dim), dtype=torch.bfloat16, device=self.device)
+        self.lib.call("rb_cache8_values", k.data_ptr(), v.data_ptr(), ranges.items.data_ptr(), ranges.count, *_cache8(view), view.max_pages,
+                      view.page_size, view.n_kv_heads, view.head_dim, self._stream())
         return k, v
 
     def _attention8(self, q, meta, view, n_heads: int, scale: float, window, sinks, softcap: float, keep_first: int):
@@ -786,28 +796,33 @@ class CudaOps:
                 self._check(sinks, torch.float32, "attention sinks")
             self.lib.call("rb_attention_next", _ptr(sinks), float(softcap), keep, launches=0)
         if not in_rows:
-            self.lib.call("rb_attention8_simple", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v), _ptr(view.scales[0]),
-                          _ptr(view.scales[1]), _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos),
-                          _ptr(meta.tok_slot), T, H, Kh, D, float(scale), win, self._stream())
+            self.lib.call("rb_attention8_simple", out.data_ptr(), q.data_ptr(), *_cache8(view), view.max_pages, view.page_size,
+                          meta.tok_pos.data_ptr(), meta.tok_slot.data_ptr(), T, H, Kh, D, float(scale), win, self._stream())
             return out
-        tok0 = ntok = part_o = part_ml = None
-        n_tiles, rows = T, G
-        if not meta.single_token:
-            per_tile = min(most_new, 32 // G)
-            tok0, ntok, n_tiles = self._prefill_tiles(meta, per_tile)
-            rows = per_tile * G
-        # the most keys a row tile can have to visit, in whole tiles
-        context = int(meta.max_context) if not win else min(int(meta.max_context), win + 126 + rows // G + (keep + 63) // 64 * 64)
-        plan = (ctypes.c_longlong * 4)()
-        self.lib.call("rb_attention8_rows_plan", n_tiles, rows, Kh, D, context, plan, launches=0)
-        parts, blocks, n_o, n_ml = plan
+        # how a step's rows are cut is the same for all of its layers of these sizes
+        key = ("attention8", Kh, G, D, win, keep)
+        cut = meta.extra.get(key)
+        if cut is None:
+            tok0 = ntok = None
+            n_tiles, rows = T, G
+            if not meta.single_token:
+                per_tile = min(most_new, 32 // G)
+                tok0, ntok, n_tiles = self._prefill_tiles(meta, per_tile)
+                rows = per_tile * G
+            # the most keys a row tile can have to visit, in whole tiles
+            context = int(meta.max_context) if not win else min(int(meta.max_context), win + 126 + rows // G + (keep + 63) // 64 * 64)
+            plan = (ctypes.c_longlong * 4)()
+            self.lib.call("rb_attention8_rows_plan", n_tiles, rows, Kh, D, context, plan, launches=0)
+            cut = meta.extra[key] = (tok0, ntok, n_tiles, rows, *plan)
+        tok0, ntok, n_tiles, rows, parts, blocks, n_o, n_ml = cut
+        part = None
         if parts == 0:
-            part_o = torch.empty((n_o,), dtype=torch.float32, device=self.device)
-            part_ml = torch.empty((n_ml,), dtype=torch.float32, device=self.device)
-        self.lib.call("rb_attention8_rows", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v), _ptr(view.scales[0]), _ptr(view.scales[1]),
-                      view.k.shape[0], _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos), _ptr(meta.tok_slot), _ptr(tok0),
-                      _ptr(ntok), n_tiles, rows, H, Kh, D, float(scale), win, parts, blocks, _ptr(part_o), _ptr(part_ml),
-                      self._stream(), launches=2 if parts == 0 else 1)
+            part = torch.empty((n_o + n_ml,), dtype=torch.float32, device=self.device)
+        at = _address(part)
+        self.lib.call("rb_attention8_rows", out.data_ptr(), q.data_ptr(), *_cache8(view)[:4], view.k.shape[0], view.page_table.data_ptr(),
+                      view.max_pages, view.page_size, meta.tok_pos.data_ptr(), meta.tok_slot.data_ptr(), _address(tok0), _address(ntok),
+                      n_tiles, rows, H, Kh, D, float(scale), win, parts, blocks, at, at + 4 * n_o, self._stream(),
+                      launches=2 if parts == 0 else 1)
         return out
 
     def _attention_unpacked(self, q, meta, view, n_heads: int, scale: float, window, sinks, softcap: float, keep: int):

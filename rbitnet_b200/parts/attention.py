@@ -98,6 +98,12 @@ class Attention(Mixer):
         return bool(self.value_dim != self.head_dim or self.qk_norm or self.head_gate or self.value_gate
                     or not plain_position or self.prepared)
 
+    @property
+    def cache_in_8_bits(self) -> bool:
+        """Turned q, k and v rows go to the cache by ``ops.rotate_append``, which takes one held in 8 bits; the kernels of the
+        options do not."""
+        return not self.extended
+
     def weight_shapes(self):
         H, K, D, E, Dv = self.n_heads, self.n_kv_heads, self.head_dim, self.width, self.value_dim
         shapes = {"q": ((H * D, E), "matrix"), "k": ((K * D, E), "matrix"),

@@ -89,6 +89,8 @@ class PositionEncoding(Part):
 
 class Mixer(Part):
     role = "mixer"
+    #: whether what the mixer caches may be held in 8 bits (its kernels take a view with scales)
+    cache_in_8_bits = False
 
     def cache_need(self) -> Optional[CacheNeed]:
         return None

@@ -11,6 +11,7 @@ import pytest
 import torch
 
 import plain_cache8 as plain
+from helpers import bf16_rtol
 from rbitnet_b200.cache import CacheLayerView
 from rbitnet_b200.engine.step import SeqChunk, build_meta
 
@@ -280,3 +281,279 @@ def test_verify_at_the_edges(ops):
     a, t = verified(ops, logits, torch.tensor([0, 0, 2], dtype=torch.int32), torch.zeros(9, dtype=torch.int32), torch.zeros(2),
                     torch.zeros(9, 2), 3, None)
     assert a[0] == 0 and t[0] == [-1, -1, -1, -1]
+
+
+# ---- used as a program uses them
+def test_a_step_on_another_stream_with_strided_rows(ops):
+    """Rows that are a part of wider ones, a stream of the caller's own, the result read there."""
+    H, Kh, D = 8, 2, 128
+    view, cpu = make_view(9, Kh, 64, D, 2, 3, seed=11)
+    seqs = [(0, 100, 1), (1, 63, 1)]
+    wide = rows_of(seqs, (H + 2 * Kh) * D + 64, seed=4)
+    x = wide[:, 64:]
+    meta, freq = make_meta(seqs), frequencies(D)
+    on_gpu, side = wide.cuda()[:, 64:], torch.cuda.Stream()
+    rotary = (freq.cuda(), False, D)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        q = ops.rotate_append(on_gpu, rotary, meta, view, H)
+        out = ops.attention(q, meta, view, H, D ** -0.5, None)
+    side.synchronize()
+    r = x.to(F64).view(2, -1, D)
+    for i, (slot, start, n) in enumerate(seqs):
+        t = plain.turned(r[i:i + 1, :H + Kh], torch.tensor([start]), freq, D, False)
+        plain.append(cpu, slot, start, t[:, H:], r[i:i + 1, H + Kh:])
+    assert same_codes(view.v, cpu.v)
+    cpu.k.copy_(view.k.cpu())                   # (a code apart at most: compared in test_append)
+    for i, (slot, start, n) in enumerate(seqs):
+        want, size = plain.attend(cpu, slot, start, q[i:i + 1].cpu(), D ** -0.5)
+        assert torch.all((out[i:i + 1].cpu().to(F64) - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size)
+
+
+@pytest.mark.parametrize("H,Kh,D", [(8, 2, 128), (8, 8, 64), (4, 2, 80)])
+def test_a_captured_step_replayed_at_other_positions(ops, H, Kh, D):
+    """Append and attention of single tokens recorded once: the replays work on the positions, slots and rows that lie in the buffers
+    then, also where two graphs alternate, and give what the calls themselves give, to the bit."""
+    a, _ = make_view(40, Kh, 64, D, 4, 10, seed=12)
+    b, _ = make_view(40, Kh, 64, D, 4, 10, seed=12)
+    rotary = (frequencies(D).cuda(), True, D)
+    x = torch.zeros(3, (H + 2 * Kh) * D, dtype=BF16, device="cuda")
+    metas, graphs, outs = [], [], []
+    side = torch.cuda.Stream()
+    for g in range(2):
+        meta = make_meta([(0, 0, 1), (1, 0, 1), (2, 0, 1)])
+        meta.max_context = 640
+        body = lambda meta=meta: ops.attention(ops.rotate_append(x, rotary, meta, a, H), meta, a, H, D ** -0.5, 100 if g else None)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            body()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(body())
+        metas.append(meta)
+        graphs.append(graph)
+    for t in (a.k, a.v):
+        t.view(torch.uint8).copy_((b.k if t is a.k else b.v).view(torch.uint8))
+    for s, t in zip(a.scales, b.scales):
+        s.copy_(t)
+    gen = torch.Generator().manual_seed(5)
+    for i in range(8):
+        pos = [64 * i + 5, 63 + i, 600 + i]
+        metas[i % 2].tok_pos.copy_(torch.tensor(pos, dtype=torch.int32))
+        metas[i % 2].tok_slot.copy_(torch.tensor([3, 1, i % 2 * 2], dtype=torch.int32))
+        x.copy_((torch.randn(x.shape, generator=gen) * 2.0 ** (i - 3)).to(BF16))
+        graphs[i % 2].replay()
+        eager = make_meta([(3, pos[0], 1), (1, pos[1], 1), (i % 2 * 2, pos[2], 1)])
+        eager.max_context = 640
+        want = ops.attention(ops.rotate_append(x, rotary, eager, b, H), eager, b, H, D ** -0.5, 100 if i % 2 else None)
+        assert torch.equal(outs[i % 2], want), i
+        assert torch.equal(a.k.view(torch.uint8), b.k.view(torch.uint8)) and torch.equal(a.scales[1], b.scales[1])
+
+
+def test_rows_that_do_not_begin_on_16_bytes(ops):
+    H, Kh, D = 4, 2, 64
+    seqs = [(0, 40, 30), (1, 0, 1)]
+    view, cpu = make_view(7, Kh, 64, D, 2, 2, seed=13)
+    other, _ = make_view(7, Kh, 64, D, 2, 2, seed=13)
+    wide = rows_of(seqs, (H + 2 * Kh) * D + 8, seed=5).cuda()
+    rotary = (frequencies(D).cuda(), False, D)
+    q = ops.rotate_append(wide[:, 1:-7], rotary, make_meta(seqs), view, H)
+    want = ops.rotate_append(wide[:, 1:-7].contiguous(), rotary, make_meta(seqs), other, H)
+    # (two kernels: products and sums of float32 pairs, 2^-22 of the row's size apart, may round to different sides in bfloat16)
+    assert torch.all((q.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 2.0 ** -20 * want.float().abs().max())
+    assert same_codes(view.v, other.v.cpu()) and torch.equal(view.scales[1], other.scales[1])
+    # queries that begin elsewhere
+    one = [(0, 60, 1)]
+    base = rows_of(one, H * D + 8, seed=6).cuda()
+    x = base.view(-1)[1:1 + H * D].view(1, H, D)
+    a = ops.attention(x, make_meta(one), view, H, 0.1, None)
+    b = ops.attention(x.clone(), make_meta(one), view, H, 0.1, None)
+    assert float((a.float() - b.float()).abs().max()) <= 2.0 ** -7 * float(b.float().abs().max())
+
+
+def test_masked_places_may_hold_anything(ops):
+    """NaN codes behind a sequence's end and before its window, pages that were given back (-1 places), scales that are NaN there."""
+    H, Kh, D, page = 8, 2, 128, 64
+    for seqs, window, keep in (([(0, 130, 1)], 0, 0), ([(0, 250, 1)], 60, 0), ([(0, 250, 4)], 60, 10), ([(0, 250, 1)], 100, 5)):
+        view, cpu = make_view(12, Kh, page, D, 2, 5, seed=14)
+        start, n = seqs[0][1], seqs[0][2]
+        first = max(0, start - window + 1) if window else 0
+        for pool in (view.k, view.v, cpu.k, cpu.v):
+            codes = pool.view(torch.uint8)
+            for pos in list(range(start + n, 5 * page)) + [p for p in range(first) if p >= keep]:
+                codes[int(cpu.page_table[0, pos // page]), :, pos % page] = 0x7f
+        for i in range(5):                       # whole pages that no row sees
+            if window and (i + 1) * page <= first and i * page >= keep:
+                view.page_table[0, i] = -1
+        q = rows_of(seqs, H * D, seed=7).view(-1, H, D)
+        got = ops.attention(q.cuda(), make_meta(seqs), view, H, D ** -0.5, window, keep_first=keep).cpu().to(F64)
+        # (a row may see a window's older keys that the later rows do not: only what no row sees holds NaN)
+        want, size = plain.attend(cpu, 0, start, q, D ** -0.5, window, None, 0.0, keep)
+        assert torch.isfinite(got).all()
+        assert torch.all((got - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size)
+
+
+def test_blocks_of_very_different_size(ops):
+    """Scales from 2^-60 to 2^100 side by side: the sums stay finite and right where large values have no weight, and where they have."""
+    H, Kh, D, page = 4, 1, 128, 64
+    view, cpu = make_view(8, Kh, page, D, 1, 8, seed=15)
+    for i, e in enumerate((0, 100, -60, 3, 90, -40, 1, -7)):
+        for v in (view, cpu):
+            v.scales[1][int(cpu.page_table[0, i])] = 2.0 ** e
+    for v in (view, cpu):
+        v.scales[0].fill_(2.0 ** -9)
+    q = rows_of([(0, 511, 1)], H * D, seed=8).view(1, H, D)
+    got = ops.attention(q.cuda(), make_meta([(0, 511, 1)]), view, H, D ** -0.5, None).cpu().to(F64)
+    want, size = plain.attend(cpu, 0, 511, q, D ** -0.5)
+    assert torch.all((got - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size)
+    # only the small blocks are seen
+    got = ops.attention(q.cuda(), make_meta([(0, 511, 1)]), view, H, D ** -0.5, 100).cpu().to(F64)
+    want, size = plain.attend(cpu, 0, 511, q, D ** -0.5, 100)
+    assert torch.all((got - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size)
+
+
+def test_many_sequences_of_unequal_lengths(ops):
+    """More pairs than blocks: all tiles are dealt out, pairs are shared by blocks and joined again; steps of one and of several tokens."""
+    for H, Kh, D, new in ((32, 8, 128, 1), (16, 16, 64, 1), (8, 2, 128, 5), (7, 1, 64, 4)):
+        B, max_pages = 40, 24
+        view, cpu = make_view(B * max_pages, Kh, 64, D, B, max_pages, seed=H)
+        seqs = [(B - 1 - i, (i * 37 * (1 + i % 5)) % (24 * 64 - new), 1 + i % new) for i in range(B)]
+        q = rows_of(seqs, H * D, seed=9).view(-1, H, D)
+        got = ops.attention(q.cuda(), make_meta(seqs), view, H, D ** -0.5, None).cpu().to(F64)
+        at = 0
+        for slot, start, n in seqs:
+            want, size = plain.attend(cpu, slot, start, q[at:at + n], D ** -0.5)
+            assert torch.all((got[at:at + n] - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size), (H, slot)
+            at += n
+
+
+def test_prompts_through_bfloat16_pages_and_through_codes_are_the_same_attention(ops):
+    """The rule between the two is one of speed: rows of a few tokens either way."""
+    H, Kh, D = 8, 2, 128
+    seqs = [(0, 100, 7), (1, 0, 7), (2, 300, 2)]
+    view, _ = make_view(30, Kh, 64, D, 3, 6, seed=16)
+    q = rows_of(seqs, H * D, seed=10).view(-1, H, D).cuda()
+    a = ops.attention(q, make_meta(seqs), view, H, D ** -0.5, None)
+    kept, ops.cache8_rows = ops.cache8_rows, 0
+    try:
+        b = ops.attention(q, make_meta(seqs), view, H, D ** -0.5, None)
+    finally:
+        ops.cache8_rows = kept
+    assert float((a.float() - b.float()).abs().max()) <= 2.0 ** -6 * float(b.float().abs().max())
+
+
+def test_verify_of_rows_that_are_part_of_wider_ones_and_of_long_vocabularies(ops):
+    case = list(drafts_case(3, 2, 5003, False, 5))
+    wide, wide_p = torch.randn(case[0].shape[0], 6001), torch.rand(case[0].shape[0], 5500)
+    wide[:, 3:5006], wide_p[:, 1:5004] = case[0], case[6]
+    a, t = ops.verify_drafts(wide.cuda()[:, 3:5006], case[1].cuda(), case[2].cuda(), case[3].cuda(), case[4].cuda(), 2,
+                             draft_probs=wide_p.cuda()[:, 1:5004])
+    assert (a.tolist(), t.tolist()) == plain.verify(*case)
+    case = drafts_case(2, 2, 300001, False, 6)
+    assert verified(ops, *case) == plain.verify(*case)
+    # a draft on the very border of acceptance: float32 sums leave it open
+    z = torch.randn(2, 40000, generator=torch.Generator().manual_seed(2)) * 2
+    p = torch.softmax(z[0].double(), 0)
+    top = int(p.argmax())
+    for d in (-3, -1, 0, 1, 3):
+        u = torch.full((2, 2), float(p[top]) * (1 + d * 2.0 ** -22))
+        case = (z, torch.tensor([0, 2], dtype=torch.int32), torch.tensor([top, 0], dtype=torch.int32), torch.ones(1), u, 1, None)
+        assert verified(ops, *case) == plain.verify(*case), d
+
+
+def test_verify_captured_twice_and_replayed_in_turn(ops):
+    cases = [drafts_case(4, 3, 3000, True, s, ragged=False) for s in (1, 2)]
+    held = [[t.cuda() for t in c[:5]] for c in cases]
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for h in held:
+        ops.verify_drafts(*h, 3)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.verify_drafts(*h, 3))
+        graphs.append(g)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for c, (a, t) in zip(cases, outs):
+            assert (a.tolist(), t.tolist()) == plain.verify(*c)
+
+
+# ---- the engine
+def test_a_run_of_them_together():
+    """A model whose heads the fast kernels take: prompts, drafted steps, decode steps (captured), over a cache of 8 bits.  Logits are
+    near the bfloat16 cache's (a tenth of the largest: what codes of four digits move, see the CPU tests); the tokens that drafted steps
+    give are the arg-max of the logits that plain steps over the same cache give, but for near ties."""
+    from rbitnet_b200 import Engine, StepEntry
+    cfg = dict(architectures=["LlamaForCausalLM"], num_hidden_layers=2, hidden_size=512, num_attention_heads=8, num_key_value_heads=2,
+               head_dim=64, intermediate_size=1024, vocab_size=1000, rope_theta=10000.0, rms_norm_eps=1e-5, max_position_embeddings=1024,
+               tie_word_embeddings=False, hidden_act="silu")
+    kw = dict(seed=5, dtype="bfloat16", max_tokens=8192, max_batch=8)
+    full, half = Engine.from_random(cfg, **kw), Engine.from_random(cfg, cache_dtype="float8_e4m3", **kw)
+    assert half.cache.bytes() < 0.52 * full.cache.bytes() and "cache=" in half.model_summary()
+    g = torch.Generator().manual_seed(1)
+    ps = [torch.randint(0, 1000, (n,), generator=g).tolist() for n in (300, 64, 63, 1, 130)]
+    rows = []
+    for eng in (full, half):
+        slots = [eng.new_sequence() for _ in ps]
+        out = [eng.step([StepEntry(s, p, [len(p) - 1]) for s, p in zip(slots, ps)])]
+        for i in range(70):
+            out.append(eng.step([StepEntry(s, [(7 * i + j) % 1000], [0]) for j, s in enumerate(slots)], captured=i % 2 == 0))
+        out.append(eng.step([StepEntry(s, [3, 4, 5 + j, 6], [0, 3]) for j, s in enumerate(slots)]))
+        rows.append(torch.cat(out))
+        for s in slots:
+            eng.end_sequence(s)
+        eng.ops.check_errors()
+    size = float(rows[0].abs().max())
+    assert 0 < float((rows[0] - rows[1]).abs().max()) <= 0.1 * size
+    again = [p + p[-40:] for p in ps]
+    plainly = half.generate(again, max_tokens=40, temperature=0.0, stop_ids=[])
+    drafted = half.generate(again, max_tokens=40, temperature=0.0, stop_ids=[], draft_tokens=4)
+    assert half.last_stats["drafted_tokens"] > 0 and half.last_stats["steps"] <= 40
+    for p, a, b in zip(again, plainly, drafted):
+        assert len(b.tokens) == 40
+        if a.tokens == b.tokens:
+            continue
+        at = next(i for i in range(40) if a.tokens[i] != b.tokens[i])
+        slot = half.new_sequence()
+        z = half.step([StepEntry(slot, p + a.tokens[:at], [len(p) + at - 1])])[0]
+        half.end_sequence(slot)
+        # a near tie: two logits, each off by the band of two layers in bfloat16 (helpers.bf16_rtol: 1.7 % of the largest)
+        assert abs(float(z[a.tokens[at]] - z[b.tokens[at]])) <= 2 * bf16_rtol(2) * float(z.abs().max()), at
+    sampled = half.generate(again, max_tokens=20, temperature=0.8, seed=3, stop_ids=[], draft_tokens=4)
+    assert [len(r.tokens) for r in sampled] == [20] * len(ps)
+    assert [r.tokens for r in half.generate(again, max_tokens=20, temperature=0.8, seed=3, stop_ids=[], draft_tokens=4)] == [r.tokens for r in sampled]
+
+
+def test_the_checked_build_sees_addresses_outside_the_8_bit_cache():
+    """In a process of its own with RBITNET_CHECKED: a slot and a position outside are recorded, not read or written."""
+    import os
+    import subprocess
+    import sys
+    code = '''
+import torch, sys
+sys.path[:0] = ["tests"]
+from test_gpu_cache8 import make_view, make_meta, rows_of, BF16
+from rbitnet_b200.kernels.ops import CudaOps
+from rbitnet_b200.kernels.lib import KernelError
+ops = CudaOps(BF16)
+view, _ = make_view(4, 2, 64, 128, 2, 2)
+for bad in (lambda m: ops.rotate_append(rows_of([(0, 0, 1)], 8 * 128).cuda(), None, m, view, 4),
+            lambda m: ops.attention(rows_of([(0, 0, 1)], 4 * 128).view(1, 4, 128).cuda(), m, view, 4, 0.1, None)):
+    meta = make_meta([(0, 64 * 2, 1)])
+    bad(meta)
+    torch.cuda.synchronize()
+    try:
+        ops.check_errors()
+        print("not seen")
+    except KernelError as e:
+        assert "checked build" in str(e), e
+        print("seen")
+'''
+    env = dict(os.environ, RBITNET_CHECKED="1")
+    out = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), env=env,
+                         capture_output=True, text=True, timeout=600)
+    assert out.returncode == 0 and out.stdout.split() == ["seen", "seen"], out.stdout + out.stderr
