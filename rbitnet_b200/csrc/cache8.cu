@@ -389,14 +389,18 @@ __global__ void __launch_bounds__(256) append8_step_kernel(Append8 p) {
   }
 }
 
-// The values of whole pages: item i is (slot, page of the sequence, positions in use); what lies behind those is zero.
+// The values of whole pages: item i is (slot, page of the sequence, positions in use); what lies behind those is zero, and all of a page
+// that the sequence has given back (a negative number in its table).
+__device__ __forceinline__ int in_use(const RbPagedLayer& c, int slot, int page, int used) {
+  return c.page_table[(int64_t)slot * c.max_pages + page] < 0 ? 0 : used;
+}
 __global__ void __launch_bounds__(256) cache8_values_kernel(__nv_bfloat16* k_out, __nv_bfloat16* v_out, RbPagedLayer c, const float* k_scale,
                                                            const float* v_scale, const int* items, int block) {
   rb_pdl_launch_dependents();
   const int i = blockIdx.x, kvh = blockIdx.y, D = c.head_dim, n = c.page_size * D;
-  const int slot = items[3 * i], page = items[3 * i + 1], used = items[3 * i + 2];
+  const int slot = items[3 * i], page = items[3 * i + 1], used = in_use(c, slot, page, items[3 * i + 2]);
   rb_pdl_wait();
-  const int64_t at = rb_page_offset(c, slot, page * c.page_size, kvh), to = ((int64_t)i * c.n_kv_heads + kvh) * n;
+  const int64_t at = used > 0 ? rb_page_offset(c, slot, page * c.page_size, kvh) : 0, to = ((int64_t)i * c.n_kv_heads + kvh) * n;
   const uint8_t* k = (const uint8_t*)c.k + at;
   const uint8_t* v = (const uint8_t*)c.v + at;
   const int64_t s = at / ((int64_t)block * D);
@@ -413,9 +417,9 @@ __global__ void __launch_bounds__(256) cache8_values16_kernel(__nv_bfloat16* k_o
                                                              const float* v_scale, const int* items, int block) {
   rb_pdl_launch_dependents();
   const int i = blockIdx.x, kvh = blockIdx.y, D = c.head_dim, n = c.page_size * D;
-  const int slot = items[3 * i], page = items[3 * i + 1], used = items[3 * i + 2];
+  const int slot = items[3 * i], page = items[3 * i + 1], used = in_use(c, slot, page, items[3 * i + 2]);
   rb_pdl_wait();
-  const int64_t at = rb_page_offset(c, slot, page * c.page_size, kvh), to = ((int64_t)i * c.n_kv_heads + kvh) * n;
+  const int64_t at = used > 0 ? rb_page_offset(c, slot, page * c.page_size, kvh) : 0, to = ((int64_t)i * c.n_kv_heads + kvh) * n;
   const uint8_t* in = (const uint8_t*)(blockIdx.z ? c.v : c.k) + at;
   const float* scale = (blockIdx.z ? v_scale : k_scale) + at / ((int64_t)block * D);
   __nv_bfloat16* out = (blockIdx.z ? v_out : k_out) + to;

@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(Verify p, int
   }
   // ---- the token: sums over the blocks' and the warps' shares
   const float* z = p.logits + (int64_t)r * p.stride;
-  const int d = r + 1 < r1 ? p.drafts[r] : -1;
+  const int d = r + 1 < r1 && r - r0 < p.most ? p.drafts[r] : -1;
   const bool judged = d >= 0 && d < p.V;
   const float* q = judged && p.probs ? p.probs + (int64_t)r * p.probs_stride : nullptr;
   const float m = s_m;

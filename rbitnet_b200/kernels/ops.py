@@ -264,6 +264,10 @@ class CudaOps:
         index = self.device.index
         return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index))
 
+    def _raw_stream(self) -> int:
+        index = self.device.index
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
     def _check(self, t: torch.Tensor, dtype, what: str):
         if t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
             raise KernelError(f"{what}: expected a contiguous {dtype} CUDA tensor, found {t.dtype} "
@@ -694,15 +698,16 @@ class CudaOps:
     # ------------------------------------------------------------------ the cache held in 8 bits
     def _check_cache8(self, view, what: str) -> int:
         """Refuses what the 8-bit kernels do not take; returns the positions of a block."""
-        (k, v), (ks, vs), table, page = (view.k, view.v), view.scales, view.page_table, view.page_size
+        k, v, (ks, vs), table, page = view.k, view.v, view.scales, view.page_table, view.page_size
         block = page if 0 < page <= 64 else (64 if page > 0 and page % 64 == 0 else 0)
-        shape = k.shape
-        if (self.dtype == torch.bfloat16 and block and k.dtype == v.dtype == torch.float8_e4m3fn and k.is_cuda and table.dtype == torch.int32
-                and ks.dtype == vs.dtype == torch.float32 and k.device == v.device == ks.device == vs.device == table.device
-                and shape == v.shape == (shape[0], view.n_kv_heads, page, view.head_dim)
-                and ks.shape == vs.shape == (shape[0], view.n_kv_heads, page // block)
-                and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and table.is_contiguous()
-                and table.dim() == 2 and table.shape[1] == view.max_pages):
+        pages, device, code, f32 = k.shape[0], k.get_device(), torch.float8_e4m3fn, torch.float32
+        # (what a step calls for every layer: as few looks at the tensors as say it all)
+        if (self.dtype is torch.bfloat16 and block and device >= 0 and k.dtype is code and v.dtype is code and ks.dtype is f32 and vs.dtype is f32
+                and table.dtype is torch.int32 and v.get_device() == device == ks.get_device() and vs.get_device() == device == table.get_device()
+                and k.shape == (pages, view.n_kv_heads, page, view.head_dim) and v.shape == k.shape
+                and ks.shape == (pages, view.n_kv_heads, page // block) and vs.shape == ks.shape and table.dim() == 2
+                and table.shape[1] == view.max_pages and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous()
+                and vs.is_contiguous() and table.is_contiguous()):
             return block
         if self.dtype != torch.bfloat16:
             raise KernelError(f"{what}: a cache held in 8 bits goes with the bfloat16 mode, not with {self.dtype}")
@@ -744,10 +749,10 @@ class CudaOps:
             raise KernelError(f"rotate_append: expected {self.dtype} CUDA rows, found {qkv.dtype} on {qkv.device}")
         inv_freq, interleaved, rot_dim = (self._zeros_freq(D), False, 0) if rotary is None else rotary
         tok0, ntok, n_tiles = self._block_tiles(meta, block)
-        q = torch.empty((T, n_heads, D), dtype=self.dtype, device=self.device)
+        q = qkv.new_empty((T, n_heads, D))
         self.lib.call("rb_append8", q.data_ptr(), qkv.data_ptr(), qkv.stride(0), inv_freq.data_ptr(), meta.tok_pos.data_ptr(),
                       meta.tok_slot.data_ptr(), _address(tok0), _address(ntok), n_tiles, *_cache8(view), view.max_pages, view.page_size,
-                      n_heads, Kh, D, 1 if view.writes else 0, rot_dim, 1 if interleaved else 0, self._stream())
+                      n_heads, Kh, D, 1 if view.writes else 0, rot_dim, 1 if interleaved else 0, self._raw_stream())
         return q
 
     def cache_ranges(self, view, ranges) -> CacheRanges:
@@ -772,7 +777,7 @@ class CudaOps:
         self._check_cache8(view, "cache_values")
         k, v = torch.empty((2, ranges.count, view.n_kv_heads, view.page_size, view.head_dim), dtype=torch.bfloat16, device=self.device)
         self.lib.call("rb_cache8_values", k.data_ptr(), v.data_ptr(), ranges.items.data_ptr(), ranges.count, *_cache8(view), view.max_pages,
-                      view.page_size, view.n_kv_heads, view.head_dim, self._stream())
+                      view.page_size, view.n_kv_heads, view.head_dim, self._raw_stream())
         return k, v
 
     def _attention8(self, q, meta, view, n_heads: int, scale: float, window, sinks, softcap: float, keep_first: int):
@@ -780,15 +785,21 @@ class CudaOps:
         Kh, win = view.n_kv_heads, int(window or 0)
         self._check_cache8(view, "attention")
         self._check(q, self.dtype, "attention queries")
-        if D != view.head_dim or H != n_heads or H % Kh:
-            raise KernelError(f"attention: {H} heads of {D} values on {Kh} kv heads of {view.head_dim}")
+        if D != view.head_dim or H != n_heads or H % Kh or T != meta.n_tokens:
+            raise KernelError(f"attention: {T} rows of {H} heads of {D} values, expected {meta.n_tokens} of {n_heads} on {Kh} kv heads of "
+                              f"{view.head_dim}")
         keep = int(keep_first or 0) if win else 0
-        G, most_new = H // Kh, 1 if meta.single_token else max((c.n_new for c in meta.seqs), default=1)
-        aligned = not (q.data_ptr() | view.k.data_ptr() | view.v.data_ptr()) % 16
-        in_rows = aligned and self.lib.raw("rb_attention8_rows_supports")(H, Kh, D, view.page_size)
-        if not meta.single_token and not (in_rows and most_new * G <= self.cache8_rows):
+        # how a step's rows are cut is the same for all of its layers of these sizes
+        key = ("attention8", H, Kh, D, win, keep, self.cache8_rows)
+        cut = meta.extra.get(key)
+        if cut is None:
+            cut = meta.extra[key] = self._cut_rows8(meta, view, T, H, Kh, D, win, keep)
+        in_rows, tok0, ntok, n_tiles, rows, parts, blocks, n_o, n_ml = cut
+        at_q, cache = q.data_ptr(), _cache8(view)
+        in_rows = in_rows and not (at_q | cache[0] | cache[1]) & 15
+        if not in_rows and not meta.single_token:
             return self._attention_unpacked(q, meta, view, n_heads, scale, window, sinks, softcap, keep)
-        out = torch.empty((T, H * D), dtype=self.dtype, device=self.device)
+        out = q.new_empty((T, H * D))
         if T == 0:
             return out
         if sinks is not None or softcap > 0.0 or keep > 0:
@@ -796,34 +807,33 @@ class CudaOps:
                 self._check(sinks, torch.float32, "attention sinks")
             self.lib.call("rb_attention_next", _ptr(sinks), float(softcap), keep, launches=0)
         if not in_rows:
-            self.lib.call("rb_attention8_simple", out.data_ptr(), q.data_ptr(), *_cache8(view), view.max_pages, view.page_size,
-                          meta.tok_pos.data_ptr(), meta.tok_slot.data_ptr(), T, H, Kh, D, float(scale), win, self._stream())
+            self.lib.call("rb_attention8_simple", out.data_ptr(), at_q, *cache, view.max_pages, view.page_size, meta.tok_pos.data_ptr(),
+                          meta.tok_slot.data_ptr(), T, H, Kh, D, float(scale), win, self._raw_stream())
             return out
-        # how a step's rows are cut is the same for all of its layers of these sizes
-        key = ("attention8", Kh, G, D, win, keep)
-        cut = meta.extra.get(key)
-        if cut is None:
-            tok0 = ntok = None
-            n_tiles, rows = T, G
-            if not meta.single_token:
-                per_tile = min(most_new, 32 // G)
-                tok0, ntok, n_tiles = self._prefill_tiles(meta, per_tile)
-                rows = per_tile * G
-            # the most keys a row tile can have to visit, in whole tiles
-            context = int(meta.max_context) if not win else min(int(meta.max_context), win + 126 + rows // G + (keep + 63) // 64 * 64)
-            plan = (ctypes.c_longlong * 4)()
-            self.lib.call("rb_attention8_rows_plan", n_tiles, rows, Kh, D, context, plan, launches=0)
-            cut = meta.extra[key] = (tok0, ntok, n_tiles, rows, *plan)
-        tok0, ntok, n_tiles, rows, parts, blocks, n_o, n_ml = cut
-        part = None
-        if parts == 0:
-            part = torch.empty((n_o + n_ml,), dtype=torch.float32, device=self.device)
-        at = _address(part)
-        self.lib.call("rb_attention8_rows", out.data_ptr(), q.data_ptr(), *_cache8(view)[:4], view.k.shape[0], view.page_table.data_ptr(),
-                      view.max_pages, view.page_size, meta.tok_pos.data_ptr(), meta.tok_slot.data_ptr(), _address(tok0), _address(ntok),
-                      n_tiles, rows, H, Kh, D, float(scale), win, parts, blocks, at, at + 4 * n_o, self._stream(),
-                      launches=2 if parts == 0 else 1)
+        scratch = None if parts else torch.empty((n_o + n_ml,), dtype=torch.float32, device=q.device)
+        part = _address(scratch)
+        self.lib.call("rb_attention8_rows", out.data_ptr(), at_q, *cache[:4], view.k.shape[0], cache[4], view.max_pages, view.page_size,
+                      meta.tok_pos.data_ptr(), meta.tok_slot.data_ptr(), _address(tok0), _address(ntok), n_tiles, rows, H, Kh, D,
+                      float(scale), win, parts, blocks, part, part + 4 * n_o, self._raw_stream(), launches=1 if parts else 2)
         return out
+
+    def _cut_rows8(self, meta, view, T: int, H: int, Kh: int, D: int, win: int, keep: int):
+        """(whether the kernel of few rows takes them, its row tiles, its parts and scratch: csrc/attention8_rows.cuh)."""
+        G, most_new = H // Kh, 1 if meta.single_token else max((c.n_new for c in meta.seqs), default=1)
+        if not self.lib.raw("rb_attention8_rows_supports")(H, Kh, D, view.page_size) or T == 0 or \
+                (not meta.single_token and most_new * G > self.cache8_rows):
+            return (False,) + (None,) * 8
+        tok0 = ntok = None
+        n_tiles, rows = T, G
+        if not meta.single_token:
+            per_tile = min(most_new, 32 // G)
+            tok0, ntok, n_tiles = self._prefill_tiles(meta, per_tile)
+            rows = per_tile * G
+        # the most keys a row tile can have to visit, in whole tiles
+        context = int(meta.max_context) if not win else min(int(meta.max_context), win + 126 + rows // G + (keep + 63) // 64 * 64)
+        plan = (ctypes.c_longlong * 4)()
+        self.lib.call("rb_attention8_rows_plan", n_tiles, rows, Kh, D, context, plan, launches=0)
+        return (True, tok0, ntok, n_tiles, rows, *plan)
 
     def _attention_unpacked(self, q, meta, view, n_heads: int, scale: float, window, sinks, softcap: float, keep: int):
         """Many rows a sequence: the codes that the step sees become bfloat16 pages once, and the attention over those follows
@@ -1828,12 +1838,11 @@ class CudaOps:
             raise KernelError(f"verify_drafts draft probabilities: expected {(R, V)}, found {tuple(draft_probs.shape)}")
         if B < 0 or most < 0 or V < 1:
             raise KernelError(f"verify_drafts: {B} sequences of at most {most} drafts, {V} logits a row")
-        accepted = torch.empty((B,), dtype=torch.int32, device=self.device)
-        tokens = torch.empty((B, most + 1), dtype=torch.int32, device=self.device)
-        scratch = torch.empty((max(1, self.lib.raw("rb_verify_scratch_bytes")(R, V)),), dtype=torch.uint8, device=self.device)
-        self.lib.call("rb_verify", _ptr(accepted), _ptr(tokens), _ptr(logits), logits.stride(0), _ptr(draft_probs),
-                      0 if draft_probs is None else draft_probs.stride(0), _ptr(first_row), _ptr(drafts), _ptr(temperature),
-                      _ptr(uniforms), B, R, V, most, _ptr(scratch), self._stream(), launches=2)
+        accepted, tokens = first_row.new_empty((B,)), first_row.new_empty((B, most + 1))
+        scratch = first_row.new_empty(((self.lib.raw("rb_verify_scratch_bytes")(R, V) + 3) // 4,))
+        self.lib.call("rb_verify", accepted.data_ptr(), tokens.data_ptr(), logits.data_ptr(), logits.stride(0), _address(draft_probs),
+                      0 if draft_probs is None else draft_probs.stride(0), first_row.data_ptr(), drafts.data_ptr(),
+                      temperature.data_ptr(), uniforms.data_ptr(), B, R, V, most, scratch.data_ptr(), self._raw_stream(), launches=2)
         return accepted, tokens
 
     def decode_advance(self, token_ids: torch.Tensor, tok_pos: torch.Tensor, sampled: torch.Tensor,
