@@ -1,9 +1,8 @@
 // Attention over the cache held in 8 bits for few rows a sequence: a decode step, drafted tokens.
 //
-// One block of four warps works for ONE kv head and a tile of at most 8 NT rows, (token, query head) pairs of one sequence
-// whose heads share the kv head, over a range of its keys in tiles of 64 (a page, or an aligned part of one: one scale each
-// of keys and of values).  A warp takes 32 keys of every other tile at a time
-// and keeps a softmax of its own; they are joined at the end.
+// One block of four warps works for ONE kv head and a tile of at most 8 NT rows, (token, query head) pairs of one sequence whose heads
+// share the kv head, over a range of its keys in tiles of 64 (a page, or an aligned part of one: one scale each of keys and of
+// values).  A warp takes 32 keys of every other tile at a time and keeps a softmax of its own; the warps are joined at the end.
 //
 // The products are mma.sync m16n8k16 in float16 with the KEYS as the 16 rows of the first, and the head's values as the 16 rows of the
 // second, so that eight query rows fill an instruction:
@@ -23,6 +22,13 @@
 // Ranges of keys: in a small grid the parts of a (tile, kv head) are a thread-block cluster and merge on chip.  In a larger one
 // all tiles of keys of all (row tile, kv head) pairs, in order, are dealt out evenly to the blocks, whatever the sequences' lengths; a
 // pair that several blocks have worked on is merged by a second kernel.
+//
+// Bounded by the cache's bytes where sequences are long: one B200, 64 sequences of up to 8,000 positions, 32 heads on 8 kv heads of 128:
+// 541 MB in 90 us, 6.0 TB/s (0.92 of a copy).  Short pairs are bound by what a pair costs to begin and to join (about 5 us a block, two
+// blocks an SM): 24 sequences of 32 heads with a window of 1,024, 202 MB in 49 us.  More rows add products and exponentials: 16
+// sequences of up to five tokens at up to 6,001 positions, 20 rows, 101 MB in 40 us.  One sequence at 2,048 positions: 8 us, waits.
+// Measured beside it (the first of these): 16-byte cp.async by every thread 154 us, of which the copies alone 136; boxes of 16 positions
+// 126 to 136; two stages and three blocks an SM 109; pairs dealt out without what their beginnings cost 113.
 #pragma once
 
 #include "attention8.cuh"
@@ -828,31 +834,34 @@ template <int D, int NT> int per_sm() {
   }
   return n[dev];
 }
-// the most parts that a cluster may have: 16 where the device runs such clusters of this kernel, else 8 (asked once)
-template <int D, int NT> int cluster_most() {
-  static int answer = 0;
-  if (answer == 0) {
+// Clusters of `parts` blocks (2, 4, 8 or 16) that run together on the device (asked once): the GPCs' sizes leave fewer than the SMs' places
+// would (72 clusters of 4 took two rounds where 296 blocks have places), and none of 16 on some devices.
+template <int D, int NT> int clusters_at_once(int parts) {
+  static int answer[RB_MAX_DEVICES][5] = {};
+  int dev = 0, i = parts == 2 ? 1 : parts == 4 ? 2 : parts == 8 ? 3 : 4;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= RB_MAX_DEVICES) dev = 0;
+  if (answer[dev][i] == 0) {
     per_sm<D, NT>();
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1, 1, 16);
+    cfg.gridDim = dim3(1, 1, parts);
     cfg.blockDim = dim3(WARPS * 32, 1, 1);
     cfg.dynamicSmemBytes = Shape<D, NT>::BYTES;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
     attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 16;
+    attr[0].val.clusterDim.z = parts;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    answer = cudaOccupancyMaxActiveClusters(&n, cluster_kernel<D, NT>, &cfg) == cudaSuccess && n >= 1 ? 16 : 8;
-    (void)cudaGetLastError();
+    answer[dev][i] = cudaOccupancyMaxActiveClusters(&n, cluster_kernel<D, NT>, &cfg) == cudaSuccess && n >= 1 ? n : -1;
+    (void)cudaGetLastError();      // a refusal is an answer, not an error of a later launch
   }
-  return answer;
+  return answer[dev][i];
 }
-inline int most_parts(int D, int NT) {
-  return D == 64 ? (NT == 1 ? cluster_most<64, 1>() : NT == 2 ? cluster_most<64, 2>() : NT == 3 ? cluster_most<64, 3>() : cluster_most<64, 4>())
-                 : (NT == 1 ? cluster_most<128, 1>() : NT == 2 ? cluster_most<128, 2>() : NT == 3 ? cluster_most<128, 3>() : cluster_most<128, 4>());
+inline int clusters(int D, int NT, int parts) {
+  return D == 64 ? (NT == 1 ? clusters_at_once<64, 1>(parts) : NT == 2 ? clusters_at_once<64, 2>(parts) : NT == 3 ? clusters_at_once<64, 3>(parts) : clusters_at_once<64, 4>(parts))
+                 : (NT == 1 ? clusters_at_once<128, 1>(parts) : NT == 2 ? clusters_at_once<128, 2>(parts) : NT == 3 ? clusters_at_once<128, 3>(parts) : clusters_at_once<128, 4>(parts));
 }
 inline int places(int D, int NT) {
   const int n = D == 64 ? (NT == 1 ? per_sm<64, 1>() : NT == 2 ? per_sm<64, 2>() : NT == 3 ? per_sm<64, 3>() : per_sm<64, 4>())
@@ -905,12 +914,12 @@ RB_EXPORT int rb_attention8_rows_supports(int H, int Kh, int D, int page_size) {
 // A cluster where two parts of every pair and more fit the SMs at once and no part is long; else all tiles are dealt out to as many
 // blocks as the SMs hold at once, four tiles to a block at least.
 RB_EXPORT int rb_attention8_rows_plan(int n_tiles, int rows, int Kh, int D, int context, long long* out4) {
-  const int NT = (rows + 7) / 8, places = rows8::places(D, NT), most = rows8::most_parts(D, NT);
+  const int NT = (rows + 7) / 8, places = rows8::places(D, NT);
   const int tiles = (context + rows8::TILE - 1) / rows8::TILE;
   const long long pairs = (long long)n_tiles * Kh;
   RB_REQUIRE(n_tiles > 0 && Kh > 0 && rows > 0 && rows <= 32, "rb_attention8_rows_plan: %d tiles of %d rows, %d kv heads", n_tiles, rows, Kh);
   int parts = 1;
-  while (parts * 2 <= tiles && parts < most && pairs * parts * 2 <= places) parts *= 2;
+  while (parts * 2 <= tiles && parts < 16 && pairs <= rows8::clusters(D, NT, parts * 2)) parts *= 2;
   out4[0] = parts; out4[1] = out4[2] = out4[3] = 0;
   if (tiles <= 1 || (parts > 1 && tiles <= 16 * parts)) return 0;
   long long blocks = (pairs * tiles + 3) / 4;
@@ -934,7 +943,7 @@ RB_EXPORT int rb_attention8_rows(void* out, const void* q, void* cache_k, void* 
              "rb_attention8_rows: sizes H=%d Kh=%d D=%d page=%d, %d rows not supported", H, Kh, D, page_size, rows);
   RB_REQUIRE(n_pages * Kh * page_size / rows8::TILE <= 2147483647ll && n_pages * Kh * page_size * D / 128 <= 2147483647ll,
              "rb_attention8_rows: a pool of %lld pages has too many blocks", n_pages);
-  RB_REQUIRE(parts >= 0 && parts <= rows8::most_parts(D, (rows + 7) / 8) && (parts > 0 || (blocks > 0 && part_o && part_ml)), "rb_attention8_rows: %d parts, %d blocks", parts, blocks);
+  RB_REQUIRE(parts >= 0 && parts <= 16 && (parts & (parts - 1)) == 0 && (parts > 0 || (blocks > 0 && part_o && part_ml)), "rb_attention8_rows: %d parts, %d blocks", parts, blocks);
   rows8::Params p;
   p.a.q = (const __nv_bfloat16*)q; p.a.out = (__nv_bfloat16*)out;
   p.a.cache = RbPagedLayer{cache_k, cache_v, page_table, max_pages, page_size, Kh, D};

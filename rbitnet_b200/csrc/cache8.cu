@@ -103,7 +103,7 @@ struct Append8 {
   int block, H, write_kv, interleaved, rot_dim;
 };
 
-// One block of threads per (tile, kv head): a tile is the new rows of one block of positions.  It turns the tile's query heads
+// Any sizes.  One block of threads per (tile, kv head): a tile is the new rows of one block of positions.  It turns the tile's query heads
 // of the kv head, then makes its keys and its values, each through shared memory because the scale comes before the codes.
 __global__ void __launch_bounds__(256) append8_kernel(Append8 p) {
   rb_pdl_launch_dependents();
@@ -224,8 +224,10 @@ __device__ __forceinline__ float largest8(const float (&a)[8], const float (&b)[
 // eight pairs of one token (SPAN of them where a head is long), and of that piece everything: it makes the sines and cosines once, in
 // registers, turns the key's piece and those of the G query heads with them, and keeps the key's and the value's pieces until the
 // block's largest values have met.  16-byte loads and stores; the blocks of a tile's kv heads run side by side, so that rows are read whole.
-// What bounds it is the chain of waits of a block (tile, positions, rows, the largest values), hidden behind the blocks beside it.
-template <int THREADS, int SPAN>
+// What bounds it is the chain of waits of a block (tile, positions, rows, the largest values), hidden behind the blocks beside it: 8,192
+// tokens of 32 heads on 8 kv heads of 128, 184 MB in 46 us, 4.0 TB/s (sines and cosines through shared memory, 256 threads: 64 us; 92
+// registers and one block an SM 60).  16 sequences of up to five tokens, 32 heads of 64 on 4: 2.4 us.
+template <int THREADS, int SPAN, bool SHARED>
 __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append8_tiles_kernel(Append8 p) {
   rb_pdl_launch_dependents();
   __shared__ float tops[2][THREADS / 32];
@@ -239,12 +241,14 @@ __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append
     at = rb_page_offset(p.cache, slot, pos0 - before, kvh);                   // of the block's first code
     unit = at / ((int64_t)p.block * D);
   }
+  // the thread's pieces; SHARED (tiles of few tokens): groups of threads share the query heads, the first has the key and the value too
+  const int per = n * pieces, groups = SHARED ? min(THREADS / per, G) : 1, group = SHARED ? (int)threadIdx.x / per : 0;
   int tok[SPAN], e[SPAN];
   float2 sc[SPAN][8];
 #pragma unroll
   for (int i = 0; i < SPAN; ++i) {
-    const int item = i * THREADS + threadIdx.x;
-    tok[i] = item / pieces;
+    const int item = i * THREADS + (int)threadIdx.x - group * per;
+    tok[i] = group < groups ? item / pieces : n;
     e[i] = item % pieces;
     if (p.rot_dim && tok[i] < n) turns8(p, pos0 + tok[i], e[i], sc[i]);        // (frequencies and positions need no wait)
   }
@@ -258,7 +262,7 @@ __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append
 #pragma unroll
       for (int i = 0; i < SPAN; ++i) {
         raw[s][i][0] = raw[s][i][1] = make_uint4(0, 0, 0, 0);
-        if (tok[i] < n) {
+        if (tok[i] < n && group == 0) {
           const __nv_bfloat16* src = rows + (int64_t)tok[i] * p.qkv_stride + (int64_t)(p.H + s * Kh + kvh) * D;
           raw[s][i][0] = *reinterpret_cast<const uint4*>(src + piece_a(p, e[i]));
           raw[s][i][1] = *reinterpret_cast<const uint4*>(src + piece_b(p, e[i]));
@@ -273,7 +277,7 @@ __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append
     const __nv_bfloat16* src = rows + (int64_t)tok[i] * p.qkv_stride + (int64_t)kvh * G * D;
     __nv_bfloat16* dst = p.q_out + ((int64_t)(tok0 + tok[i]) * p.H + kvh * G) * D;
 #pragma unroll 4
-    for (int g = 0; g < G; ++g) {
+    for (int g = group; g < G; g += groups) {
       const uint4 qa = *reinterpret_cast<const uint4*>(src + g * D + piece_a(p, e[i])), qb = *reinterpret_cast<const uint4*>(src + g * D + piece_b(p, e[i]));
       float a[8], b[8];
       unpack8(qa, a);
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append
     unpack8(raw[1][i][0], a); unpack8(raw[1][i][1], b);
     top[1] = fmaxf(top[1], largest8(a, b));
     unpack8(raw[0][i][0], ka[i]); unpack8(raw[0][i][1], kb[i]);
-    if (p.rot_dim && tok[i] < n) turn8(ka[i], kb[i], sc[i], p.interleaved);
+    if (p.rot_dim && tok[i] < n && group == 0) turn8(ka[i], kb[i], sc[i], p.interleaved);
     top[0] = fmaxf(top[0], largest8(ka[i], kb[i]));
   }
 #pragma unroll
@@ -310,7 +314,7 @@ __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append
     if (old[s] < now) rescale16(codes, before * D, old[s] * inv, threadIdx.x, THREADS);
 #pragma unroll
     for (int i = 0; i < SPAN; ++i) {
-      if (tok[i] >= n) continue;
+      if (tok[i] >= n || group > 0) continue;
       uint8_t* to = codes + (before + tok[i]) * D;
       float a[8], b[8];
       if (s) { unpack8(raw[1][i][0], a); unpack8(raw[1][i][1], b); }
@@ -322,7 +326,7 @@ __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append
 }
 
 // The same for one token a tile (a decode step): a warp per (row, kv head), up to 8 kv heads a block; the sines and cosines once a block.
-// What bounds it is latency: a wait, the row, the old scales, the codes.
+// What bounds it is latency: a wait, the row, the old scales, the codes.  One row of 32 heads on 8 kv heads of 128: 2.5 us, 64 rows 2.9.
 __global__ void __launch_bounds__(256) append8_step_kernel(Append8 p) {
   rb_pdl_launch_dependents();
   extern __shared__ float2 turns[];              // [D / 2]
@@ -412,7 +416,8 @@ __global__ void __launch_bounds__(256) cache8_values_kernel(__nv_bfloat16* k_out
   }
 }
 
-// The same for heads of a multiple of 16 values: a thread turns 16 codes at a time.
+// The same for heads of a multiple of 16 values: a thread turns 16 codes at a time.  Bounded by its bytes: 128 pages of 8 heads of 128, 50 MB in
+// 13 us (a code at a time: 49).
 __global__ void __launch_bounds__(256) cache8_values16_kernel(__nv_bfloat16* k_out, __nv_bfloat16* v_out, RbPagedLayer c, const float* k_scale,
                                                              const float* v_scale, const int* items, int block) {
   rb_pdl_launch_dependents();
@@ -443,9 +448,9 @@ RB_EXPORT int rb_cache8_block(int page_size) {
 }
 
 // q_out[T, H, D] = turned q rows; k (turned) and v rows enter the cache.  Tile i is the tile_ntok[i] rows from tile_tok0[i] on: new
-// positions of one block of one sequence, in order (null: every row is a tile of its own).
+// positions of one block of one sequence, in order, `tile_most` at most (null: every row is a tile of its own).
 RB_EXPORT int rb_append8(void* q_out, const void* qkv, int64_t qkv_stride, const float* inv_freq, const int* tok_pos, const int* tok_slot,
-                         const int* tile_tok0, const int* tile_ntok, int n_tiles, void* cache_k, void* cache_v, float* k_scale,
+                         const int* tile_tok0, const int* tile_ntok, int n_tiles, int tile_most, void* cache_k, void* cache_v, float* k_scale,
                          float* v_scale, const int* page_table, int max_pages, int page_size, int H, int Kh, int D, int write_kv,
                          int rot_dim, int interleaved, cudaStream_t stream) {
   if (n_tiles == 0) return 0;
@@ -454,6 +459,7 @@ RB_EXPORT int rb_append8(void* q_out, const void* qkv, int64_t qkv_stride, const
   RB_REQUIRE(H > 0 && Kh > 0 && H % Kh == 0 && Kh <= 65535, "rb_append8: %d heads on %d kv heads", H, Kh);
   RB_REQUIRE(!tile_tok0 || n_tiles <= 65535, "rb_append8: %d tiles in one launch", n_tiles);
   const int block = rb_cache8_block(page_size);
+  RB_REQUIRE(!tile_tok0 || (tile_ntok && tile_most >= 1 && tile_most <= block), "rb_append8: tiles of %d tokens", tile_most);
   RB_REQUIRE(block > 0, "rb_append8: a page of %d positions must be 64 at most, or a multiple of 64", page_size);
   Append8 p;
   p.q_out = (__nv_bfloat16*)q_out; p.qkv = (const __nv_bfloat16*)qkv; p.qkv_stride = qkv_stride;
@@ -468,9 +474,14 @@ RB_EXPORT int rb_append8(void* q_out, const void* qkv, int64_t qkv_stride, const
       RB_LAUNCH("rb_append8 (step)", (append8_step_kernel), dim3(n_tiles, (Kh + warps - 1) / warps), warps * 32, (size_t)D / 2 * 8, stream, p);
       return 0;
     }
-    if (D <= 64) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<256, 1>), dim3(Kh, n_tiles), 256, 0, stream, p);
-    else if (D <= 128) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<512, 1>), dim3(Kh, n_tiles), 512, 0, stream, p);
-    else RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<512, 2>), dim3(Kh, n_tiles), 512, 0, stream, p);
+    // (5 tokens of 32 heads of 64 on 4 kv heads: 4.1 us by one group of threads, 2.3 shared; the shared form costs full tiles 4 %)
+    const bool shared = D <= 128 && 2 * tile_most * (D / 16) <= (D <= 64 ? 256 : 512);
+    const dim3 grid(Kh, n_tiles);
+    if (D <= 64 && shared) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<256, 1, true>), grid, 256, 0, stream, p);
+    else if (D <= 64) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<256, 1, false>), grid, 256, 0, stream, p);
+    else if (D <= 128 && shared) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<512, 1, true>), grid, 512, 0, stream, p);
+    else if (D <= 128) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<512, 1, false>), grid, 512, 0, stream, p);
+    else RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<512, 2, false>), grid, 512, 0, stream, p);
     return 0;
   }
   static RbOncePerDevice configured;

@@ -116,7 +116,7 @@ _SIGNATURES = {
     "rb_qk_prepare": [P, P, I, P, L, P, I, P, P, I, P, P, F, P, F, I, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, L, F, I, P],
     "rb_latent_rotate_append": [P, I, P, L, P, F, P, F, I, P, P, P, P, I, I, I, I, I, I, I, I, P],
     "rb_rotate_rows": [P, L, I, I, I, P, F, I, I, P, I, P],
-    "rb_append8": [P, P, L, P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
+    "rb_append8": [P, P, L, P, P, P, P, P, I, I, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
     "rb_cache8_values": [P, P, P, I, P, P, P, P, P, I, I, I, I, P],
     "rb_attention8_simple": [P, P, P, P, P, P, P, I, I, P, P, I, I, I, I, F, I, P],
     "rb_attention8_rows": [P, P, P, P, P, P, L, P, I, I, P, P, P, P, I, I, I, I, I, F, I, I, I, P, P, P],

@@ -719,10 +719,10 @@ class CudaOps:
                           f"found {found}")
 
     def _block_tiles(self, meta, block: int):
-        """(first row, rows, count) of the tiles of a step's rows that lie in one block of one sequence, made once per step;
+        """(first row, rows, count, most rows) of the tiles of a step's rows that lie in one block of one sequence, made once per step;
         nothing for a step of one token per sequence, whose rows are tiles each."""
         if meta.single_token:
-            return None, None, meta.n_tokens
+            return None, None, meta.n_tokens, 1
         import numpy as np
         key = ("block_tiles", block)
         if key not in meta.extra:
@@ -735,7 +735,7 @@ class CudaOps:
                     ntok.append(n)
                     at += n
             both = upload(np.asarray([tok0, ntok], dtype=np.int32).reshape(2, -1), self.device)
-            meta.extra[key] = (both[0], both[1], len(tok0))
+            meta.extra[key] = (both[0], both[1], len(tok0), max(ntok, default=1))
         return meta.extra[key]
 
     def _rotate_append8(self, qkv: torch.Tensor, rotary, meta, view, n_heads: int) -> torch.Tensor:
@@ -748,10 +748,10 @@ class CudaOps:
         if qkv.dtype != self.dtype or not qkv.is_cuda or qkv.stride(1) != 1:
             raise KernelError(f"rotate_append: expected {self.dtype} CUDA rows, found {qkv.dtype} on {qkv.device}")
         inv_freq, interleaved, rot_dim = (self._zeros_freq(D), False, 0) if rotary is None else rotary
-        tok0, ntok, n_tiles = self._block_tiles(meta, block)
+        tok0, ntok, n_tiles, most = self._block_tiles(meta, block)
         q = qkv.new_empty((T, n_heads, D))
         self.lib.call("rb_append8", q.data_ptr(), qkv.data_ptr(), qkv.stride(0), inv_freq.data_ptr(), meta.tok_pos.data_ptr(),
-                      meta.tok_slot.data_ptr(), _address(tok0), _address(ntok), n_tiles, *_cache8(view), view.max_pages, view.page_size,
+                      meta.tok_slot.data_ptr(), _address(tok0), _address(ntok), n_tiles, most, *_cache8(view), view.max_pages, view.page_size,
                       n_heads, Kh, D, 1 if view.writes else 0, rot_dim, 1 if interleaved else 0, self._raw_stream())
         return q
 

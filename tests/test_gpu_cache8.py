@@ -81,6 +81,11 @@ APPENDS = [
     (16, 1, 512, 64, 512, False, [(0, 10, 70)]),
     (7, 7, 2, 1, 2, False, [(0, 0, 3), (1, 2, 1)]),
     (32, 8, 128, 64, 128, False, [(0, 0, 700), (1, 100, 333)]),
+    (4, 2, 256, 64, 256, False, [(0, 10, 70), (1, 5, 1)]),
+    (4, 2, 256, 64, 256, True, [(0, 3, 1), (2, 70, 1)]),
+    (8, 1, 96, 64, 96, False, [(0, 61, 5), (2, 0, 3)]),
+    (20, 1, 64, 64, 64, True, [(0, 61, 5), (2, 0, 3)]),
+    (12, 12, 64, 64, 64, False, [(0, 7, 1)]),
 ]
 
 
