@@ -21,11 +21,12 @@
 //
 // Ranges of keys: in a small grid the parts of a (tile, kv head) are a thread-block cluster and merge on chip.  In a larger one
 // all tiles of keys of all (row tile, kv head) pairs, in order, are dealt out evenly to the blocks, whatever the sequences' lengths; a
-// pair that several blocks have worked on is merged by a second kernel.
+// pair that several blocks have worked on is merged by a second kernel.  Where pairs are many and short a pair is one warp's work.
 //
 // Bounded by the cache's bytes where sequences are long: one B200, 64 sequences of up to 8,000 positions, 32 heads on 8 kv heads of 128:
-// 541 MB in 90 us, 6.0 TB/s (0.92 of a copy).  Short pairs are bound by what a pair costs to begin and to join (about 5 us a block, two
-// blocks an SM): 24 sequences of 32 heads with a window of 1,024, 202 MB in 49 us.  More rows add products and exponentials: 16
+// 541 MB in 90 us, 6.0 TB/s (0.92 of a copy).  Short pairs are bound by what a pair costs to begin and to join (about 5 us in a block, two
+// blocks an SM) or, a pair a warp, by a warp's chain from score to sum, a microsecond for 32 keys: 24 sequences of 32 heads with a window of
+// 1,024, 202 MB in 45 us, 4.5 TB/s.  More rows add products and exponentials: 16
 // sequences of up to five tokens at up to 6,001 positions, 20 rows, 101 MB in 40 us.  One sequence at 2,048 positions: 8 us, waits.
 // Measured beside it (the first of these): 16-byte cp.async by every thread 154 us, of which the copies alone 136; boxes of 16 positions
 // 126 to 136; two stages and three blocks an SM 109; pairs dealt out without what their beginnings cost 113.
@@ -47,7 +48,7 @@ struct Params {
   const int* tile_tok0;       // null: row tile i is row i alone
   const int* tile_ntok;
   int n_tiles, Kh, G;
-  int parts;                  // > 0: the parts of a pair are a cluster; 0: the tiles are dealt out to gridDim.x blocks
+  int parts;                  // > 0: the parts of a pair are a cluster; 0: the tiles are dealt out to gridDim.x blocks; -2, -3: a pair is a warp's, so many stages
   int least;                  // dealt out: tiles of a block, at least
   float4* part_o;             // dealt out: [blocks + pairs][NT][D / 16][lane], what the accumulators of a lane hold, and
   float2* part_ml;            // [blocks + pairs][8 NT] (maximum in base-2 units, sum)
@@ -84,11 +85,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-template <int D, int NT> struct Shape {
+// N: stages of a warp's ring.
+template <int D, int NT, int N = 3> struct Shape {
   static constexpr int KG = 2;                            // groups of 16 keys of a tile that a warp takes at a time
   static constexpr int CHUNK = KG * 16 * D;               // bytes of their codes, of keys and of values each
   static constexpr int STAGE = 2 * CHUNK;                 // of a warp
-  static constexpr int NS = 3;
+  static constexpr int NS = N;
   static constexpr int ROWS = 8 * NT;
   static constexpr bool Q_SHARED = NT >= 3;               // the query operands lie in shared memory, not in registers
   static constexpr int Q_BYTES = Q_SHARED ? (D / 16) * NT * 256 : 0;
@@ -102,7 +104,7 @@ template <int D, int NT> struct Shape {
   static constexpr int BYTES = OFF_BAR + WARPS * NS * 8 + 1024;         // + room to align
   static constexpr int LEFT = STAGE / (MT * 512);         // eights of rows whose accumulators a stage holds
   static constexpr int AHEAD = NS - (NT + LEFT - 1) / LEFT;             // stages of the next pair filled while a pair's warps are joined
-  static_assert(AHEAD >= 1, "a warp leaves its accumulators in its own ring");
+  static_assert(N < 3 || AHEAD >= 1, "a warp leaves its accumulators in its own ring");
   static_assert(NT * MT * 512 <= RING, "what the cluster's other blocks read, over the ring");
 };
 
@@ -148,32 +150,36 @@ __device__ __forceinline__ int visited_tiles(const Params& p, int tile) {
 
 // A warp's way through a segment: where the sequence lies, the tiles that it asks for next and their pages, scales of the tiles on their way.
 // The positions, slots and page tables were written before the step began: `Job` may be made before the wait, `ask` not.
-template <int D, int NT> struct Job {
-  using S = Shape<D, NT>;
-  static constexpr int SHARES = TILE / (16 * S::KG), STEP = WARPS / SHARES;      // the warp's share of a tile, and of the tiles
+// It counts in units of 32 keys: of every other tile the warp's half, or (ALONE > 0: a pair is one warp's work, with a ring of so many stages)
+// all halves in turn.
+template <int D, int NT, int ALONE = 0> struct Job {
+  using S = Shape<D, NT, ALONE ? ALONE : 3>;
+  static constexpr int KEYS = 16 * S::KG, SHARES = TILE / KEYS, STEP = ALONE ? 1 : WARPS / SHARES;
   Segment seg;
   Where w;
   RbKeyTiles tiles;
-  int in_tile, next;               // the warp's first key in a tile; the tile that is asked for next
-  int page[S::NS];                 // pages of tiles next, next + STEP, ...
-  float2 scales[S::NS - 1];        // of the tiles on their way (keys, values)
+  int begin, end, next;            // units; the one that is asked for next
+  int page[S::NS];                 // pages of units next, next + STEP, ...
+  float2 scales[S::NS - 1];        // of the units on their way (keys, values)
   __device__ __forceinline__ Job(const Params& p, const Segment& s)
       : seg(s), w(p, s.tile), tiles(w.key_lo, w.key_hi, p.a.keep, TILE) {
     const int warp = threadIdx.x >> 5;
-    in_tile = warp % SHARES * (16 * S::KG);
-    next = seg.first + warp / SHARES;
+    begin = next = ALONE ? seg.first * SHARES : seg.first + warp / SHARES;
+    end = ALONE ? seg.last * SHARES : seg.last;
 #pragma unroll
     for (int i = 0; i < S::NS; ++i) page[i] = page_of(p, next + i * STEP);
   }
-  __device__ __forceinline__ int page_of(const Params& p, int kt) const {
-    if (kt >= seg.last) return 0;
-    const int tile = tiles.at(kt), per = p.a.cache.page_size / TILE;
+  __device__ __forceinline__ int tile_of(int unit) const { return tiles.at(ALONE ? unit / SHARES : unit); }
+  __device__ __forceinline__ int in_tile(int unit) const { return (ALONE ? unit % SHARES : (int)(threadIdx.x >> 5) % SHARES) * KEYS; }
+  __device__ __forceinline__ int page_of(const Params& p, int unit) const {
+    if (unit >= end) return 0;
+    const int tile = tile_of(unit), per = p.a.cache.page_size / TILE;
 #ifdef RB_CHECKED
     return (int)(rb_page_offset(p.a.cache, w.slot, tile * TILE, seg.kvh) / ((int64_t)p.Kh * p.a.cache.page_size * D));
 #endif
     return p.a.cache.page_table[(int64_t)w.slot * p.a.cache.max_pages + (per == 1 ? tile : tile / per)];
   }
-  // The next tile's codes on their way, and its scales (place i of the queue); nothing of a tile that ends before the warp's share.
+  // The next unit's codes on their way, and its scales (place i of the queue); nothing of one that lies behind the sequence.
   __device__ __forceinline__ void ask(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV, uint8_t* stages, uint64_t* full,
                                       Ring& ring, int i) {
     const int kt = next, at = page[0];
@@ -182,15 +188,15 @@ template <int D, int NT> struct Job {
     for (int j = 0; j + 1 < S::NS; ++j) page[j] = page[j + 1];
     page[S::NS - 1] = page_of(p, next + (S::NS - 1) * STEP);
     scales[i] = make_float2(1.f, 1.f);
-    if (kt >= seg.last || ring.failed) return;
-    const int tile = tiles.at(kt);
-    if (tile * TILE + in_tile > w.key_hi) return;
+    if (kt >= end || ring.failed) return;
+    const int tile = tile_of(kt), in = in_tile(kt);
+    if (tile * TILE + in > w.key_hi) return;
     const int per = p.a.cache.page_size / TILE;
     const int unit = (at * p.Kh + seg.kvh) * per + (per == 1 ? 0 : tile % per);     // the block's number in the pool
     const uint32_t s = ring.asked % S::NS;
     if (elect_one()) {
       mbar_expect_tx(&full[s], S::STAGE);
-      const int row = (int)(((int64_t)unit * TILE + in_tile) * D / 128);            // of 128 bytes
+      const int row = (int)(((int64_t)unit * TILE + in) * D / 128);            // of 128 bytes
       tma_load_2d(stages + s * S::STAGE, tmK, 0, row, &full[s]);
       tma_load_2d(stages + s * S::STAGE + S::CHUNK, tmV, 0, row, &full[s]);
     }
@@ -200,20 +206,21 @@ template <int D, int NT> struct Job {
   }
 };
 
-// The block's part of a pair, whose first S::AHEAD tiles have been asked for; `then(ahead)` asks for those of the pair after it.
-template <int D, int NT, typename F>
-__device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV, Job<D, NT>& job, uint8_t* smem,
-                                     Ring& ring, Joined<D, NT>& joined, F then) {
-  using S = Shape<D, NT>;
-  constexpr int KG = S::KG, KP = D / 64, MT = D / 16, ROWS = S::ROWS, VW = D / 32;
+// A warp's sums: O^T in units of `unit`, maxima in base-2 units, this lane's part of the sums of the weights; rows 2t, 2t + 1 of every eight.
+template <int D, int NT> struct Sums {
+  float o[NT][D / 16][4], m[NT][2], l[NT][2], unit;
+};
+
+// The warp's way through a segment, whose first S::NS - 1 units have been asked for.
+template <int D, int NT, int ALONE>
+__device__ __forceinline__ void run(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV, Job<D, NT, ALONE>& job, uint8_t* smem,
+                                    uint8_t* stages, uint64_t* full, Ring& ring, Sums<D, NT>& sums) {
+  using S = typename Job<D, NT, ALONE>::S;
+  constexpr int KG = S::KG, KP = D / 64, MT = D / 16, VW = D / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const Where w = job.w;
   const Segment seg = job.seg;
-  const int kvh = seg.kvh, G = p.G, H = p.a.H, n_rows = w.ntok * G, in_tile = job.in_tile;
-  uint8_t* stages = smem + warp * S::NS * S::STAGE;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR) + warp * S::NS;
-#pragma unroll
-  for (int i = S::AHEAD; i < S::NS - 1; ++i) job.ask(p, tmK, tmV, stages, full, ring, i);
+  const int kvh = seg.kvh, G = p.G, H = p.a.H, n_rows = w.ntok * G;
 
   // ---- the query rows as B operands: of row g of every eight, values 64 j + 16 t + 4 i + (0, 1) and (2, 3)
   uint32_t qf[S::Q_SHARED ? 1 : MT][S::Q_SHARED ? 1 : NT][2];
@@ -270,7 +277,10 @@ __device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, co
   }
   if (S::Q_SHARED) __syncthreads();
 
-  float o[NT][MT][4], m[NT][2], l[NT][2], unit = 1.f;
+  auto& o = sums.o;
+  auto& m = sums.m;
+  auto& l = sums.l;
+  float unit = 1.f;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -280,7 +290,7 @@ __device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, co
       m[n][c] = -INFINITY;
       l[n][c] = 0.f;
       const int rc = n * 8 + 2 * t + c;
-      if (p.a.sinks != nullptr && seg.first == 0 && seg.last > 0 && warp == 0 && rc < n_rows) {     // counted once: by the part with the first tile
+      if (p.a.sinks != nullptr && seg.first == 0 && seg.last > 0 && (ALONE || warp == 0) && rc < n_rows) {     // counted once: by the part with the first tile
         m[n][c] = p.a.sinks[kvh * G + rc % G] * LOG2E;
         l[n][c] = g == 0 ? 1.f : 0.f;
       }
@@ -288,12 +298,12 @@ __device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, co
   }
 
   bool begun = false;
-  for (int kt = seg.first + warp / Job<D, NT>::SHARES; kt < seg.last && !ring.failed; kt += Job<D, NT>::STEP) {
+  for (int kt = job.begin; kt < job.end && !ring.failed; kt += job.STEP) {
     const float2 scales = job.scales[0];
 #pragma unroll
     for (int i = 0; i + 2 < S::NS; ++i) job.scales[i] = job.scales[i + 1];
     job.ask(p, tmK, tmV, stages, full, ring, S::NS - 2);
-    const int key0 = job.tiles.at(kt) * TILE + in_tile;
+    const int key0 = job.tile_of(kt) * TILE + job.in_tile(kt);
     if (key0 > w.key_hi) continue;
     const uint32_t stage = ring.used % S::NS;
     if (!mbar_wait_warp(&full[stage], (ring.used / S::NS) & 1, 15)) {
@@ -471,6 +481,26 @@ __device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, co
     __syncwarp();                    // everybody has left this stage: it may be filled again
   }
 
+  sums.unit = unit;
+}
+
+// The block's part of a pair, whose first S::AHEAD units have been asked for; `then` asks for those of the pair after it.
+template <int D, int NT, typename F>
+__device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV, Job<D, NT>& job, uint8_t* smem,
+                                     Ring& ring, Joined<D, NT>& joined, F then) {
+  using S = Shape<D, NT>;
+  constexpr int MT = S::MT, ROWS = S::ROWS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* stages = smem + warp * S::NS * S::STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR) + warp * S::NS;
+#pragma unroll
+  for (int i = S::AHEAD; i < S::NS - 1; ++i) job.ask(p, tmK, tmV, stages, full, ring, i);
+  Sums<D, NT> sums;
+  run<D, NT, 0>(p, tmK, tmV, job, smem, stages, full, ring, sums);
+  auto& o = sums.o;
+  auto& m = sums.m;
+  auto& l = sums.l;
+  const float unit = sums.unit;
   // ---- the next pair's first tiles, which arrive meanwhile; then the four warps: each leaves its accumulators, as its lanes hold them,
   // in those stages of its own ring that are not being filled, and takes a quarter of the row tiles from all
   const uint32_t beside = ring.asked + S::AHEAD;
@@ -574,8 +604,7 @@ __device__ __forceinline__ void add_part(float4& acc, float (&m)[2], float (&l)[
 }
 
 // The warps' barriers; what follows is ordered by the caller's or the first barrier of the block.
-template <int D, int NT> __device__ __forceinline__ void begin(uint8_t* smem) {
-  using S = Shape<D, NT>;
+template <typename S> __device__ __forceinline__ void begin(uint8_t* smem) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < WARPS * S::NS; ++i) mbar_init(reinterpret_cast<uint64_t*>(smem + S::OFF_BAR) + i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -590,7 +619,7 @@ __global__ void __launch_bounds__(WARPS * 32) cluster_kernel(const __grid_consta
   using S = Shape<D, NT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  begin<D, NT>(smem);
+  begin<S>(smem);
   Ring ring{0, 0, false};
   Segment seg;
   seg.tile = blockIdx.x; seg.kvh = blockIdx.y;
@@ -684,7 +713,7 @@ __global__ void __launch_bounds__(WARPS * 32) dealt_kernel(const __grid_constant
   using S = Shape<D, NT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  begin<D, NT>(smem);
+  begin<S>(smem);
   Ring ring{0, 0, false};
   __shared__ int counts[WARPS], s_tile, s_before;
   // positions, slots and page tables were written before the step began: the deal needs no wait
@@ -817,6 +846,72 @@ __global__ void __launch_bounds__(D * 2) join_kernel(Params p, int blocks) {
   store<D>(p, w, kvh, n, (int)threadIdx.x >> 5, lane, acc, l);
 }
 
+// Pairs that are short, and many: each is ONE warp's work, from its first key to its output, and a block is one warp; nobody waits for
+// anybody.  (24 sequences of 32 heads with a window of 1,024: 45 us, dealt out 49; 54 of up to 56 positions: 6.4, a block a pair 28.)
+template <int D, int NT, int STAGES>
+__global__ void __launch_bounds__(32) alone_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, Params p) {
+  rb_pdl_launch_dependents();
+  using S = typename Job<D, NT, STAGES>::S;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(stages + STAGES * S::STAGE);
+  const int lane = threadIdx.x, g = lane >> 2, t = lane & 3;
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) mbar_init(full + i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_shared();
+  }
+  __syncwarp();
+  Ring ring{0, 0, false};
+  const int64_t pairs = (int64_t)p.n_tiles * p.Kh, step = gridDim.x;
+  auto segment = [&](int64_t pair) {
+    Segment seg;
+    seg.tile = (int)(pair / p.Kh);
+    seg.kvh = (int)(pair % p.Kh);
+    seg.first = 0;
+    seg.last = seg.visited = visited_tiles(p, seg.tile);
+    return seg;
+  };
+  int64_t pair = blockIdx.x;
+  Job<D, NT, STAGES> job(p, segment(pair));
+  rb_pdl_wait();
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) job.ask(p, &tmK, &tmV, stages, full, ring, i);
+  for (; pair < pairs; pair += step) {
+    Sums<D, NT> sums;
+    run<D, NT, STAGES>(p, &tmK, &tmV, job, stages, stages, full, ring, sums);
+    const Where w = job.w;
+    const int kvh = job.seg.kvh;
+    if (pair + step < pairs) {
+      job = Job<D, NT, STAGES>(p, segment(pair + step));
+#pragma unroll
+      for (int i = 0; i < STAGES - 1; ++i) job.ask(p, &tmK, &tmV, stages, full, ring, i);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float sum = sums.l[n][c];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int r = n * 8 + 2 * t + c;
+        if (r < w.ntok * p.G) {
+          const float by = sums.unit / sum;
+          uint32_t out[D / 16];
+#pragma unroll
+          for (int u = 0; u < D / 16; ++u) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(sums.o[n][u][c] * by, sums.o[n][u][c + 2] * by);
+            out[u] = *reinterpret_cast<const uint32_t*>(&b);
+          }
+          uint4* dst = reinterpret_cast<uint4*>(p.a.out + ((int64_t)(w.tok0 + r / p.G) * p.a.H + kvh * p.G + r % p.G) * D + D / 8 * g);
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x) dst[x] = make_uint4(out[4 * x], out[4 * x + 1], out[4 * x + 2], out[4 * x + 3]);
+        }
+      }
+  }
+}
+
 // blocks of the kernel that an SM holds: by registers at the kernel's bound and by shared memory
 template <int D, int NT> int per_sm() {
   static int n[RB_MAX_DEVICES] = {0};
@@ -869,9 +964,29 @@ inline int places(int D, int NT) {
   return n * rb_sm_count();
 }
 
+// blocks: pairs; as many as the SMs hold at once take them in turn
+template <int D, int NT, int STAGES>
+int launch_alone(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, int blocks, cudaStream_t stream) {
+  constexpr int bytes = STAGES * Shape<D, NT, STAGES>::STAGE + STAGES * 8 + 1024;
+  static int places[RB_MAX_DEVICES] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= RB_MAX_DEVICES) dev = 0;
+  if (places[dev] == 0) {
+    int n = 0;
+    RB_CUDA(cudaFuncSetAttribute(alone_kernel<D, NT, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    RB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, alone_kernel<D, NT, STAGES>, 32, bytes));
+    places[dev] = (n > 0 ? n : 1) * rb_sm_count();
+  }
+  RB_LAUNCH("rb_attention8_rows (alone)", (alone_kernel<D, NT, STAGES>), blocks < places[dev] ? blocks : places[dev], 32, bytes, stream, tk, tv, p);
+  return 0;
+}
 template <int D, int NT>
 int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, int blocks, cudaStream_t stream) {
   using S = Shape<D, NT>;
+  if (p.parts < 0) {
+    if constexpr (NT <= 2) return p.parts == -2 ? launch_alone<D, NT, 2>(tk, tv, p, blocks, stream) : launch_alone<D, NT, 3>(tk, tv, p, blocks, stream);
+    RB_FAIL("rb_attention8_rows: %d rows do not go a pair a warp", S::ROWS);
+  }
   per_sm<D, NT>();                                 // (sets the kernels' attributes)
   if (p.parts == 0) {
     RB_LAUNCH("rb_attention8_rows", (dealt_kernel<D, NT>), blocks, WARPS * 32, S::BYTES, stream, tk, tv, p);
@@ -895,6 +1010,15 @@ int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, int bl
   RB_CUDA(cudaLaunchKernelEx(&cfg, cluster_kernel<D, NT>, tk, tv, p));
   return 0;
 }
+// Whether a warp a pair is sooner done than tiles dealt out: microseconds of the two on one B200, from 128 to 1,728 pairs of 1 to 30 tiles.  A warp takes
+// two units of 32 keys a tile, one a microsecond, eight warps an SM, or the bytes' time; dealt out a pair costs ten tiles beside its own.
+// (Pairs x tiles, alone and dealt out: 320 x 4 10, 13; 960 x 5 17, 32; 768 x 17 45, 49; 1,024 x 30 78, 88; but 200 x 8 19, 13; 400 x 16 39, 29.)
+inline bool alone_pays(long long pairs, int tiles, int D) {
+  const double sms = rb_sm_count(), rounds = (double)((pairs + 8 * (long long)sms - 1) / (8 * (long long)sms));
+  const double alone = rounds * (3.0 + 2.05 * tiles), bytes = 0.41 * pairs * tiles / sms * D / 128.0;
+  return (alone > bytes ? alone : bytes) < 5.0 + 0.31 * pairs * (tiles + 10) / sms;
+}
+
 template <int D>
 int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, int NT, int blocks, cudaStream_t stream) {
   return NT == 1 ? launch<D, 1>(tk, tv, p, blocks, stream) : NT == 2 ? launch<D, 2>(tk, tv, p, blocks, stream)
@@ -911,8 +1035,8 @@ RB_EXPORT int rb_attention8_rows_supports(int H, int Kh, int D, int page_size) {
 
 // How a launch of `n_tiles` row tiles of at most `rows` rows is cut, the longest sequence `context` positions: out4 = parts of a pair that
 // are a cluster (0: dealt out), blocks when dealt out, floats of part_o, floats of part_ml.
-// A cluster where two parts of every pair and more fit the SMs at once and no part is long; else all tiles are dealt out to as many
-// blocks as the SMs hold at once, four tiles to a block at least.
+// A cluster where two parts of every pair and more run at once and no part is long; a warp a pair (parts -2 or -3: the stages of its ring)
+// where pairs are many and short; else all tiles are dealt out to as many blocks as the SMs hold at once, four tiles to a block at least.
 RB_EXPORT int rb_attention8_rows_plan(int n_tiles, int rows, int Kh, int D, int context, long long* out4) {
   const int NT = (rows + 7) / 8, places = rows8::places(D, NT);
   const int tiles = (context + rows8::TILE - 1) / rows8::TILE;
@@ -921,7 +1045,13 @@ RB_EXPORT int rb_attention8_rows_plan(int n_tiles, int rows, int Kh, int D, int 
   int parts = 1;
   while (parts * 2 <= tiles && parts < 16 && pairs <= rows8::clusters(D, NT, parts * 2)) parts *= 2;
   out4[0] = parts; out4[1] = out4[2] = out4[3] = 0;
-  if (tiles <= 1 || (parts > 1 && tiles <= 16 * parts)) return 0;
+  if (parts > 1 && tiles <= 16 * parts) return 0;
+  if (NT <= 2 && pairs <= 2147483647ll && (tiles <= 1 || rows8::alone_pays(pairs, tiles, D))) {
+    out4[0] = tiles <= 2 ? -2 : -3;
+    out4[1] = pairs;
+    return 0;
+  }
+  if (tiles <= 1) return 0;
   long long blocks = (pairs * tiles + 3) / 4;
   if (blocks > places) blocks = places;
   out4[0] = 0;
@@ -943,7 +1073,8 @@ RB_EXPORT int rb_attention8_rows(void* out, const void* q, void* cache_k, void* 
              "rb_attention8_rows: sizes H=%d Kh=%d D=%d page=%d, %d rows not supported", H, Kh, D, page_size, rows);
   RB_REQUIRE(n_pages * Kh * page_size / rows8::TILE <= 2147483647ll && n_pages * Kh * page_size * D / 128 <= 2147483647ll,
              "rb_attention8_rows: a pool of %lld pages has too many blocks", n_pages);
-  RB_REQUIRE(parts >= 0 && parts <= 16 && (parts & (parts - 1)) == 0 && (parts > 0 || (blocks > 0 && part_o && part_ml)), "rb_attention8_rows: %d parts, %d blocks", parts, blocks);
+  RB_REQUIRE(parts >= -3 && parts != -1 && parts <= 16 && (parts <= 0 || (parts & (parts - 1)) == 0) && (parts > 0 || blocks > 0) &&
+                 (parts != 0 || (part_o && part_ml)), "rb_attention8_rows: %d parts, %d blocks", parts, blocks);
   rows8::Params p;
   p.a.q = (const __nv_bfloat16*)q; p.a.out = (__nv_bfloat16*)out;
   p.a.cache = RbPagedLayer{cache_k, cache_v, page_table, max_pages, page_size, Kh, D};

@@ -433,6 +433,28 @@ def test_many_sequences_of_unequal_lengths(ops):
             at += n
 
 
+def test_many_short_pairs(ops):
+    """Pairs that are one warp's work each: one tile, a few, windows with sinks and first keys that stay; one and two eights of rows; more
+    pairs than run at once."""
+    for H, Kh, D, new, most, window, sinks, cap, keep in ((16, 16, 128, 1, 60, 0, False, 0.0, 0), (32, 8, 64, 1, 250, 0, True, 0.0, 0),
+                                                          (8, 8, 128, 1, 1100, 150, True, 20.0, 70), (16, 8, 64, 5, 200, 0, False, 0.0, 0),
+                                                          (32, 8, 128, 4, 300, 90, True, 0.0, 10), (12, 6, 128, 2, 64, 0, False, 5.0, 0)):
+        B, max_pages = 100 if most < 500 else 60, -(-(most + new) // 64)
+        view, cpu = make_view(B * max_pages, Kh, 64, D, B, max_pages, seed=H + D)
+        seqs = [(B - 1 - i, (i * 37 * (1 + i % 5)) % (most + 1 - new), 1 + i % new) for i in range(B)]
+        q = rows_of(seqs, H * D, seed=9).view(-1, H, D)
+        sink = torch.linspace(-2.0, 3.0, H) if sinks else None
+        meta = make_meta(seqs)
+        got = ops.attention(q.cuda(), meta, view, H, D ** -0.5, window, sinks=None if sink is None else sink.cuda(), softcap=cap,
+                            keep_first=keep).cpu().to(F64)
+        assert [v[5] for k, v in meta.extra.items() if k[0] == "attention8"][0] < 0
+        at = 0
+        for slot, start, n in seqs:
+            want, size = plain.attend(cpu, slot, start, q[at:at + n], D ** -0.5, window, sink, cap, keep)
+            assert torch.all((got[at:at + n] - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size), (H, slot)
+            at += n
+
+
 def test_prompts_through_bfloat16_pages_and_through_codes_are_the_same_attention(ops):
     """The rule between the two is one of speed: rows of a few tokens either way."""
     H, Kh, D = 8, 2, 128
