@@ -425,16 +425,28 @@ __global__ void __launch_bounds__(256) cache8_values16_kernel(__nv_bfloat16* k_o
   const int slot = items[3 * i], page = items[3 * i + 1], used = in_use(c, slot, page, items[3 * i + 2]);
   rb_pdl_wait();
   const int64_t at = used > 0 ? rb_page_offset(c, slot, page * c.page_size, kvh) : 0, to = ((int64_t)i * c.n_kv_heads + kvh) * n;
-  const uint8_t* in = (const uint8_t*)(blockIdx.z ? c.v : c.k) + at;
+  const uint8_t* data = (const uint8_t*)(blockIdx.z ? c.v : c.k) + at;
   const float* scale = (blockIdx.z ? v_scale : k_scale) + at / ((int64_t)block * D);
   __nv_bfloat16* out = (blockIdx.z ? v_out : k_out) + to;
-#pragma unroll 2
-  for (int idx = threadIdx.x * 16; idx < n; idx += 256 * 16) {
-    const int pos = idx / D;
-    uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-    if (pos < used) values16(*reinterpret_cast<const uint4*>(in + idx), scale[block == c.page_size ? 0 : pos / block], v);
-    *reinterpret_cast<uint4*>(out + idx) = v[0];
-    *reinterpret_cast<uint4*>(out + idx + 8) = v[1];
+  for (int base = threadIdx.x * 16; base < n; base += 2 * 256 * 16) {              // (two pieces asked for together)
+    uint4 codes[2];
+    float by[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int idx = base + i * 256 * 16, pos = idx / D;
+      const bool in = idx < n && pos < used;
+      codes[i] = in ? *reinterpret_cast<const uint4*>(data + idx) : make_uint4(0, 0, 0, 0);
+      by[i] = in ? scale[block == c.page_size ? 0 : pos / block] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int idx = base + i * 256 * 16;
+      if (idx >= n) break;
+      uint4 v[2];
+      values16(codes[i], by[i], v);
+      *reinterpret_cast<uint4*>(out + idx) = v[0];
+      *reinterpret_cast<uint4*>(out + idx + 8) = v[1];
+    }
   }
 }
 

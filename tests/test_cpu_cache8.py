@@ -168,6 +168,21 @@ def test_an_engine_with_8_bits_is_near_the_one_without(config, page):
     assert float((out[2] - out[1]).abs().max()) <= 0.1 * size
 
 
+def test_the_command_line(tmp_path, capsys):
+    """generate with a cache of 8 bits and drafts: the engine's own results."""
+    import json
+    from rbitnet_b200 import write_random_model
+    from rbitnet_b200.cli import main
+    write_random_model(tmp_path / "m", config_from_dict(TINY_B), seed=7)
+    argv = ["generate", "--model", str(tmp_path / "m"), "--cache-dtype", "float8_e4m3", "--cache-tokens", "512", "--draft-tokens", "3",
+            "--prompt-ids", "1 5 9 1 5 9 1", "--max-tokens", "8", "--temperature", "0"]
+    assert main(argv, ops=TorchOps8(torch.bfloat16)) == 0
+    got = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    eng = Engine.load_path(tmp_path / "m", dtype="bfloat16", ops=TorchOps8(torch.bfloat16), max_tokens=512, cache_dtype="float8_e4m3")
+    want = eng.generate([[1, 5, 9, 1, 5, 9, 1]], max_tokens=8, temperature=0.0, draft_tokens=3)[0]
+    assert got == {"tokens": want.tokens, "finish_reason": want.finish_reason, "prompt_tokens": 7}
+
+
 # ---- refusals
 def test_what_is_refused():
     with pytest.raises(ValueError, match="bfloat16 mode"):

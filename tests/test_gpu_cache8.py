@@ -252,11 +252,15 @@ def verified(ops, logits, first, drafts, temperature, uniforms, most, probs):
 
 
 @pytest.mark.parametrize("B,most,V,certain", [(1, 4, 1000, True), (5, 3, 5000, False), (9, 1, 1, True), (4, 0, 77, False), (7, 8, 4096, False),
-                                              (3, 5, 32000, True), (2, 2, 128256, False), (70, 2, 33, False)])
+                                              (3, 5, 32000, True), (2, 2, 128256, False), (70, 2, 33, False), (4, 40, 60, True)])
 def test_verify(ops, B, most, V, certain):
     for seed in range(3):
         case = drafts_case(B, most, V, certain, seed)
         assert verified(ops, *case) == plain.verify(*case)
+    # everything is accepted but the last few
+    case[2].copy_(torch.where(torch.arange(len(case[2])) % 37 < 36, case[0].argmax(1).to(torch.int32), case[2]))
+    case[3].zero_()
+    assert verified(ops, *case) == plain.verify(*case)
 
 
 def test_verify_at_the_edges(ops):
