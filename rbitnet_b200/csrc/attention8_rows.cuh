@@ -1037,6 +1037,8 @@ RB_EXPORT int rb_attention8_rows_supports(int H, int Kh, int D, int page_size) {
 // are a cluster (0: dealt out), blocks when dealt out, floats of part_o, floats of part_ml.
 // A cluster where two parts of every pair and more run at once and no part is long; a warp a pair (parts -2 or -3: the stages of its ring)
 // where pairs are many and short; else all tiles are dealt out to as many blocks as the SMs hold at once, four tiles to a block at least.
+// (Parts of up to 32 tiles: us as a cluster and dealt out, 8 sequences of 32 heads on 8 at 2,048 positions 11.9, 13.7, at 8,000 27.0, 29.0, but at
+// unequal lengths up to 8,000 25.4, 20.7: a captured step's `context` is the longest its sequences may get, so most of its parts are shorter.)
 RB_EXPORT int rb_attention8_rows_plan(int n_tiles, int rows, int Kh, int D, int context, long long* out4) {
   const int NT = (rows + 7) / 8, places = rows8::places(D, NT);
   const int tiles = (context + rows8::TILE - 1) / rows8::TILE;
@@ -1045,7 +1047,7 @@ RB_EXPORT int rb_attention8_rows_plan(int n_tiles, int rows, int Kh, int D, int 
   int parts = 1;
   while (parts * 2 <= tiles && parts < 16 && pairs <= rows8::clusters(D, NT, parts * 2)) parts *= 2;
   out4[0] = parts; out4[1] = out4[2] = out4[3] = 0;
-  if (parts > 1 && tiles <= 16 * parts) return 0;
+  if (parts > 1 && tiles <= 32 * parts) return 0;
   if (NT <= 2 && pairs <= 2147483647ll && (tiles <= 1 || rows8::alone_pays(pairs, tiles, D))) {
     out4[0] = tiles <= 2 ? -2 : -3;
     out4[1] = pairs;

@@ -225,7 +225,7 @@ __device__ __forceinline__ float largest8(const float (&a)[8], const float (&b)[
 // registers, turns the key's piece and those of the G query heads with them, and keeps the key's and the value's pieces until the
 // block's largest values have met.  16-byte loads and stores; the blocks of a tile's kv heads run side by side, so that rows are read whole.
 // What bounds it is the chain of waits of a block (tile, positions, rows, the largest values), hidden behind the blocks beside it: 8,192
-// tokens of 32 heads on 8 kv heads of 128, 184 MB in 46 us, 4.0 TB/s (sines and cosines through shared memory, 256 threads: 64 us; 92
+// tokens of 32 heads on 8 kv heads of 128, 184 MB in 45 us, 4.1 TB/s (sines and cosines through shared memory, 256 threads: 64 us; 92
 // registers and one block an SM 60).  16 sequences of up to five tokens, 32 heads of 64 on 4: 2.4 us.
 template <int THREADS, int SPAN, bool SHARED>
 __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append8_tiles_kernel(Append8 p) {
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append
     if (tok[i] >= n) continue;
     const __nv_bfloat16* src = rows + (int64_t)tok[i] * p.qkv_stride + (int64_t)kvh * G * D;
     __nv_bfloat16* dst = p.q_out + ((int64_t)(tok0 + tok[i]) * p.H + kvh * G) * D;
-#pragma unroll 4
+#pragma unroll 2
     for (int g = group; g < G; g += groups) {
       const uint4 qa = *reinterpret_cast<const uint4*>(src + g * D + piece_a(p, e[i])), qb = *reinterpret_cast<const uint4*>(src + g * D + piece_b(p, e[i]));
       float a[8], b[8];
