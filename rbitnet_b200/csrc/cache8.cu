@@ -88,6 +88,30 @@ __device__ __forceinline__ float2 turn_of(int pos, float freq) {
   return make_float2(sn, cs);
 }
 
+// A turned key, scaled, is a float32 number off by at most `off`; its code is that of the exact number unless a border between two codes
+// lies that near.  (Steps of e4m3: an eighth of the power of two below the value, 2^-9 at least.)
+__device__ __forceinline__ bool near_border(float v, float off) {
+  const uint32_t e = max(__float_as_uint(fabsf(v)) >> 23, 121u);                 // 2^-6 and above
+  const float per_step = __uint_as_float((127u + 130u - e) << 23), t = fabsf(v) * per_step;
+  return fabsf(t - floorf(t) - 0.5f) <= off * per_step;
+}
+// Then both numbers of the pair are made in float64 from the row itself, and handed on rounded to odd, so that the rounding to a code
+// that follows is the only one: what is stored does not depend on how well float32 sines are rounded.
+__device__ __forceinline__ float to_odd(double y) {
+  const float f = __double2float_rz(y);
+  return (double)f == y ? f : __uint_as_float(__float_as_uint(f) | 1u);
+}
+__device__ __noinline__ float2 exact_turned(const __nv_bfloat16* first, const __nv_bfloat16* second, const float* freq, int pos, float inv) {
+  const double x0 = (double)__bfloat162float(*first), x1 = (double)__bfloat162float(*second);
+  const double turns = (double)pos * ((double)*freq * 0.15915494309189533577);
+  double sn, cs;
+  sincospi((turns - rint(turns)) * 2.0, &sn, &cs);
+  return make_float2(to_odd((x0 * cs - x1 * sn) * (double)inv), to_odd((x0 * sn + x1 * cs) * (double)inv));
+}
+// How far a turned pair x, y (of length r <= |x| + |y|) may be off: the float32 angle by pi 2^-25, which moves it by pi 2^-25 r; its sine and
+// cosine by 2^-24 each, sqrt(2) 2^-24 r; the products by 2^-24 r and the sum by 2^-24 r: 9.98 2^-25 r in all.
+__device__ __forceinline__ float pair_off(float x, float y) { return (fabsf(x) + fabsf(y)) * 0x1.4p-22f; }
+
 struct Append8 {
   __nv_bfloat16* q_out;          // [T, H, D]
   const __nv_bfloat16* qkv;      // [T, (H + 2 Kh) D], rows qkv_stride apart (H D without writing)
@@ -161,7 +185,28 @@ __global__ void __launch_bounds__(256) append8_kernel(Append8 p) {
       const float ratio = old * inv;
       for (int idx = threadIdx.x; idx < before * D; idx += blockDim.x) codes[idx] = to_code(of_code(codes[idx]) * ratio);
     }
-    for (int idx = threadIdx.x; idx < n * D; idx += blockDim.x) codes[(int64_t)before * D + idx] = to_code(rows[idx] * inv);
+    for (int idx = threadIdx.x; idx < n * half; idx += blockDim.x) {
+      const int tok = idx / half, i = idx % half;
+      uint8_t* to = codes + (int64_t)(before + tok) * D;
+      if (stream == 1 || i >= rhalf) {
+        a = stream == 1 ? 2 * i : p.rot_dim + 2 * (i - rhalf);
+        to[a] = to_code(rows[tok * D + a] * inv);
+        to[a + 1] = to_code(rows[tok * D + a + 1] * inv);
+        continue;
+      }
+      a = p.interleaved ? 2 * i : i;
+      b = p.interleaved ? 2 * i + 1 : i + rhalf;
+      float x = rows[tok * D + a] * inv, y = rows[tok * D + b] * inv;
+      const float off = pair_off(x, y);
+      if (near_border(x, off) || near_border(y, off)) {
+        const __nv_bfloat16* head = p.qkv + (int64_t)(tok0 + tok) * p.qkv_stride + (int64_t)(p.H + kvh) * D;
+        const float2 exact = exact_turned(head + a, head + b, p.inv_freq + i, pos0 + tok, inv);
+        x = exact.x;
+        y = exact.y;
+      }
+      to[a] = to_code(x);
+      to[b] = to_code(y);
+    }
     __syncthreads();                             // everybody has read the old scale and the rows
     if (threadIdx.x == 0) *scale = now;
   }
@@ -220,13 +265,39 @@ __device__ __forceinline__ float largest8(const float (&a)[8], const float (&b)[
   return m;
 }
 
+// Turned pairs of a key (a: first values, b: second ones; interleaved: values in their order) times the scale's inverse, ready for their codes.
+// head: the row's head before the rotation.
+__device__ __forceinline__ void scaled_key8(const Append8& p, float (&a)[8], float (&b)[8], const __nv_bfloat16* head, int e, int pos, float inv) {
+  uint32_t near = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float& x = p.interleaved ? (i < 4 ? a[2 * i] : b[2 * i - 8]) : a[i];
+    float& y = p.interleaved ? (i < 4 ? a[2 * i + 1] : b[2 * i - 7]) : b[i];
+    x *= inv;
+    y *= inv;
+    const float off = pair_off(x, y);
+    if (near_border(x, off) || near_border(y, off)) near |= 1u << i;
+  }
+  if (near == 0) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (!(near >> i & 1u)) continue;
+    const int pair = 8 * e + i;
+    const __nv_bfloat16* first = head + (p.interleaved ? 2 * pair : pair);
+    const float2 exact = exact_turned(first, p.interleaved ? first + 1 : first + p.cache.head_dim / 2, p.inv_freq + pair, pos, inv);
+    (p.interleaved ? (i < 4 ? a[2 * i] : b[2 * i - 8]) : a[i]) = exact.x;
+    (p.interleaved ? (i < 4 ? a[2 * i + 1] : b[2 * i - 7]) : b[i]) = exact.y;
+  }
+}
+
 // Heads of a multiple of 16 values, turned whole, rows on 16 bytes: a block of threads per (tile, kv head).  A thread takes one piece of
 // eight pairs of one token (SPAN of them where a head is long), and of that piece everything: it makes the sines and cosines once, in
 // registers, turns the key's piece and those of the G query heads with them, and keeps the key's and the value's pieces until the
 // block's largest values have met.  16-byte loads and stores; the blocks of a tile's kv heads run side by side, so that rows are read whole.
 // What bounds it is the chain of waits of a block (tile, positions, rows, the largest values), hidden behind the blocks beside it: 8,192
-// tokens of 32 heads on 8 kv heads of 128, 184 MB in 45 us, 4.1 TB/s (sines and cosines through shared memory, 256 threads: 64 us; 92
-// registers and one block an SM 60).  16 sequences of up to five tokens, 32 heads of 64 on 4: 2.4 us.
+// tokens of 32 heads on 8 kv heads of 128, 184 MB in 51 us, 3.6 TB/s; 45 us but for the keys that lie near a border (a warp in about 100
+// makes its sines in float64, and its block waits).  Measured in float32 alone: 44 us, sines and cosines through shared memory and 256
+// threads 64, 92 registers and one block an SM 60.  16 sequences of up to five tokens, 32 heads of 64 on 4: 3.3 us.
 template <int THREADS, int SPAN, bool SHARED>
 __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append8_tiles_kernel(Append8 p) {
   rb_pdl_launch_dependents();
@@ -316,17 +387,28 @@ __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append
     for (int i = 0; i < SPAN; ++i) {
       if (tok[i] >= n || group > 0) continue;
       uint8_t* to = codes + (before + tok[i]) * D;
-      float a[8], b[8];
-      if (s) { unpack8(raw[1][i][0], a); unpack8(raw[1][i][1], b); }
-      *reinterpret_cast<uint2*>(to + piece_a(p, e[i])) = codes8(s ? a : ka[i], inv);
-      *reinterpret_cast<uint2*>(to + piece_b(p, e[i])) = codes8(s ? b : kb[i], inv);
+      if (s) {
+        float a[8], b[8];
+        unpack8(raw[1][i][0], a); unpack8(raw[1][i][1], b);
+        *reinterpret_cast<uint2*>(to + piece_a(p, e[i])) = codes8(a, inv);
+        *reinterpret_cast<uint2*>(to + piece_b(p, e[i])) = codes8(b, inv);
+      } else {
+        float by = inv;
+        if (p.rot_dim) {
+          scaled_key8(p, ka[i], kb[i], rows + (int64_t)tok[i] * p.qkv_stride + (int64_t)(p.H + kvh) * D, e[i], pos0 + tok[i], inv);
+          by = 1.f;
+        }
+        *reinterpret_cast<uint2*>(to + piece_a(p, e[i])) = codes8(ka[i], by);
+        *reinterpret_cast<uint2*>(to + piece_b(p, e[i])) = codes8(kb[i], by);
+      }
     }
     if (threadIdx.x == 0) (s ? p.v_scale : p.k_scale)[unit] = now;
   }
 }
 
 // The same for one token a tile (a decode step): a warp per (row, kv head), up to 8 kv heads a block; the sines and cosines once a block.
-// What bounds it is latency: a wait, the row, the old scales, the codes.  One row of 32 heads on 8 kv heads of 128: 2.5 us, 64 rows 2.9.
+// What bounds it is latency: a wait, the row, the old scales, the codes.  One row of 32 heads on 8 kv heads of 128: 3.5 us, 64 rows 4.3
+// (2.9 and 3.3 where no key lies near a border).
 __global__ void __launch_bounds__(256) append8_step_kernel(Append8 p) {
   rb_pdl_launch_dependents();
   extern __shared__ float2 turns[];              // [D / 2]
@@ -383,7 +465,11 @@ __global__ void __launch_bounds__(256) append8_step_kernel(Append8 p) {
       if (old_k < now_k) rescale16(k, before * D, old_k / now_k, lane, 32);
       if (old_v < now_v) rescale16(v, before * D, old_v / now_v, lane, 32);
       if (is_k || is_v) {
-        const float inv = 1.0f / (is_k ? now_k : now_v);
+        float inv = 1.0f / (is_k ? now_k : now_v);
+        if (is_k && p.rot_dim) {
+          scaled_key8(p, a, b, src + head * D, e, pos, inv);
+          inv = 1.f;
+        }
         uint8_t* to = (is_k ? k : v) + before * D;
         *reinterpret_cast<uint2*>(to + piece_a(p, e)) = codes8(a, inv);
         *reinterpret_cast<uint2*>(to + piece_b(p, e)) = codes8(b, inv);
@@ -486,7 +572,8 @@ RB_EXPORT int rb_append8(void* q_out, const void* qkv, int64_t qkv_stride, const
       RB_LAUNCH("rb_append8 (step)", (append8_step_kernel), dim3(n_tiles, (Kh + warps - 1) / warps), warps * 32, (size_t)D / 2 * 8, stream, p);
       return 0;
     }
-    // (5 tokens of 32 heads of 64 on 4 kv heads: 4.1 us by one group of threads, 2.3 shared; the shared form costs full tiles 4 %)
+    // (5 tokens of 32 heads of 64 on 4 kv heads, keys by float32 alone: 4.1 us by one group of threads, 2.3 shared; the shared form costs full
+    // tiles 4 %)
     const bool shared = D <= 128 && 2 * tile_most * (D / 16) <= (D <= 64 ? 256 : 512);
     const dim3 grid(Kh, n_tiles);
     if (D <= 64 && shared) RB_LAUNCH("rb_append8 (tiles)", (append8_tiles_kernel<256, 1, true>), grid, 256, 0, stream, p);

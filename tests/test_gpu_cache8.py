@@ -131,6 +131,32 @@ def test_append(ops, H, Kh, D, page, rot, inter, seqs):
         at += n
 
 
+@pytest.mark.parametrize("H,Kh,D,page,rot,inter,seqs", [
+    (4, 4, 128, 64, 128, False, [(0, 9000, 1500), (1, 9998, 3)]),                    # whole tiles
+    (8, 8, 64, 64, 64, True, [(0, 9000, 1500)]),
+    (2, 2, 256, 64, 256, False, [(0, 9000, 500)]),
+    (16, 16, 128, 64, 128, False, [(s, 8000 + 77 * s, 1) for s in range(8)]),        # a token a sequence
+    (16, 16, 128, 64, 128, True, [(s, 8000 + 77 * s, 3) for s in range(8)]),
+    (4, 4, 80, 16, 40, False, [(0, 9000, 500)]),                                     # any sizes
+    (4, 4, 10, 8, 10, True, [(0, 900, 700)]),
+])
+def test_the_codes_of_keys_are_those_of_the_exact_rotation(ops, H, Kh, D, page, rot, inter, seqs):
+    """To the bit: a number that lies as near a border between two codes as float32 sines are off is turned in float64."""
+    max_pages = -(-max(s + n for _, s, n in seqs) // page)
+    slots = 1 + max(s for s, _, _ in seqs)
+    view, cpu = make_view(slots * max_pages, Kh, page, D, slots, max_pages, seed=3 * D)
+    freq = frequencies(rot)
+    x = rows_of(seqs, (H + 2 * Kh) * D, seed=21, size=3.0)
+    ops.rotate_append(x.cuda(), (freq.cuda(), inter, rot), make_meta(seqs), view, H)
+    rows, at = x.to(F64).view(-1, H + 2 * Kh, D), 0
+    for slot, start, n in seqs:
+        r = rows[at:at + n]
+        plain.append(cpu, slot, start, plain.turned(r[:, H:H + Kh], torch.arange(start, start + n), freq, rot, inter), r[:, H + Kh:])
+        at += n
+    assert torch.equal(view.scales[0].cpu(), cpu.scales[0]) and torch.equal(view.scales[1].cpu(), cpu.scales[1])
+    assert same_codes(view.k, cpu.k) and same_codes(view.v, cpu.v)
+
+
 def test_a_scale_grows_with_a_block_and_begins_afresh(ops):
     """Single tokens of growing and shrinking size through two blocks: the codes are those of the plain form at every step."""
     H, Kh, D, page = 2, 2, 64, 64
