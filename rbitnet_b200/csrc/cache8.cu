@@ -88,29 +88,38 @@ __device__ __forceinline__ float2 turn_of(int pos, float freq) {
   return make_float2(sn, cs);
 }
 
-// A turned key, scaled, is a float32 number off by at most `off`; its code is that of the exact number unless a border between two codes
-// lies that near.  (Steps of e4m3: an eighth of the power of two below the value, 2^-9 at least.)
-__device__ __forceinline__ bool near_border(float v, float off) {
-  const uint32_t e = max(__float_as_uint(fabsf(v)) >> 23, 121u);                 // 2^-6 and above
-  const float per_step = __uint_as_float((127u + 130u - e) << 23), t = fabsf(v) * per_step;
-  return fabsf(t - floorf(t) - 0.5f) <= off * per_step;
-}
-// Then both numbers of the pair are made in float64 from the row itself, and handed on rounded to odd, so that the rounding to a code
-// that follows is the only one: what is stored does not depend on how well float32 sines are rounded.
+// A turned pair x, y (of length r <= |x| + |y|) may be off by this: the float32 angle by pi 2^-25, which moves it by pi 2^-25 r; its sine and
+// cosine by 2^-24 each, sqrt(2) 2^-24 r; the products by 2^-24 r and the sum by 2^-24 r: 9.98 2^-25 r.  And 2^-24 r for the sums |x| +- off
+// that are looked at: where both have one code, x has it; else a border between two codes is near, and the pair is turned in float64.
+__device__ __forceinline__ float pair_off(float x, float y) { return (fabsf(x) + fabsf(y)) * 0x1.8p-22f; }
+
+// A pair turned in float64, rounded to odd, so that the rounding to a code that follows is the only one: what is stored does not depend on
+// how well float32 sines are rounded.
 __device__ __forceinline__ float to_odd(double y) {
   const float f = __double2float_rz(y);
   return (double)f == y ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
-__device__ __noinline__ float2 exact_turned(const __nv_bfloat16* first, const __nv_bfloat16* second, const float* freq, int pos, float inv) {
-  const double x0 = (double)__bfloat162float(*first), x1 = (double)__bfloat162float(*second);
-  const double turns = (double)pos * ((double)*freq * 0.15915494309189533577);
+__device__ __forceinline__ float2 exact_turned(float x0, float x1, float freq, int pos, float inv) {
+  const double turns = (double)pos * ((double)freq * 0.15915494309189533577);
   double sn, cs;
   sincospi((turns - rint(turns)) * 2.0, &sn, &cs);
   return make_float2(to_odd((x0 * cs - x1 * sn) * (double)inv), to_odd((x0 * sn + x1 * cs) * (double)inv));
 }
-// How far a turned pair x, y (of length r <= |x| + |y|) may be off: the float32 angle by pi 2^-25, which moves it by pi 2^-25 r; its sine and
-// cosine by 2^-24 each, sqrt(2) 2^-24 r; the products by 2^-24 r and the sum by 2^-24 r: 9.98 2^-25 r in all.
-__device__ __forceinline__ float pair_off(float x, float y) { return (fabsf(x) + fabsf(y)) * 0x1.4p-22f; }
+// Of eight pairs at `to`, the codes of those that are marked: a byte that is not zero in `da` or `db`, at the pair's values in the pieces
+// that begin at a0 and b0.  (Rare, so not a part of the kernels' straight line; the thread has written these codes itself.)
+__device__ __noinline__ void exact_codes(uint8_t* to, const __nv_bfloat16* head, const float* freq, int pos, float inv, uint2 da, uint2 db, int a0, int b0,
+                                         int interleaved) {
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t wa = i < 4 ? da.x : da.y, wb = i < 4 ? db.x : db.y;                               // words of byte i
+    const uint32_t w = i < 4 ? (i < 2 ? da.x : da.y) : (i < 6 ? db.x : db.y);                        // of bytes 2i, 2i + 1
+    if (!(interleaved ? w >> 16 * (i & 1) & 0xffffu : (wa | wb) >> 8 * (i & 3) & 0xffu)) continue;
+    const int x = interleaved ? a0 + 2 * i : a0 + i, y = interleaved ? x + 1 : b0 + i;
+    const float2 v = exact_turned(__bfloat162float(head[x]), __bfloat162float(head[y]), freq[i], pos, inv);
+    to[x] = to_code(v.x);
+    to[y] = to_code(v.y);
+  }
+}
 
 struct Append8 {
   __nv_bfloat16* q_out;          // [T, H, D]
@@ -198,9 +207,9 @@ __global__ void __launch_bounds__(256) append8_kernel(Append8 p) {
       b = p.interleaved ? 2 * i + 1 : i + rhalf;
       float x = rows[tok * D + a] * inv, y = rows[tok * D + b] * inv;
       const float off = pair_off(x, y);
-      if (near_border(x, off) || near_border(y, off)) {
+      if (to_code(fabsf(x) - off) != to_code(fabsf(x) + off) || to_code(fabsf(y) - off) != to_code(fabsf(y) + off)) {
         const __nv_bfloat16* head = p.qkv + (int64_t)(tok0 + tok) * p.qkv_stride + (int64_t)(p.H + kvh) * D;
-        const float2 exact = exact_turned(head + a, head + b, p.inv_freq + i, pos0 + tok, inv);
+        const float2 exact = exact_turned(__bfloat162float(head[a]), __bfloat162float(head[b]), p.inv_freq[i], pos0 + tok, inv);
         x = exact.x;
         y = exact.y;
       }
@@ -265,29 +274,24 @@ __device__ __forceinline__ float largest8(const float (&a)[8], const float (&b)[
   return m;
 }
 
-// Turned pairs of a key (a: first values, b: second ones; interleaved: values in their order) times the scale's inverse, ready for their codes.
-// head: the row's head before the rotation.
-__device__ __forceinline__ void scaled_key8(const Append8& p, float (&a)[8], float (&b)[8], const __nv_bfloat16* head, int e, int pos, float inv) {
-  uint32_t near = 0;
+// Eight pairs at `to`, as codes; turned: a key's, of which those near a border are made anew from `head`, the row's head before the rotation.
+__device__ __forceinline__ void store8(const Append8& p, uint8_t* to, const float (&a)[8], const float (&b)[8], bool turned, const __nv_bfloat16* head, int e,
+                                       int pos, float inv) {
+  *reinterpret_cast<uint2*>(to + piece_a(p, e)) = codes8(a, inv);
+  *reinterpret_cast<uint2*>(to + piece_b(p, e)) = codes8(b, inv);
+  if (!turned) return;
+  float alow[8], ahigh[8], blow[8], bhigh[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float& x = p.interleaved ? (i < 4 ? a[2 * i] : b[2 * i - 8]) : a[i];
-    float& y = p.interleaved ? (i < 4 ? a[2 * i + 1] : b[2 * i - 7]) : b[i];
-    x *= inv;
-    y *= inv;
-    const float off = pair_off(x, y);
-    if (near_border(x, off) || near_border(y, off)) near |= 1u << i;
+    const float aoff = pair_off(a[i], p.interleaved ? a[i ^ 1] : b[i]), boff = pair_off(b[i], p.interleaved ? b[i ^ 1] : a[i]);
+    alow[i] = fabsf(a[i]) - aoff;
+    ahigh[i] = fabsf(a[i]) + aoff;
+    blow[i] = fabsf(b[i]) - boff;
+    bhigh[i] = fabsf(b[i]) + boff;
   }
-  if (near == 0) return;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (!(near >> i & 1u)) continue;
-    const int pair = 8 * e + i;
-    const __nv_bfloat16* first = head + (p.interleaved ? 2 * pair : pair);
-    const float2 exact = exact_turned(first, p.interleaved ? first + 1 : first + p.cache.head_dim / 2, p.inv_freq + pair, pos, inv);
-    (p.interleaved ? (i < 4 ? a[2 * i] : b[2 * i - 8]) : a[i]) = exact.x;
-    (p.interleaved ? (i < 4 ? a[2 * i + 1] : b[2 * i - 7]) : b[i]) = exact.y;
-  }
+  const uint2 al = codes8(alow, inv), ah = codes8(ahigh, inv), bl = codes8(blow, inv), bh = codes8(bhigh, inv);
+  const uint2 da = make_uint2(al.x ^ ah.x, al.y ^ ah.y), db = make_uint2(bl.x ^ bh.x, bl.y ^ bh.y);
+  if (da.x | da.y | db.x | db.y) exact_codes(to, head, p.inv_freq + 8 * e, pos, inv, da, db, piece_a(p, e), piece_b(p, e), p.interleaved);
 }
 
 // Heads of a multiple of 16 values, turned whole, rows on 16 bytes: a block of threads per (tile, kv head).  A thread takes one piece of
@@ -295,9 +299,9 @@ __device__ __forceinline__ void scaled_key8(const Append8& p, float (&a)[8], flo
 // registers, turns the key's piece and those of the G query heads with them, and keeps the key's and the value's pieces until the
 // block's largest values have met.  16-byte loads and stores; the blocks of a tile's kv heads run side by side, so that rows are read whole.
 // What bounds it is the chain of waits of a block (tile, positions, rows, the largest values), hidden behind the blocks beside it: 8,192
-// tokens of 32 heads on 8 kv heads of 128, 184 MB in 51 us, 3.6 TB/s; 45 us but for the keys that lie near a border (a warp in about 100
-// makes its sines in float64, and its block waits).  Measured in float32 alone: 44 us, sines and cosines through shared memory and 256
-// threads 64, 92 registers and one block an SM 60.  16 sequences of up to five tokens, 32 heads of 64 on 4: 3.3 us.
+// tokens of 32 heads on 8 kv heads of 128, 184 MB in 51 us, 3.6 TB/s, of which looking for keys near a border takes 4 and turning those anew
+// 2.5 (the same in one straight line: 51.5, and a row of the step kernel 3.7 for 2.7).  Measured without it: 44 us, sines and cosines through shared memory and 256
+// threads 64, 92 registers and one block an SM 60.  16 sequences of up to five tokens, 32 heads of 64 on 4: 2.9 us.
 template <int THREADS, int SPAN, bool SHARED>
 __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append8_tiles_kernel(Append8 p) {
   rb_pdl_launch_dependents();
@@ -393,13 +397,7 @@ __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append
         *reinterpret_cast<uint2*>(to + piece_a(p, e[i])) = codes8(a, inv);
         *reinterpret_cast<uint2*>(to + piece_b(p, e[i])) = codes8(b, inv);
       } else {
-        float by = inv;
-        if (p.rot_dim) {
-          scaled_key8(p, ka[i], kb[i], rows + (int64_t)tok[i] * p.qkv_stride + (int64_t)(p.H + kvh) * D, e[i], pos0 + tok[i], inv);
-          by = 1.f;
-        }
-        *reinterpret_cast<uint2*>(to + piece_a(p, e[i])) = codes8(ka[i], by);
-        *reinterpret_cast<uint2*>(to + piece_b(p, e[i])) = codes8(kb[i], by);
+        store8(p, to, ka[i], kb[i], p.rot_dim > 0, rows + (int64_t)tok[i] * p.qkv_stride + (int64_t)(p.H + kvh) * D, e[i], pos0 + tok[i], inv);
       }
     }
     if (threadIdx.x == 0) (s ? p.v_scale : p.k_scale)[unit] = now;
@@ -407,8 +405,8 @@ __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append
 }
 
 // The same for one token a tile (a decode step): a warp per (row, kv head), up to 8 kv heads a block; the sines and cosines once a block.
-// What bounds it is latency: a wait, the row, the old scales, the codes.  One row of 32 heads on 8 kv heads of 128: 3.5 us, 64 rows 4.3
-// (2.9 and 3.3 where no key lies near a border).
+// What bounds it is latency: a wait, the row, the old scales, the codes.  One row of 32 heads on 8 kv heads of 128: 2.7 us, 64 rows 3.5
+// (3.1 where no key lies near a border).
 __global__ void __launch_bounds__(256) append8_step_kernel(Append8 p) {
   rb_pdl_launch_dependents();
   extern __shared__ float2 turns[];              // [D / 2]
@@ -464,16 +462,8 @@ __global__ void __launch_bounds__(256) append8_step_kernel(Append8 p) {
       uint8_t* v = (uint8_t*)p.cache.v + at;
       if (old_k < now_k) rescale16(k, before * D, old_k / now_k, lane, 32);
       if (old_v < now_v) rescale16(v, before * D, old_v / now_v, lane, 32);
-      if (is_k || is_v) {
-        float inv = 1.0f / (is_k ? now_k : now_v);
-        if (is_k && p.rot_dim) {
-          scaled_key8(p, a, b, src + head * D, e, pos, inv);
-          inv = 1.f;
-        }
-        uint8_t* to = (is_k ? k : v) + before * D;
-        *reinterpret_cast<uint2*>(to + piece_a(p, e)) = codes8(a, inv);
-        *reinterpret_cast<uint2*>(to + piece_b(p, e)) = codes8(b, inv);
-      }
+      if (is_k || is_v)
+        store8(p, (is_k ? k : v) + before * D, a, b, is_k && p.rot_dim > 0, src + head * D, e, pos, 1.0f / (is_k ? now_k : now_v));
       if (lane == 0) { p.k_scale[unit] = now_k; p.v_scale[unit] = now_v; }
     }
   }
