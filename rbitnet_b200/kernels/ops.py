@@ -790,7 +790,7 @@ class CudaOps:
                               f"{view.head_dim}")
         keep = int(keep_first or 0) if win else 0
         # how a step's rows are cut is the same for all of its layers of these sizes
-        key = ("attention8", H, Kh, D, win, keep, self.cache8_rows)
+        key = ("attention8", H, Kh, D, view.page_size, win, keep, self.cache8_rows)
         cut = meta.extra.get(key)
         if cut is None:
             cut = meta.extra[key] = self._cut_rows8(meta, view, T, H, Kh, D, win, keep)
@@ -839,7 +839,7 @@ class CudaOps:
         """Many rows a sequence: the codes that the step sees become bfloat16 pages once, and the attention over those follows
         (a tile of rows would have to turn every code again: 64 times in a prompt of 2,048 tokens of 32 heads)."""
         import numpy as np
-        key = ("unpacked", view.page_size, window, keep, view.page_table.data_ptr())
+        key = ("unpacked", view.page_size, view.max_pages, view.page_table.shape[0], window, keep)
         if key not in meta.extra:
             P, ranges = view.page_size, []
             for c in meta.seqs:

@@ -258,6 +258,25 @@ def test_attention(ops, H, Kh, D, page, seqs, window, sinks, cap, keep):
         at += n
 
 
+@pytest.mark.parametrize("new", [1, 3, 90])
+def test_one_step_over_caches_of_different_pages(ops, new):
+    """What a step keeps for its layers goes by the pages' size and the table's, so that layers of another cache get their own."""
+    H, Kh, D = 4, 2, 64
+    seqs = [(0, 130, new), (2, 40, new)]
+    meta = make_meta(seqs)
+    q = rows_of(seqs, H * D, seed=4).view(-1, H, D)
+    for i, (page, spare, slots) in enumerate([(64, 0, 4), (16, 0, 4), (64, 3, 3), (128, 0, 4), (64, 0, 4)]):
+        max_pages = -(-(130 + new) // page) + spare
+        view, cpu = make_view(slots * max_pages, Kh, page, D, slots, max_pages, seed=50 + i)
+        got = ops.attention(q.cuda(), meta, view, H, D ** -0.5, 0).cpu().to(F64)
+        at = 0
+        for slot, start, n in seqs:
+            want, size = plain.attend(cpu, slot, start, q[at:at + n], D ** -0.5)
+            off = (got[at:at + n] - want).abs()
+            assert torch.all(off <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size + 1e-30), (i, float((off / (size + 1e-30)).max()))
+            at += n
+
+
 def drafts_case(B, most, V, certain, seed, ragged=True):
     g = torch.Generator().manual_seed(seed)
     rows = [1 + (most if not ragged else int(torch.randint(0, most + 1, (1,), generator=g))) for _ in range(B)]
