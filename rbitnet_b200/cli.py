@@ -44,6 +44,8 @@ def _engine(args):
 
 
 def cmd_generate(args) -> int:
+    if args.prompt is not None and args.draft_tokens:
+        raise SystemExit("--draft-tokens goes with --prompt-ids, not with --prompt")
     eng = _engine(args)
     if args.prompt is not None:
         for text in args.prompt:

@@ -170,10 +170,12 @@ class NormedRows:
 @dataclass
 class CacheRanges:
     """Pages of sequences whose values are read back (``CudaOps.cache_ranges``): ``items`` int32 [count, 3] (slot, page of the
-    sequence, positions in use), ``first_item`` the first page of every range."""
+    sequence, positions in use), ``first_item`` the first page of every range, ``sizes`` the slots, a slot's most pages and the page
+    size of the caches that they are pages of."""
     items: torch.Tensor
     count: int
     first_item: List[int]
+    sizes: tuple
 
 
 #: per device: the workspace of the tensor-core products (arrival counters, then partial sums of
@@ -767,13 +769,17 @@ class CudaOps:
                                   f"{view.max_pages * page} positions")
             first_item.append(len(items))
             items.extend((slot, i, min(page, end - i * page)) for i in range(first // page, -(-end // page)))
-        return CacheRanges(upload(np.asarray(items, dtype=np.int32).reshape(-1, 3), self.device), len(items), first_item)
+        return CacheRanges(upload(np.asarray(items, dtype=np.int32).reshape(-1, 3), self.device), len(items), first_item,
+                           (slots, view.max_pages, page))
 
     def cache_values(self, view, ranges: CacheRanges):
         """Keys and values of the ranges' pages as bfloat16 [pages, kv heads, page size, head size] each: what the codes of a cache
         held in 8 bits stand for (exactly), and zeros behind a range's end."""
         if not view.scales:
             raise KernelError("cache_values: the cache holds its values in the compute dtype")
+        if ranges.sizes != (view.page_table.shape[0], view.max_pages, view.page_size):
+            raise KernelError(f"cache_values: ranges of (slots, pages, page size) {ranges.sizes}, a cache of "
+                              f"{(view.page_table.shape[0], view.max_pages, view.page_size)}")
         self._check_cache8(view, "cache_values")
         k, v = torch.empty((2, ranges.count, view.n_kv_heads, view.page_size, view.head_dim), dtype=torch.bfloat16, device=self.device)
         self.lib.call("rb_cache8_values", k.data_ptr(), v.data_ptr(), ranges.items.data_ptr(), ranges.count, *_cache8(view), view.max_pages,

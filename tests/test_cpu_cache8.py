@@ -1,5 +1,6 @@
 """The cache held in 8 bits and drafted steps without a GPU: the plain forms against themselves, the host's part, the refusals."""
 import math
+from dataclasses import replace
 
 import pytest
 import torch
@@ -247,3 +248,21 @@ def test_kernel_calls_that_are_refused_before_anything_is_launched():
     for args in ((z, i, i, torch.zeros(2), f, 1), (z.double(), i, i, torch.zeros(2), f, 1), (z[0], i, i, torch.zeros(2), f, 1)):
         with pytest.raises(KernelError, match="verify_drafts"):
             bare_ops().verify_drafts(*args)
+
+
+def test_ranges_of_a_cache_of_other_sizes_are_refused():
+    """(Their slots and pages would be looked up outside the other cache's table.)"""
+    ops = bare_ops()
+    made = ops.cache_ranges(view_of(), [(1, 0, 128)])
+    for other in (view_of(page=32), replace(view_of(), max_pages=1, page_table=torch.zeros(2, 1, dtype=torch.int32)),
+                  replace(view_of(), page_table=torch.zeros(1, 2, dtype=torch.int32))):
+        with pytest.raises(KernelError, match="ranges of"):
+            ops.cache_values(other, made)
+    with pytest.raises(KernelError, match="CUDA device"):
+        ops.cache_values(view_of(), made)
+
+
+def test_the_command_line_refuses_drafts_for_text(tmp_path):
+    from rbitnet_b200.cli import main
+    with pytest.raises(SystemExit, match="draft-tokens"):
+        main(["generate", "--model", str(tmp_path), "--draft-tokens", "2", "--prompt", "text"])
