@@ -467,6 +467,42 @@ __device__ __forceinline__ void run(const Params& p, const CUtensorMap* tmK, con
           }
         }
       }
+      // (a NaN among values that some of the tile's tokens see and others do not would stay in the others' rows: a token at a time then)
+      if (!whole && w.ntok > 1) {
+        uint32_t nan = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int x = 0; x < VW; ++x) nan |= ((v[k][x] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        if (__any_sync(0xffffffffu, nan != 0)) {
+#pragma unroll 1
+          for (int q = w.pos0; q <= w.key_hi; ++q) {
+            uint32_t seen[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int key = key0 + 16 * u + 2 * t + (k & 1) + (k >> 1) * 8;
+              seen[k] = key > q || (p.a.window > 0 && key <= q - p.a.window && key >= p.a.keep) ? 0u : 0xffffffffu;
+            }
+#pragma unroll
+            for (int x = 0; x < VW; ++x)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const uint32_t ab = __byte_perm(v[0][x] & seen[0], v[1][x] & seen[1], y == 0 ? 0x5140 : 0x7362);
+                const uint32_t cd = __byte_perm(v[2][x] & seen[2], v[3][x] & seen[3], y == 0 ? 0x5140 : 0x7362);
+                const uint32_t a0 = half2_lo(ab), a1 = half2_hi(ab), a2 = half2_lo(cd), a3 = half2_hi(cd);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  float (&to)[4] = o[n][2 * x + y];
+                  float sum[4] = {to[0], to[1], to[2], to[3]};
+                  mma_f16(sum, a0, a1, a2, a3, pf[u][n][0], pf[u][n][1]);
+#pragma unroll
+                  for (int c = 0; c < 4; ++c) to[c] = pos[n][c & 1] == q ? sum[c] : to[c];
+                }
+              }
+          }
+          continue;
+        }
+      }
 #pragma unroll
       for (int x = 0; x < VW; ++x)
 #pragma unroll

@@ -633,3 +633,34 @@ for bad in (lambda m: ops.rotate_append(rows_of([(0, 0, 1)], 8 * 128).cuda(), No
     out = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), env=env,
                          capture_output=True, text=True, timeout=600)
     assert out.returncode == 0 and out.stdout.split() == ["seen", "seen"], out.stdout + out.stderr
+
+
+@pytest.mark.parametrize("H,Kh,D,B,start,n,window,keep", [(8, 2, 128, 1, 130, 4, 0, 0), (8, 2, 128, 1, 250, 5, 60, 10), (16, 4, 64, 1, 61, 7, 0, 0),
+                                                          (8, 8, 128, 100, 61, 5, 0, 0), (8, 2, 64, 60, 700, 8, 0, 0)])
+def test_a_later_token_of_the_step_may_hold_nan(ops, H, Kh, D, B, start, n, window, keep):
+    """NaN among values that only some of a step's tokens see: a drafted token's, and a window's oldest; just the sums of the rows that see
+    them are NaN (one sequence: a cluster's parts; many: a warp a pair, or tiles dealt out)."""
+    page = 64
+    max_pages = -(-(start + n) // page)
+    view, cpu = make_view(B * max_pages, Kh, page, D, B, max_pages, seed=D + n)
+    places = [(start + 2, 0, 5), (start + n - 1, Kh - 1, D - 1)] + ([(start - window + 2, Kh - 1, 7)] if window else [])
+    for slot in range(B):
+        for pos, kvh, d in places:
+            for v in (view, cpu):
+                v.v.view(torch.uint8)[int(cpu.page_table[slot, pos // page]), kvh, pos % page, d] = 0x7f
+                v.k.view(torch.uint8)[int(cpu.page_table[slot, (start + 3) // page]), 0, (start + 3) % page, 1] = 0xff
+    seqs = [(slot, start, n) for slot in range(B)]
+    q = rows_of(seqs, H * D, seed=7).view(-1, H, D)
+    got = ops.attention(q.cuda(), make_meta(seqs), view, H, D ** -0.5, window, keep_first=keep).cpu().to(F64).view(B, n, H * D)
+    some = 0
+    for slot in (0, B // 2, B - 1):
+        for i in range(n):
+            row = q[slot * n + i][None]
+            want, size = plain.attend(cpu, slot, start + i, row, D ** -0.5, window, None, 0.0, keep)
+            nan = want[0].isnan()
+            some += int(nan.sum())
+            assert torch.equal(got[slot, i].isnan(), nan), (slot, i)
+            fine = ~nan
+            assert torch.all((got[slot, i] - want[0]).abs()[fine] <= (2.0 ** -8 * want[0].abs() + (2.0 ** -8 + 2.0 ** -14) * size[0])[fine])
+            assert i > 1 or not nan[5]
+    assert some
