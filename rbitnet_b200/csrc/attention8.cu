@@ -1,7 +1,8 @@
 // Attention over the cache held in 8 bits (cache8.cu): value = code * scale, a power-of-two scale per block of positions and
 // kv head.  Token t at position p of its sequence sees keys max(0, p - window + 1) .. p (and with keep_first the first keys);
 // score = (q.k) * scale, in float32, capped where a soft cap is set; softmax with the running maximum and sum in float32 (the
-// sink one more term of the sum); o = sum of p v.  A key that a row does not see is not multiplied by anything.
+// sink one more term of the sum); o = sum of p v.  A key that a row does not see is not multiplied by anything
+// (but in steps of more than 64 rows a kv head, whose bfloat16 pages the prefill kernel reads: there a NaN value of a prompt reaches earlier tokens of its tile).
 #include "attention8.cuh"
 
 #include <cuda_fp8.h>

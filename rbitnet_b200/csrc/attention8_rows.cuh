@@ -27,7 +27,7 @@
 // 541 MB in 90 us, 6.0 TB/s (0.92 of a copy).  Short pairs are bound by what a pair costs to begin and to join (about 5 us in a block, two
 // blocks an SM) or, a pair a warp, by a warp's chain from score to sum, a microsecond for 32 keys: 24 sequences of 32 heads with a window of
 // 1,024, 202 MB in 45 us, 4.5 TB/s.  More rows add products and exponentials: 16
-// sequences of up to five tokens at up to 6,001 positions, 20 rows, 101 MB in 40 us.  One sequence at 2,048 positions: 8 us, waits.
+// sequences of up to five tokens at up to 6,001 positions, 20 rows, 101 MB in 42 us.  One sequence at 2,048 positions: 8 us, waits.
 // Measured beside it (the first of these): 16-byte cp.async by every thread 154 us, of which the copies alone 136; boxes of 16 positions
 // 126 to 136; two stages and three blocks an SM 109; pairs dealt out without what their beginnings cost 113.
 #pragma once
@@ -212,7 +212,9 @@ template <int D, int NT> struct Sums {
 };
 
 // The warp's way through a segment, whose first S::NS - 1 units have been asked for.
-template <int D, int NT, int ALONE>
+// ONE: every row tile is a single token, so that its rows see the same keys (the code for a NaN that only some see,
+// though not run there, cost such steps 94 -> 101 us; without it 91 - 98).
+template <int D, int NT, int ALONE, bool ONE = false>
 __device__ __forceinline__ void run(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV, Job<D, NT, ALONE>& job, uint8_t* smem,
                                     uint8_t* stages, uint64_t* full, Ring& ring, Sums<D, NT>& sums) {
   using S = typename Job<D, NT, ALONE>::S;
@@ -468,7 +470,7 @@ __device__ __forceinline__ void run(const Params& p, const CUtensorMap* tmK, con
         }
       }
       // (a NaN among values that some of the tile's tokens see and others do not would stay in the others' rows: a token at a time then)
-      if (!whole && w.ntok > 1) {
+      if (!ONE && !whole && w.ntok > 1) {
         uint32_t nan = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -521,7 +523,7 @@ __device__ __forceinline__ void run(const Params& p, const CUtensorMap* tmK, con
 }
 
 // The block's part of a pair, whose first S::AHEAD units have been asked for; `then` asks for those of the pair after it.
-template <int D, int NT, typename F>
+template <int D, int NT, bool ONE, typename F>
 __device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV, Job<D, NT>& job, uint8_t* smem,
                                      Ring& ring, Joined<D, NT>& joined, F then) {
   using S = Shape<D, NT>;
@@ -532,7 +534,7 @@ __device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, co
 #pragma unroll
   for (int i = S::AHEAD; i < S::NS - 1; ++i) job.ask(p, tmK, tmV, stages, full, ring, i);
   Sums<D, NT> sums;
-  run<D, NT, 0>(p, tmK, tmV, job, smem, stages, full, ring, sums);
+  run<D, NT, 0, ONE>(p, tmK, tmV, job, smem, stages, full, ring, sums);
   auto& o = sums.o;
   auto& m = sums.m;
   auto& l = sums.l;
@@ -671,7 +673,7 @@ __global__ void __launch_bounds__(WARPS * 32) cluster_kernel(const __grid_consta
     for (int i = 0; i < S::AHEAD; ++i) job.ask(p, &tmK, &tmV, stages, full, ring, i);
   }
   Joined<D, NT> mine;
-  work<D, NT>(p, &tmK, &tmV, job, smem, ring, mine, [](uint8_t*, uint64_t*) {});
+  work<D, NT, false>(p, &tmK, &tmV, job, smem, ring, mine, [](uint8_t*, uint64_t*) {});
   const Where& w = job.w;
   if (p.parts == 1) {
     store<D, NT>(p, w, seg.kvh, mine);
@@ -743,7 +745,7 @@ __device__ __forceinline__ int block_count(int v, int* s) {
   return sum;
 }
 
-template <int D, int NT>
+template <int D, int NT, bool ONE>
 __global__ void __launch_bounds__(WARPS * 32) dealt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, Params p) {
   rb_pdl_launch_dependents();
   using S = Shape<D, NT>;
@@ -815,7 +817,7 @@ __global__ void __launch_bounds__(WARPS * 32) dealt_kernel(const __grid_constant
     const Segment now = seg;
     const Where w = job.w;
     Joined<D, NT> mine;
-    work<D, NT>(p, &tmK, &tmV, job, smem, ring, mine, [&](uint8_t* stages, uint64_t* full) {
+    work<D, NT, ONE>(p, &tmK, &tmV, job, smem, ring, mine, [&](uint8_t* stages, uint64_t* full) {
       seg = next_segment();
       if (seg.tile < 0) return;
       job = Job<D, NT>(p, seg);
@@ -955,10 +957,11 @@ template <int D, int NT> int per_sm() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= RB_MAX_DEVICES) dev = 0;
   if (n[dev] == 0) {
     int v = 0;
-    if (cudaFuncSetAttribute(dealt_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D, NT>::BYTES) != cudaSuccess ||
+    if (cudaFuncSetAttribute(dealt_kernel<D, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D, NT>::BYTES) != cudaSuccess ||
+        cudaFuncSetAttribute(dealt_kernel<D, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D, NT>::BYTES) != cudaSuccess ||
         cudaFuncSetAttribute(cluster_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D, NT>::BYTES) != cudaSuccess ||
         cudaFuncSetAttribute(cluster_kernel<D, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, dealt_kernel<D, NT>, WARPS * 32, Shape<D, NT>::BYTES) != cudaSuccess || v < 1)
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, dealt_kernel<D, NT, false>, WARPS * 32, Shape<D, NT>::BYTES) != cudaSuccess || v < 1)
       v = 1;
     (void)cudaGetLastError();
     n[dev] = v;
@@ -1025,7 +1028,8 @@ int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, int bl
   }
   per_sm<D, NT>();                                 // (sets the kernels' attributes)
   if (p.parts == 0) {
-    RB_LAUNCH("rb_attention8_rows", (dealt_kernel<D, NT>), blocks, WARPS * 32, S::BYTES, stream, tk, tv, p);
+    if (p.tile_tok0) RB_LAUNCH("rb_attention8_rows", (dealt_kernel<D, NT, false>), blocks, WARPS * 32, S::BYTES, stream, tk, tv, p);
+    else RB_LAUNCH("rb_attention8_rows", (dealt_kernel<D, NT, true>), blocks, WARPS * 32, S::BYTES, stream, tk, tv, p);
     RB_LAUNCH("rb_attention8_rows (join)", (join_kernel<D, NT>), dim3(p.n_tiles, p.Kh, NT), D * 2, 0, stream, p, blocks);
     return 0;
   }
