@@ -628,6 +628,8 @@ class CudaOps:
         softcap); ``keep_first`` > 0 with a window: the sequence's first so many positions stay visible wherever the window
         is.  Every attention kernel of the library takes them all.  A cache held in 8 bits is read as the values its codes
         stand for."""
+        if q.data_ptr() & 15:
+            q = q.clone()              # (a part of a wider tensor: the kernels load 16 bytes at a time)
         if view.scales:
             return self._attention8(q, meta, view, n_heads, scale, window, sinks, softcap, keep_first)
         T, H, D = q.shape
@@ -802,7 +804,7 @@ class CudaOps:
             cut = meta.extra[key] = self._cut_rows8(meta, view, T, H, Kh, D, win, keep)
         in_rows, tok0, ntok, n_tiles, rows, parts, blocks, n_o, n_ml = cut
         at_q, cache = q.data_ptr(), _cache8(view)
-        in_rows = in_rows and not (at_q | cache[0] | cache[1]) & 15
+        in_rows = in_rows and not (cache[0] | cache[1]) & 15
         if not in_rows and not meta.single_token:
             return self._attention_unpacked(q, meta, view, n_heads, scale, window, sinks, softcap, keep)
         out = q.new_empty((T, H * D))
