@@ -7,17 +7,20 @@
 // The products are mma.sync m16n8k16 in float16 with the KEYS as the 16 rows of the first, and the head's values as the 16 rows of the
 // second, so that eight query rows fill an instruction:
 //     S^T[16 keys, 8 rows] = K[16, D] Q^T           O^T[D, 8 rows] += V^T[D, 16 keys] P^T[16 keys, 8 rows]
-// A code is a float16 value (cvt, exactly), so neither product rounds its operands but P, to float16 (2^-11; P is 256 at most and sums
-// are float32); Q, bfloat16, is brought to the middle of float16's range by a power of two a row.  The order of a product's inner index
+// A code is a float16 value (cvt, exactly), so neither product rounds its operands but P, to float16 (below; sums are float32);
+// Q, bfloat16, is brought to the middle of float16's range by a power of two a row.  The order of a product's inner index
 // and of its rows is free as long as both sides agree, and it is chosen so that every operand register is made of whole 16-byte pieces of
 // the cache as they lie: of keys g and g + 8 the pieces 16 t .. 16 t + 15 of every 64 values, of values 2t, 2t + 1, 2t + 8, 2t + 9 the pieces
 // D/8 g .. (lane = 4 g + t): no shuffle and no transposing load between the cache's bytes and the products.
 // A warp has a ring of its own in shared memory, filled by TMA (two boxes of 32 positions, 128-byte swizzle, no bank conflicts) and waited
 // for at its own barriers: the warps of a block meet only at the end.
 //
-// O is kept in units of a values' scale `unit`, which follows the tiles' scales lazily: P is multiplied by scale / unit, and O
-// is brought to another unit (exactly: powers of two) only where that ratio leaves 2^-6 .. 2^4.  Likewise the exponents' reference
-// moves only when a maximum has grown by more than 8.
+// What a sum is made of is a weight times its values' scale, and either may be small where the other is large.  So the sum of weights goes by
+// a row's largest score m (base-2 units), but O by r, the logarithm of the largest weight 2^(score - m) times scale so far: the second
+// product's operand is P' = 2^(score - m) scale 2^(7 - r), rounded to float16, and O is kept times 2^(7 - r).  Both follow lazily, moved only where
+// they have been passed by more than 8, so that P' is 2^15 at most.  Rounding leaves a P' within 2^-11 of itself where weight times
+// scale is 2^-21 of the largest or more, and within 2^-32 of the largest below that.  (A tile's largest weight counts as 2^-96 at least for r,
+// so that 2^(7 - r) scale is a float32 number, as the weights are: 2^-126 of the largest and less is 0.)
 //
 // Ranges of keys: in a small grid the parts of a (tile, kv head) are a thread-block cluster and merge on chip.  In a larger one
 // all tiles of keys of all (row tile, kv head) pairs, in order, are dealt out evenly to the blocks, whatever the sequences' lengths; a
@@ -42,6 +45,8 @@ namespace rows8 {
 
 constexpr int WARPS = 4, TILE = 64;
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float FLOOR = -3.4028234663852886e38f;  // a maximum of nothing: -inf but for differences, which are numbers
+constexpr float UP = 7.f, SLACK = 8.f, LEAST = -96.f;
 
 struct Params {
   Params8 a;
@@ -206,9 +211,10 @@ template <int D, int NT, int ALONE = 0> struct Job {
   }
 };
 
-// A warp's sums: O^T in units of `unit`, maxima in base-2 units, this lane's part of the sums of the weights; rows 2t, 2t + 1 of every eight.
+// A warp's sums: O^T and what it is to be multiplied by, maxima in base-2 units, this lane's part of the sums of the weights; rows 2t, 2t + 1 of
+// every eight.
 template <int D, int NT> struct Sums {
-  float o[NT][D / 16][4], m[NT][2], l[NT][2], unit;
+  float o[NT][D / 16][4], by[NT][2], m[NT][2], l[NT][2];
 };
 
 // The warp's way through a segment, whose first S::NS - 1 units have been asked for.
@@ -282,24 +288,23 @@ __device__ __forceinline__ void run(const Params& p, const CUtensorMap* tmK, con
   auto& o = sums.o;
   auto& m = sums.m;
   auto& l = sums.l;
-  float unit = 1.f;
+  float r[NT][2];                  // the logarithm of the largest weight times scale
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      m[n][c] = -INFINITY;
+      m[n][c] = r[n][c] = FLOOR;
       l[n][c] = 0.f;
       const int rc = n * 8 + 2 * t + c;
       if (p.a.sinks != nullptr && seg.first == 0 && seg.last > 0 && (ALONE || warp == 0) && rc < n_rows) {     // counted once: by the part with the first tile
-        m[n][c] = p.a.sinks[kvh * G + rc % G] * LOG2E;
+        m[n][c] = fminf(fmaxf(p.a.sinks[kvh * G + rc % G] * LOG2E, FLOOR), -FLOOR);
         l[n][c] = g == 0 ? 1.f : 0.f;
       }
     }
   }
 
-  bool begun = false;
   for (int kt = job.begin; kt < job.end && !ring.failed; kt += job.STEP) {
     const float2 scales = job.scales[0];
 #pragma unroll
@@ -389,22 +394,15 @@ __device__ __forceinline__ void run(const Params& p, const CUtensorMap* tmK, con
           top[n][c] = x;
         }
     }
+    // the values' scale as 2^at_scale x mantissa (a power of two but for a block that nothing was appended to, whose scale may be 0)
+    const int exponent = (int)(__float_as_uint(scales.y) >> 23);
+    const float at_scale = (float)(exponent - 127), mantissa = scales.y * __uint_as_float((uint32_t)(254 - exponent) << 23);
     bool moved = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) moved |= top[n][c] > m[n][c] + 8.f || (m[n][c] == -INFINITY && top[n][c] > -INFINITY);
-    float ratio = scales.y / unit;
-    const bool other_unit = !begun || ratio > 16.f || ratio < 0.015625f;
-    begun = true;
-    if (__any_sync(0xffffffffu, moved) || other_unit) {
-      float to = 1.f;
-      if (other_unit) {
-        const float next = fmaxf(scales.y, unit * 0x1p-90f);      // (O stays finite)
-        to = unit / next;
-        unit = next;
-        ratio = scales.y / unit;
-      }
+      for (int c = 0; c < 2; ++c) moved |= fmaxf(top[n][c] - m[n][c], LEAST) > fminf(r[n][c] + (SLACK - at_scale), SLACK);
+    if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float corr[2];
@@ -414,13 +412,17 @@ __device__ __forceinline__ void run(const Params& p, const CUtensorMap* tmK, con
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          corr[c] = 1.f;
-          if (x > m[n][c] + 8.f || (m[n][c] == -INFINITY && x > -INFINITY)) {
-            corr[c] = m[n][c] == -INFINITY ? 0.f : exp2f(m[n][c] - x);
+          if (x - m[n][c] > SLACK) {
+            l[n][c] *= exp2f(m[n][c] - x);
+            r[n][c] += m[n][c] - x;
             m[n][c] = x;
           }
-          l[n][c] *= corr[c];
-          corr[c] *= to;
+          const float y = fmaxf(x - m[n][c], LEAST) + at_scale;
+          corr[c] = 1.f;
+          if (y > r[n][c] + SLACK) {
+            corr[c] = exp2f(r[n][c] - y);
+            r[n][c] = y;
+          }
         }
 #pragma unroll
         for (int u = 0; u < MT; ++u) {
@@ -433,15 +435,16 @@ __device__ __forceinline__ void run(const Params& p, const CUtensorMap* tmK, con
     uint32_t pf[KG][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+      const float m0 = m[n][0], m1 = m[n][1];
+      const float f0 = exp2_fast(UP + at_scale - r[n][0]) * mantissa, f1 = exp2_fast(UP + at_scale - r[n][1]) * mantissa;
 #pragma unroll
       for (int u = 0; u < KG; ++u) {
         const float p0 = exp2_fast(s[u][n][0] - m0), p1 = exp2_fast(s[u][n][1] - m1);
         const float p2 = exp2_fast(s[u][n][2] - m0), p3 = exp2_fast(s[u][n][3] - m1);
         l[n][0] += p0 + p2;
         l[n][1] += p1 + p3;
-        pf[u][n][0] = transposed(pack_half2(p0 * ratio, p1 * ratio));
-        pf[u][n][1] = transposed(pack_half2(p2 * ratio, p3 * ratio));
+        pf[u][n][0] = transposed(pack_half2(p0 * f0, p1 * f1));
+        pf[u][n][1] = transposed(pack_half2(p2 * f0, p3 * f1));
       }
     }
     // ---- O^T += V^T P^T: of keys 2t, 2t + 1, 2t + 8, 2t + 9 the bytes 2u (row g) and 2u + 1 (row g + 8)
@@ -519,7 +522,10 @@ __device__ __forceinline__ void run(const Params& p, const CUtensorMap* tmK, con
     __syncwarp();                    // everybody has left this stage: it may be filled again
   }
 
-  sums.unit = unit;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) sums.by[n][c] = exp2f(r[n][c] - UP);
 }
 
 // The block's part of a pair, whose first S::AHEAD units have been asked for; `then` asks for those of the pair after it.
@@ -538,7 +544,7 @@ __device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, co
   auto& o = sums.o;
   auto& m = sums.m;
   auto& l = sums.l;
-  const float unit = sums.unit;
+  auto& by = sums.by;
   // ---- the next pair's first tiles, which arrive meanwhile; then the four warps: each leaves its accumulators, as its lanes hold them,
   // in those stages of its own ring that are not being filled, and takes a quarter of the row tiles from all
   const uint32_t beside = ring.asked + S::AHEAD;
@@ -554,7 +560,7 @@ __device__ __forceinline__ void work(const Params& p, const CUtensorMap* tmK, co
   for (int n = 0; n < NT; ++n) {
     float4* to = left(warp, beside, n);
 #pragma unroll
-    for (int u = 0; u < MT; ++u) to[u * 32] = make_float4(o[n][u][0] * unit, o[n][u][1] * unit, o[n][u][2] * unit, o[n][u][3] * unit);
+    for (int u = 0; u < MT; ++u) to[u * 32] = make_float4(o[n][u][0] * by[n][0], o[n][u][1] * by[n][1], o[n][u][2] * by[n][0], o[n][u][3] * by[n][1]);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       float sum = l[n][c];
@@ -935,7 +941,7 @@ __global__ void __launch_bounds__(32) alone_kernel(const __grid_constant__ CUten
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const int r = n * 8 + 2 * t + c;
         if (r < w.ntok * p.G) {
-          const float by = sums.unit / sum;
+          const float by = sums.by[n][c] / sum;
           uint32_t out[D / 16];
 #pragma unroll
           for (int u = 0; u < D / 16; ++u) {

@@ -1,9 +1,12 @@
 """The 8-bit cache's kernels at their edges, against plain 64-bit torch or against themselves; tolerances as in test_gpu_cache8."""
+import math
+
 import pytest
 import torch
 
+import plain_cache8 as plain
 from rbitnet_b200.cache import CacheLayerView
-from test_gpu_cache8 import BF16, make_meta, make_view, rows_of
+from test_gpu_cache8 import BF16, F64, make_meta, make_view, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +37,86 @@ def test_queries_that_begin_anywhere(ops, H, Kh, D, seqs, window, bits):
         q = base[off:off + T * H * D].view(T, H, D)
         want = ops.attention(q.clone(), make_meta(seqs), view, H, D ** -0.5, window)
         assert torch.equal(ops.attention(q, make_meta(seqs), view, H, D ** -0.5, window), want), off
+
+
+def uneven_view(B, Kh, D, tiles, seed, step=8, far=40):
+    """A view whose tiles' values are of very different scales (2^-far .. 2^far, `step` apart), and whose keys weigh them against it: a
+    query with 5 as its first value (score scale 0.2) gives a tile of scale 2^e about 2^-e of the weight, so that all tiles count."""
+    view, cpu = make_view(B * tiles, Kh, 64, D, B, tiles, seed=seed)
+    g = torch.Generator().manual_seed(seed)
+    e = torch.randint(-far // step, far // step + 1, (B * tiles, Kh, 1), generator=g) * step
+    codes = (torch.randn(B * tiles, Kh, 64, D, generator=g) * 4).to(torch.float8_e4m3fn)
+    codes[..., 0] = (-e.expand(-1, -1, 64) * (math.log(2.0) / 0.125)).to(torch.float8_e4m3fn)
+    for v in (view, cpu):
+        v.k.view(torch.uint8).copy_(codes.view(torch.uint8))
+        v.scales[0].fill_(0.125)
+        v.scales[1].copy_(torch.exp2(e.float()))
+    return view, cpu
+
+
+def attended_as_plain(ops, view, cpu, seqs, q, scale, window=0, sink=None, cap=0.0, keep=0, cut=None):
+    """The attention of a step beside the plain form's.  ``cut``: "cluster", "dealt" or "alone", the way that the step has to go."""
+    H, meta = q.shape[1], make_meta(seqs)
+    got = ops.attention(q.cuda(), meta, view, H, scale, window, sinks=None if sink is None else sink.cuda(), softcap=cap, keep_first=keep)
+    if cut is not None:
+        parts = [v[5] for k, v in meta.extra.items() if k[0] == "attention8"][0]
+        assert cut == ("cluster" if parts > 0 else "dealt" if parts == 0 else "alone"), parts
+    got, at = got.cpu().to(F64), 0
+    for slot, start, n in seqs:
+        want, size = plain.attend(cpu, slot, start, q[at:at + n], scale, window, sink, cap, keep)
+        off = (got[at:at + n] - want).abs()
+        assert torch.all(off <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size), (slot, float((off / size).max()))
+        at += n
+
+
+CUTS = [
+    # heads, kv heads, head size, sequences, positions at most, new tokens at most, the way that such a step goes
+    (4, 1, 128, 1, 8000, 1, "cluster"), (8, 2, 64, 2, 5000, 1, "cluster"), (16, 1, 128, 2, 6000, 1, "cluster"), (20, 1, 64, 1, 4096, 1, "cluster"),
+    (4, 1, 128, 2, 6000, 5, "cluster"), (32, 1, 128, 1, 3000, 2, "cluster"),
+    (8, 4, 128, 60, 1500, 1, "dealt"), (16, 4, 64, 100, 1500, 1, "dealt"), (16, 4, 128, 60, 1500, 2, "dealt"), (8, 4, 64, 100, 1500, 4, "dealt"),
+    (16, 4, 128, 60, 1500, 4, "dealt"), (16, 4, 64, 60, 1500, 4, "dealt"), (16, 4, 128, 60, 1500, 5, "dealt"), (16, 4, 64, 60, 1500, 6, "dealt"),
+    (16, 4, 128, 60, 1500, 8, "dealt"), (16, 4, 64, 60, 1500, 8, "dealt"), (16, 4, 128, 60, 1500, 16, "dealt"), (24, 1, 128, 200, 600, 1, "dealt"),
+    (8, 8, 128, 100, 180, 1, "alone"), (16, 8, 64, 100, 180, 5, "alone"), (24, 8, 128, 100, 120, 3, "alone"),
+]
+
+
+def a_step(B, most, new):
+    return [(B - 1 - i, (i * 97 * (1 + i % 5)) % (most + 1 - new) if i else most - new, 1 + (i + new - 1) % new) for i in range(B)]
+
+
+@pytest.mark.parametrize("H,Kh,D,B,most,new,cut", CUTS)
+def test_weights_and_scales_of_very_different_size(ops, H, Kh, D, B, most, new, cut):
+    """What counts in a sum is a weight times its values' scale: small weights of large values, and all of them where a sink holds most
+    of the weight, are kept as they are where weights and scales are near one another."""
+    view, cpu = uneven_view(B, Kh, D, -(-most // 64), seed=H + D + new)
+    seqs = a_step(B, most, new)
+    q = rows_of(seqs, H * D, seed=5).view(-1, H, D)
+    q[..., 0] = 5.0
+    attended_as_plain(ops, view, cpu, seqs, q, 0.2, cut=cut)
+    sink = torch.linspace(-3.0, 40.0, H)                     # (weights of 2^-58 x 2^-40 and some more: float32 numbers)
+    attended_as_plain(ops, view, cpu, seqs, q, 0.2, sink=sink, cut=cut)
+
+
+@pytest.mark.parametrize("H,Kh,D,B,most,new,cut", CUTS)
+def test_a_first_token_that_takes_the_weight_and_holds_nothing(ops, H, Kh, D, B, most, new, cut):
+    """Position 0 weighs e^14 times as much as others, and its values are zeros: the result is the others', each at 2^-20 of the largest weight
+    (e^14 = 2^20.2: rounded to float16 around a largest of 2^7 .. 2^15 that is 2^-13.2 or more, of steps of 2^-24: 2^-11.8 of a weight)."""
+    view, cpu = make_view(B * -(-most // 64), Kh, 64, D, B, -(-most // 64), seed=D + new)
+    g = torch.Generator().manual_seed(1)
+    codes = (torch.randn(view.k.shape, generator=g) * 4).to(torch.float8_e4m3fn)
+    codes[..., 0] = 0
+    codes = codes.view(torch.uint8)
+    for slot in range(B):
+        page = int(cpu.page_table[slot, 0])
+        codes[page, :, 0] = 0
+        codes[page, :, 0, 0] = int(torch.tensor(112.0).to(torch.float8_e4m3fn).view(torch.uint8))         # 14 / 0.125
+        for v in (view, cpu):
+            v.v.view(torch.uint8)[page, :, 0] = 0
+    for v in (view, cpu):
+        v.k.view(torch.uint8).copy_(codes)
+        v.scales[0].fill_(0.125)
+        v.scales[1].fill_(0.125)
+    seqs = [(s, max(p, 1), n) for s, p, n in a_step(B, most, new)]
+    q = rows_of(seqs, H * D, seed=6).view(-1, H, D) * 0.25
+    q[..., 0] = 5.0
+    attended_as_plain(ops, view, cpu, seqs, q, 0.2, cut=cut)
