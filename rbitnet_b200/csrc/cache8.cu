@@ -121,6 +121,28 @@ __device__ __noinline__ void exact_codes(uint8_t* to, const __nv_bfloat16* head,
   }
 }
 
+// The scale too is that of the exact rotation.  Both values of a pair are `amax` at most, so the exact largest value lies within 2 amax 0x1.8p-22
+// of it; where a border of scales, 448 * 2^e, lies in that range (of 500,000 blocks one), the pairs are turned in float64 and compared with it.
+// The border, or 0: float32 leaves no doubt (11 steps of amax's mantissa beside 1.75 are 0x1.8p-21 of it), or the old scale holds the
+// values either way.
+__device__ __forceinline__ float open_border(float amax, float old) {
+  if ((__float_as_uint(amax) - (0x600000u - 11) & 0x7fffffu) > 22) return 0.f;
+  const float lo = scale_for(amax * (1.f - 0x1.8p-21f)), hi = scale_for(amax * (1.f + 0x1.8p-21f));
+  return lo < hi && old < hi ? 448.f * lo : 0.f;
+}
+__device__ __forceinline__ float scale_at_border(float border, bool passed) { return scale_for(border) * (passed ? 2.f : 1.f); }
+// Whether one of eight pairs exceeds the border, the pairs in the pieces that begin at a0 and b0.
+__device__ __noinline__ bool pieces_pass(const __nv_bfloat16* head, const float* freq, int pos, float border, int a0, int b0, int interleaved) {
+  bool passed = false;
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    const int x = interleaved ? a0 + 2 * i : a0 + i, y = interleaved ? x + 1 : b0 + i;
+    const float2 v = exact_turned(__bfloat162float(head[x]), __bfloat162float(head[y]), freq[i], pos, 1.f);
+    passed |= fmaxf(fabsf(v.x), fabsf(v.y)) > border;        // (rounded to odd: above the border stays above it)
+  }
+  return passed;
+}
+
 struct Append8 {
   __nv_bfloat16* q_out;          // [T, H, D]
   const __nv_bfloat16* qkv;      // [T, (H + 2 Kh) D], rows qkv_stride apart (H D without writing)
@@ -189,7 +211,25 @@ __global__ void __launch_bounds__(256) append8_kernel(Append8 p) {
       amax = fmaxf(amax, fmaxf(fabsf(ya), fabsf(yb)));
     }
     amax = rb_block_max(amax, scratch);          // (its barriers also make the rows visible)
-    const float old = before > 0 ? *scale : 0.f, now = fmaxf(old, scale_for(amax)), inv = 1.0f / now;
+    const float old = before > 0 ? *scale : 0.f, border = stream == 0 && p.rot_dim > 0 ? open_border(amax, old) : 0.f;
+    float needed = scale_for(amax);
+    if (border > 0.f) {
+      bool passed = false;
+      for (int idx = threadIdx.x; idx < n * half; idx += blockDim.x) {
+        const int tok = idx / half, i = idx % half;
+        if (i >= rhalf) {
+          a = p.rot_dim + 2 * (i - rhalf);
+          passed |= fmaxf(fabsf(rows[tok * D + a]), fabsf(rows[tok * D + a + 1])) > border;
+          continue;
+        }
+        const __nv_bfloat16* head = p.qkv + (int64_t)(tok0 + tok) * p.qkv_stride + (int64_t)(p.H + kvh) * D;
+        const float x0 = __bfloat162float(head[p.interleaved ? 2 * i : i]), x1 = __bfloat162float(head[p.interleaved ? 2 * i + 1 : i + rhalf]);
+        const float2 v = exact_turned(x0, x1, p.inv_freq[i], pos0 + tok, 1.f);
+        passed |= fmaxf(fabsf(v.x), fabsf(v.y)) > border;
+      }
+      needed = scale_at_border(border, __syncthreads_or(passed) != 0);
+    }
+    const float now = fmaxf(old, needed), inv = 1.0f / now;
     if (old < now) {
       const float ratio = old * inv;
       for (int idx = threadIdx.x; idx < before * D; idx += blockDim.x) codes[idx] = to_code(of_code(codes[idx]) * ratio);
@@ -384,7 +424,21 @@ __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append
     float amax = tops[s][0];
 #pragma unroll
     for (int w = 1; w < THREADS / 32; ++w) amax = fmaxf(amax, tops[s][w]);
-    const float now = fmaxf(old[s], scale_for(amax)), inv = 1.0f / now;
+    float needed = scale_for(amax);
+    if (s == 0 && p.rot_dim) {
+      const float border = open_border(amax, old[0]);
+      if (border > 0.f) {
+        bool passed = false;
+#pragma unroll 1
+        for (int item = threadIdx.x; item < n * pieces; item += THREADS) {
+          const int t = item / pieces, x = item % pieces;
+          passed |= pieces_pass(rows + (int64_t)t * p.qkv_stride + (int64_t)(p.H + kvh) * D, p.inv_freq + 8 * x, pos0 + t, border, piece_a(p, x),
+                                piece_b(p, x), p.interleaved);
+        }
+        needed = scale_at_border(border, __syncthreads_or(passed) != 0);
+      }
+    }
+    const float now = fmaxf(old[s], needed), inv = 1.0f / now;
     uint8_t* codes = (uint8_t*)(s ? p.cache.v : p.cache.k) + at;
     if (old[s] < now) rescale16(codes, before * D, old[s] * inv, threadIdx.x, THREADS);
 #pragma unroll
@@ -457,7 +511,15 @@ __global__ void __launch_bounds__(256) append8_step_kernel(Append8 p) {
     if (base == 0 && p.write_kv) {
       const float big = largest8(a, b);
       const float top_k = rb_warp_max(is_k ? big : 0.f), top_v = rb_warp_max(is_v ? big : 0.f);
-      const float now_k = fmaxf(old_k, scale_for(top_k)), now_v = fmaxf(old_v, scale_for(top_v));
+      float needed = scale_for(top_k);
+      if (p.rot_dim) {
+        const float border = open_border(top_k, old_k);
+        if (border > 0.f) {
+          const bool passed = is_k && pieces_pass(src + head * D, p.inv_freq + 8 * e, pos, border, piece_a(p, e), piece_b(p, e), p.interleaved);
+          needed = scale_at_border(border, __any_sync(0xffffffffu, passed));
+        }
+      }
+      const float now_k = fmaxf(old_k, needed), now_v = fmaxf(old_v, scale_for(top_v));
       uint8_t* k = (uint8_t*)p.cache.k + at;
       uint8_t* v = (uint8_t*)p.cache.v + at;
       if (old_k < now_k) rescale16(k, before * D, old_k / now_k, lane, 32);

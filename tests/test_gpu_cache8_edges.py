@@ -6,7 +6,7 @@ import torch
 
 import plain_cache8 as plain
 from rbitnet_b200.cache import CacheLayerView
-from test_gpu_cache8 import BF16, F64, make_meta, make_view, rows_of
+from test_gpu_cache8 import BF16, F64, both_views, frequencies, make_meta, make_view, rows_of, same_codes
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +120,54 @@ def test_a_first_token_that_takes_the_weight_and_holds_nothing(ops, H, Kh, D, B,
     q = rows_of(seqs, H * D, seed=6).view(-1, H, D) * 0.25
     q[..., 0] = 5.0
     attended_as_plain(ops, view, cpu, seqs, q, 0.2, cut=cut)
+
+
+def pairs_at_a_border(freq, positions, count):
+    """(position, x0, x1): bfloat16 pairs whose turn by position * freq has its larger value within 2^-23.5 of itself of 448 * 2^-8 and not
+    within 2^-36 (what float64 may be off), and the other below nine tenths of it."""
+    border, found = 448.0 * 2.0 ** -8, []
+    x0 = (torch.arange(128, 256).to(F64)[None] * torch.exp2(torch.arange(-11.0, -5.0).to(F64))[:, None]).view(-1)
+    x0 = torch.cat([x0, -x0])
+    for pos in positions:
+        angle = torch.tensor(float(pos), dtype=F64) * float(freq)
+        c, s = float(angle.cos()), float(angle.sin())
+        if min(abs(c), abs(s)) < 0.05:
+            continue
+        for sign in (1.0, -1.0):
+            x1 = ((x0 * c - sign * border) / s).to(BF16).to(F64)
+            y, other = x0 * c - x1 * s, x0 * s + x1 * c
+            off = (y.abs() / border - 1).abs()
+            for i in ((off < 2.0 ** -23.5) & (off > 2.0 ** -36) & (other.abs() < 0.9 * border)).nonzero()[:, 0].tolist():
+                found.append((pos, float(x0[i]), float(x1[i])))
+        if len(found) >= count:
+            break
+    return found[:count]
+
+
+@pytest.mark.parametrize("D,rot,inter,new", [(128, 128, False, 1), (64, 64, True, 1), (128, 128, True, 2), (64, 64, False, 2), (256, 256, False, 2),
+                                             (128, 32, False, 1), (10, 10, True, 2)])
+def test_the_scale_of_keys_is_that_of_the_exact_rotation(ops, D, rot, inter, new):
+    """Keys whose largest value lies nearer to a border of scales than float32 sines are exact, on either side of it."""
+    Kh, B = 2, 96
+    freq = frequencies(rot)
+    which = rot // 2 - 1 if rot < 16 else 3                    # the pair that turns
+    at = (2 * which, 2 * which + 1) if inter else (which, which + rot // 2)
+    found = pairs_at_a_border(float(freq[which]), (p for p in range(1, 400000, 3) if p % 64), B)
+    assert len(found) == B
+    page, codes = 64, torch.zeros(B, Kh, 64, D).to(torch.float8_e4m3fn)
+    scales = torch.full((B, Kh, 1), 2.0 ** -60)
+    table = torch.arange(B, dtype=torch.int32)[:, None].expand(B, 1 + max(p for p, _, _ in found) // page).contiguous()
+    view, cpu = both_views([codes, codes], [scales, scales], table, page)
+    seqs = [(i, p + 1 - new, new) for i, (p, _, _) in enumerate(found)]
+    x = torch.zeros(B, new, 3 * Kh, D)
+    for i, (_, a, b) in enumerate(found):
+        x[i, -1, Kh, at[0]], x[i, -1, Kh, at[1]] = a, b        # (and the other kv head's the other way)
+        x[i, -1, Kh + 1, at[0]], x[i, -1, Kh + 1, at[1]] = -a, -b
+    x = x.to(BF16).view(B * new, 3 * Kh * D)
+    ops.rotate_append(x.cuda(), (freq.cuda(), inter, rot), make_meta(seqs), view, Kh)
+    rows = x.to(F64).view(B, new, 3 * Kh, D)
+    for i, start, _ in seqs:
+        t = plain.turned(rows[i][:, Kh:2 * Kh], torch.arange(start, start + new), freq, rot, inter)
+        plain.append(cpu, i, start, t, rows[i][:, 2 * Kh:])
+    assert set(cpu.scales[0].view(-1).tolist()) == {2.0 ** -8, 2.0 ** -7}
+    assert torch.equal(view.scales[0].cpu(), cpu.scales[0]) and same_codes(view.k, cpu.k)
