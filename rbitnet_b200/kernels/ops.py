@@ -797,6 +797,8 @@ class CudaOps:
             raise KernelError(f"attention: {T} rows of {H} heads of {D} values, expected {meta.n_tokens} of {n_heads} on {Kh} kv heads of "
                               f"{view.head_dim}")
         keep = int(keep_first or 0) if win else 0
+        if T == 0:
+            return q.new_empty((T, H * D))
         # how a step's rows are cut is the same for all of its layers of these sizes
         key = ("attention8", H, Kh, D, view.page_size, win, keep, self.cache8_rows)
         cut = meta.extra.get(key)
@@ -808,8 +810,6 @@ class CudaOps:
         if not in_rows and not meta.single_token:
             return self._attention_unpacked(q, meta, view, n_heads, scale, window, sinks, softcap, keep)
         out = q.new_empty((T, H * D))
-        if T == 0:
-            return out
         if sinks is not None or softcap > 0.0 or keep > 0:
             if sinks is not None:
                 self._check(sinks, torch.float32, "attention sinks")
@@ -828,7 +828,7 @@ class CudaOps:
     def _cut_rows8(self, meta, view, T: int, H: int, Kh: int, D: int, win: int, keep: int):
         """(whether the kernel of few rows takes them, its row tiles, its parts and scratch: csrc/attention8_rows.cuh)."""
         G, most_new = H // Kh, 1 if meta.single_token else max((c.n_new for c in meta.seqs), default=1)
-        if not self.lib.raw("rb_attention8_rows_supports")(H, Kh, D, view.page_size) or T == 0 or \
+        if not self.lib.raw("rb_attention8_rows_supports")(H, Kh, D, view.page_size) or \
                 (not meta.single_token and most_new * G > self.cache8_rows):
             return (False,) + (None,) * 8
         tok0 = ntok = None
@@ -850,21 +850,22 @@ class CudaOps:
         key = ("unpacked", view.page_size, view.max_pages, view.page_table.shape[0], window, keep)
         if key not in meta.extra:
             P, ranges = view.page_size, []
-            for c in meta.seqs:
+            seqs = [c for c in meta.seqs if c.n_new > 0]
+            for c in seqs:
                 first = 0 if not window or keep else max(0, c.start - int(window) + 1)
                 ranges.append((c.slot, first, c.start + c.n_new))
             plan = self.cache_ranges(view, ranges)
             width = max(-(-end // P) for _, _, end in ranges)
             table = np.zeros((len(ranges), width), dtype=np.int32)
             slots = np.zeros(meta.n_tokens, dtype=np.int32)
-            for i, ((_, first, end), at, c) in enumerate(zip(ranges, plan.first_item, meta.seqs)):
+            for i, ((_, first, end), at, c) in enumerate(zip(ranges, plan.first_item, seqs)):
                 table[i, :] = at                       # (places that no row sees: any of the sequence's pages)
                 n = -(-end // P) - first // P
                 table[i, first // P:first // P + n] = np.arange(at, at + n)
                 slots[c.offset:c.offset + c.n_new] = i
             both = upload(np.concatenate([table.reshape(-1), slots]), self.device)
             step = replace(meta, tok_slot=both[table.size:], extra={},
-                           seqs=[replace(c, slot=i) for i, c in enumerate(meta.seqs)])
+                           seqs=[replace(c, slot=i) for i, c in enumerate(seqs)])
             meta.extra[key] = (plan, both[:table.size].view(table.shape), step)
         plan, table, step = meta.extra[key]
         k, v = self.cache_values(view, plan)

@@ -4,6 +4,7 @@ from dataclasses import replace
 import pytest
 import torch
 
+from rbitnet_b200.engine.step import SeqChunk, build_meta
 from rbitnet_b200.kernels.ops import CudaOps
 from test_cpu_cache8 import _NoLibrary, bare_ops, meta_of, view_of
 
@@ -39,3 +40,25 @@ def test_queries_that_begin_between_16_bytes_are_copied(monkeypatch, kind, token
         at = args[1] if isinstance(args[1], int) else args[1].value or 0
         assert at % 16 == 0, (name, off)
         assert (at == q.data_ptr()) == (q.data_ptr() % 16 == 0)
+
+
+@pytest.mark.parametrize("seqs", [[(0, 0, 0), (1, 0, 100)], [(0, 3, 0), (1, 60, 40)], [(1, 5, 90), (0, 128, 0)], [(0, 0, 0)], []])
+def test_a_step_may_hold_sequences_without_tokens(monkeypatch, seqs):
+    """They bring no rows and no pages; a step of them alone launches nothing."""
+    import numpy as np
+    ops, H, D, at, chunks = bare_ops(), 64, 128, 0, []
+    ops.lib, ops.prefill_on_tcgen05, ops.decode_on_tma = _Recorder(), True, True
+    for name in ("_stream", "_raw_stream"):
+        monkeypatch.setattr(CudaOps, name, lambda self: 0)
+    monkeypatch.setattr(CudaOps, "_check", lambda self, t, dtype, what: None)
+    monkeypatch.setattr(CudaOps, "_check_cache8", lambda self, view, what: 64)
+    for slot, start, n in seqs:
+        chunks.append(SeqChunk(slot, start, n, at))
+        at += n
+    meta = build_meta(chunks, np.zeros(at, dtype=np.int32), np.zeros(0, dtype=np.int32), "cpu")
+    out = ops.attention(torch.zeros(at, H, D, dtype=torch.bfloat16), meta, view_of(), H, 1.0, None)
+    assert out.shape == (at, H * D) and bool(ops.lib.calls) == (at > 0)
+    if at:
+        plan, table, step = next(v for k, v in meta.extra.items() if k[0] == "unpacked")
+        assert [c.n_new for c in step.seqs] == [n for _, _, n in seqs if n] and table.shape[0] == 1
+        assert plan.count == 2 and set(step.tok_slot.tolist()) == {0}

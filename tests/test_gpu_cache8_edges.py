@@ -171,3 +171,21 @@ def test_the_scale_of_keys_is_that_of_the_exact_rotation(ops, D, rot, inter, new
         plain.append(cpu, i, start, t, rows[i][:, 2 * Kh:])
     assert set(cpu.scales[0].view(-1).tolist()) == {2.0 ** -8, 2.0 ** -7}
     assert torch.equal(view.scales[0].cpu(), cpu.scales[0]) and same_codes(view.k, cpu.k)
+
+
+@pytest.mark.parametrize("new", [1, 4, 100])
+def test_sequences_without_tokens_in_a_step(ops, new):
+    """They change nothing for the others: a few rows, and many."""
+    H, Kh, D = 8, 2, 128
+    rotary = (frequencies(D).cuda(), False, D)
+    x = rows_of([(0, 0, 2 * new)], (H + 2 * Kh) * D, seed=2).cuda()
+    results = []
+    for seqs in ([(0, 60, new), (2, 3, new)], [(1, 0, 0), (0, 60, new), (3, 64, 0), (2, 3, new)]):
+        view, _ = make_view(12, Kh, 64, D, 4, 3, seed=4)
+        meta = make_meta(seqs)
+        q = ops.rotate_append(x, rotary, meta, view, H)
+        results.append((q, ops.attention(q, meta, view, H, 0.1, None), view.k.view(torch.uint8), view.v.view(torch.uint8), *view.scales))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    meta = make_meta([(1, 0, 0), (0, 70, 0)])
+    q = ops.rotate_append(x[:0], rotary, meta, view, H)
+    assert ops.attention(q, meta, view, H, 0.1, None).shape == (0, H * D)
