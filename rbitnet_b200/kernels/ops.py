@@ -637,10 +637,11 @@ class CudaOps:
         out = torch.empty((T, H * D), dtype=self.dtype, device=self.device)
         win = int(window or 0)
         keep = int(keep_first or 0) if win else 0
-        if sinks is not None or softcap > 0.0 or keep > 0:
-            if sinks is not None:
-                self._check(sinks, torch.float32, "attention sinks")
-            self.lib.call("rb_attention_next", _ptr(sinks), float(softcap), keep, launches=0)
+
+        def launch(name, *args, launches=1):
+            self._attention_options(sinks, softcap, keep)
+            self.lib.call(name, *args, launches=launches)
+
         # the most keys a new token can have to visit, in whole tiles
         context = int(meta.max_context) if not win else min(int(meta.max_context), win + 126 + (keep + 63) // 64 * 64)
         # keys and values that are the same rows (attention through latents) let the tcgen05 kernel take wider heads
@@ -663,16 +664,16 @@ class CudaOps:
                 part_ml = torch.empty((T, H, n_splits, 2), dtype=torch.float32, device=self.device)
             if on_tma:
                 # keys and values by TMA (head sizes 64 and 128)
-                self.lib.call("rb_attention_decode_tma", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v),
-                              view.k.shape[0], _ptr(view.page_table), view.max_pages, view.page_size,
-                              _ptr(meta.tok_pos), _ptr(meta.tok_slot), T, H, Kh, D, float(scale), win,
-                              _ptr(part_o), _ptr(part_ml), n_splits, self._stream(),
-                              launches=2 if n_splits > 1 and not on_chip else 1)
+                launch("rb_attention_decode_tma", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v),
+                       view.k.shape[0], _ptr(view.page_table), view.max_pages, view.page_size,
+                       _ptr(meta.tok_pos), _ptr(meta.tok_slot), T, H, Kh, D, float(scale), win,
+                       _ptr(part_o), _ptr(part_ml), n_splits, self._stream(),
+                       launches=2 if n_splits > 1 and not on_chip else 1)
             else:
-                self.lib.call("rb_attention_decode", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v),
-                              _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos),
-                              _ptr(meta.tok_slot), T, H, Kh, D, float(scale), win, _ptr(part_o), _ptr(part_ml),
-                              n_splits, self._stream(), launches=2 if n_splits > 1 else 1)
+                launch("rb_attention_decode", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v),
+                       _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos),
+                       _ptr(meta.tok_slot), T, H, Kh, D, float(scale), win, _ptr(part_o), _ptr(part_ml),
+                       n_splits, self._stream(), launches=2 if n_splits > 1 else 1)
         elif on_tc:
             tok0, ntok, n_tiles = self._prefill_tiles(meta, 128 // (H // Kh))
             parts, part_o, part_ml = 1, None, None
@@ -682,22 +683,29 @@ class CudaOps:
             if parts > 1:
                 part_o = torch.empty((T, H, parts, D), dtype=torch.float32, device=self.device)
                 part_ml = torch.empty((T, H, parts, 2), dtype=torch.float32, device=self.device)
-            self.lib.call("rb_attention_prefill_tc", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v),
-                          view.k.shape[0], _ptr(view.page_table), view.max_pages, view.page_size,
-                          _ptr(meta.tok_pos), _ptr(meta.tok_slot), _ptr(tok0), _ptr(ntok), n_tiles, H, Kh, D,
-                          float(scale), win, _ptr(part_o), _ptr(part_ml), parts, T, self._stream(), launches=2 if parts > 1 else 1)
+            launch("rb_attention_prefill_tc", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v),
+                   view.k.shape[0], _ptr(view.page_table), view.max_pages, view.page_size,
+                   _ptr(meta.tok_pos), _ptr(meta.tok_slot), _ptr(tok0), _ptr(ntok), n_tiles, H, Kh, D,
+                   float(scale), win, _ptr(part_o), _ptr(part_ml), parts, T, self._stream(), launches=2 if parts > 1 else 1)
         elif self.dtype == torch.bfloat16 and \
                 self.lib.raw("rb_attention_tiled_supports")(H, Kh, D, view.page_size, 0):
             tok0, ntok, n_tiles = self._prefill_tiles(meta, 64 // (H // Kh))
-            self.lib.call("rb_attention_prefill", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v),
-                          _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos),
-                          _ptr(meta.tok_slot), _ptr(tok0), _ptr(ntok), n_tiles, H, Kh, D, float(scale), win,
-                          self._stream())
+            launch("rb_attention_prefill", _ptr(out), _ptr(q), _ptr(view.k), _ptr(view.v),
+                   _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos),
+                   _ptr(meta.tok_slot), _ptr(tok0), _ptr(ntok), n_tiles, H, Kh, D, float(scale), win,
+                   self._stream())
         else:
-            self.lib.call("rb_attention_simple", _ptr(out), _ptr(q), self.code, _ptr(view.k), _ptr(view.v),
-                          _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos),
-                          _ptr(meta.tok_slot), T, H, Kh, D, float(scale), win, self._stream())
+            launch("rb_attention_simple", _ptr(out), _ptr(q), self.code, _ptr(view.k), _ptr(view.v),
+                   _ptr(view.page_table), view.max_pages, view.page_size, _ptr(meta.tok_pos),
+                   _ptr(meta.tok_slot), T, H, Kh, D, float(scale), win, self._stream())
         return out
+
+    def _attention_options(self, sinks, softcap: float, keep: int) -> None:
+        """Of the next attention launch, whichever it is: nothing that may fail comes in between."""
+        if sinks is not None or softcap > 0.0 or keep > 0:
+            if sinks is not None:
+                self._check(sinks, torch.float32, "attention sinks")
+            self.lib.call("rb_attention_next", _ptr(sinks), float(softcap), keep, launches=0)
 
     # ------------------------------------------------------------------ the cache held in 8 bits
     def _check_cache8(self, view, what: str) -> int:
@@ -810,15 +818,12 @@ class CudaOps:
         if not in_rows and not meta.single_token:
             return self._attention_unpacked(q, meta, view, n_heads, scale, window, sinks, softcap, keep)
         out = q.new_empty((T, H * D))
-        if sinks is not None or softcap > 0.0 or keep > 0:
-            if sinks is not None:
-                self._check(sinks, torch.float32, "attention sinks")
-            self.lib.call("rb_attention_next", _ptr(sinks), float(softcap), keep, launches=0)
+        scratch = None if parts or not in_rows else torch.empty((n_o + n_ml,), dtype=torch.float32, device=q.device)
+        self._attention_options(sinks, softcap, keep)
         if not in_rows:
             self.lib.call("rb_attention8_simple", out.data_ptr(), at_q, *cache, view.max_pages, view.page_size, meta.tok_pos.data_ptr(),
                           meta.tok_slot.data_ptr(), T, H, Kh, D, float(scale), win, self._raw_stream())
             return out
-        scratch = None if parts else torch.empty((n_o + n_ml,), dtype=torch.float32, device=q.device)
         part = _address(scratch)
         self.lib.call("rb_attention8_rows", out.data_ptr(), at_q, *cache[:4], view.k.shape[0], cache[4], view.max_pages, view.page_size,
                       meta.tok_pos.data_ptr(), meta.tok_slot.data_ptr(), _address(tok0), _address(ntok), n_tiles, rows, H, Kh, D,

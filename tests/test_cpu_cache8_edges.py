@@ -62,3 +62,37 @@ def test_a_step_may_hold_sequences_without_tokens(monkeypatch, seqs):
         plan, table, step = next(v for k, v in meta.extra.items() if k[0] == "unpacked")
         assert [c.n_new for c in step.seqs] == [n for _, _, n in seqs if n] and table.shape[0] == 1
         assert plan.count == 2 and set(step.tok_slot.tolist()) == {0}
+
+
+@pytest.mark.parametrize("kind", ["16 bits", "8 bits"])
+@pytest.mark.parametrize("tokens", [1, 3, 100])
+def test_options_are_not_left_behind_where_a_call_fails(monkeypatch, kind, tokens):
+    """A sink, a cap and first keys are set for the launch that follows: whatever fails before it, they are not."""
+    ops, H, D = bare_ops(), 8, 128
+    ops.prefill_on_tcgen05, ops.decode_on_tma = True, True
+    for name in ("_stream", "_raw_stream"):
+        monkeypatch.setattr(CudaOps, name, lambda self: 0)
+    monkeypatch.setattr(CudaOps, "_check", lambda self, t, dtype, what: None)
+    monkeypatch.setattr(CudaOps, "_check_cache8", lambda self, view, what: 64)
+    view = view_of()
+    if kind == "16 bits":
+        view = replace(view, k=view.k.to(torch.bfloat16), v=view.v.to(torch.bfloat16), scales=())
+    real, fails = torch.empty, [0]
+
+    def empty(*a, **kw):                         # the nth tensor cannot be had
+        fails[0] -= 1
+        if fails[0] < 0:
+            raise torch.OutOfMemoryError("none left")
+        return real(*a, **kw)
+    monkeypatch.setattr(torch, "empty", empty)
+    for n in range(5):
+        ops.lib, fails[0] = _Recorder(), n
+        ops.lib.raw = lambda name: lambda *a: 0 if name.endswith("_on_chip") else 2
+        try:
+            ops.attention(torch.zeros(tokens, H, D, dtype=torch.bfloat16), meta_of(tokens), view, H, 1.0, None, sinks=torch.zeros(H), softcap=3.0)
+        except torch.OutOfMemoryError:
+            pass
+        names = [name for name, _ in ops.lib.calls]
+        for i, name in enumerate(names):
+            assert name != "rb_attention_next" or names[i + 1:][:1] and names[i + 1].startswith("rb_attention"), names
+    assert "rb_attention_next" in names
