@@ -639,7 +639,7 @@ class CudaOps:
         keep = int(keep_first or 0) if win else 0
 
         def launch(name, *args, launches=1):
-            self._attention_options(sinks, softcap, keep)
+            self._attention_options(H, sinks, softcap, keep)
             self.lib.call(name, *args, launches=launches)
 
         # the most keys a new token can have to visit, in whole tiles
@@ -700,11 +700,13 @@ class CudaOps:
                    _ptr(meta.tok_slot), T, H, Kh, D, float(scale), win, self._stream())
         return out
 
-    def _attention_options(self, sinks, softcap: float, keep: int) -> None:
+    def _attention_options(self, H: int, sinks, softcap: float, keep: int) -> None:
         """Of the next attention launch, whichever it is: nothing that may fail comes in between."""
         if sinks is not None or softcap > 0.0 or keep > 0:
             if sinks is not None:
                 self._check(sinks, torch.float32, "attention sinks")
+                if sinks.shape != (H,):
+                    raise KernelError(f"attention sinks: expected one for each of {H} heads, found {tuple(sinks.shape)}")
             self.lib.call("rb_attention_next", _ptr(sinks), float(softcap), keep, launches=0)
 
     # ------------------------------------------------------------------ the cache held in 8 bits
@@ -819,7 +821,7 @@ class CudaOps:
             return self._attention_unpacked(q, meta, view, n_heads, scale, window, sinks, softcap, keep)
         out = q.new_empty((T, H * D))
         scratch = None if parts or not in_rows else torch.empty((n_o + n_ml,), dtype=torch.float32, device=q.device)
-        self._attention_options(sinks, softcap, keep)
+        self._attention_options(H, sinks, softcap, keep)
         if not in_rows:
             self.lib.call("rb_attention8_simple", out.data_ptr(), at_q, *cache, view.max_pages, view.page_size, meta.tok_pos.data_ptr(),
                           meta.tok_slot.data_ptr(), T, H, Kh, D, float(scale), win, self._raw_stream())

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from rbitnet_b200.engine.step import SeqChunk, build_meta
+from rbitnet_b200.kernels.lib import KernelError
 from rbitnet_b200.kernels.ops import CudaOps
 from test_cpu_cache8 import _NoLibrary, bare_ops, meta_of, view_of
 
@@ -96,3 +97,23 @@ def test_options_are_not_left_behind_where_a_call_fails(monkeypatch, kind, token
         for i, name in enumerate(names):
             assert name != "rb_attention_next" or names[i + 1:][:1] and names[i + 1].startswith("rb_attention"), names
     assert "rb_attention_next" in names
+
+
+@pytest.mark.parametrize("kind", ["16 bits", "8 bits"])
+@pytest.mark.parametrize("tokens", [1, 3, 100])
+def test_sinks_of_other_heads_are_refused(monkeypatch, kind, tokens):
+    """(A kernel reads one for every head of the queries.)"""
+    ops, H, D = bare_ops(), 8, 128
+    ops.lib, ops.prefill_on_tcgen05, ops.decode_on_tma = _Recorder(), True, True
+    for name in ("_stream", "_raw_stream"):
+        monkeypatch.setattr(CudaOps, name, lambda self: 0)
+    monkeypatch.setattr(CudaOps, "_check", lambda self, t, dtype, what: None)
+    monkeypatch.setattr(CudaOps, "_check_cache8", lambda self, view, what: 64)
+    view = view_of()
+    if kind == "16 bits":
+        view = replace(view, k=view.k.to(torch.bfloat16), v=view.v.to(torch.bfloat16), scales=())
+    for shape in ((H - 1,), (H + 1,), (2, H), ()):
+        with pytest.raises(KernelError, match="sinks"):
+            ops.attention(torch.zeros(tokens, H, D, dtype=torch.bfloat16), meta_of(tokens), view, H, 1.0, None, sinks=torch.zeros(shape))
+        assert "rb_attention_next" not in [name for name, _ in ops.lib.calls]
+    ops.attention(torch.zeros(tokens, H, D, dtype=torch.bfloat16), meta_of(tokens), view, H, 1.0, None, sinks=torch.zeros(H))
