@@ -762,6 +762,10 @@ class CudaOps:
         if qkv.dtype != self.dtype or not qkv.is_cuda or qkv.stride(1) != 1:
             raise KernelError(f"rotate_append: expected {self.dtype} CUDA rows, found {qkv.dtype} on {qkv.device}")
         inv_freq, interleaved, rot_dim = (self._zeros_freq(D), False, 0) if rotary is None else rotary
+        if inv_freq.dtype is not torch.float32 or inv_freq.device != qkv.device or 2 * inv_freq.numel() < rot_dim or \
+                not inv_freq.is_contiguous():
+            raise KernelError(f"rotate_append: expected {rot_dim // 2} contiguous float32 frequencies on {qkv.device}, found {inv_freq.dtype} "
+                              f"{tuple(inv_freq.shape)} on {inv_freq.device}")
         tok0, ntok, n_tiles, most = self._block_tiles(meta, block)
         q = qkv.new_empty((T, n_heads, D))
         self.lib.call("rb_append8", q.data_ptr(), qkv.data_ptr(), qkv.stride(0), inv_freq.data_ptr(), meta.tok_pos.data_ptr(),

@@ -117,3 +117,22 @@ def test_sinks_of_other_heads_are_refused(monkeypatch, kind, tokens):
             ops.attention(torch.zeros(tokens, H, D, dtype=torch.bfloat16), meta_of(tokens), view, H, 1.0, None, sinks=torch.zeros(shape))
         assert "rb_attention_next" not in [name for name, _ in ops.lib.calls]
     ops.attention(torch.zeros(tokens, H, D, dtype=torch.bfloat16), meta_of(tokens), view, H, 1.0, None, sinks=torch.zeros(H))
+
+
+def test_frequencies_that_are_too_few_or_elsewhere_are_refused(monkeypatch):
+    """(A kernel reads one for every pair that it turns.)"""
+    ops, H, D = bare_ops(), 4, 128
+    ops.lib = _Recorder()
+    monkeypatch.setattr(CudaOps, "_raw_stream", lambda self: 0)
+    monkeypatch.setattr(CudaOps, "_check_cache8", lambda self, view, what: 64)
+    rows = torch.zeros(3, (H + 4) * D, dtype=torch.bfloat16)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    good = torch.zeros(64)
+    for bad in (good[:63], good.double(), torch.zeros(128)[::2], good.to("meta")):
+        with pytest.raises(KernelError, match="frequencies"):
+            ops.rotate_append(rows, (bad, False, D), meta_of(3), view_of(), H)
+    assert ops.lib.calls == []
+    for fine in ((good, False, D), (good[:32], True, 64), None):
+        ops._zf = good
+        ops.rotate_append(rows, fine, meta_of(3), view_of(), H)
+    assert [name for name, _ in ops.lib.calls] == ["rb_append8"] * 3
