@@ -759,7 +759,7 @@ class CudaOps:
         want = (n_heads + (2 * Kh if view.writes else 0)) * D
         if width != want or T != meta.n_tokens:
             raise KernelError(f"rotate_append: {T} rows of {width} values, expected {meta.n_tokens} of {want}")
-        if qkv.dtype != self.dtype or not qkv.is_cuda or qkv.stride(1) != 1:
+        if qkv.dtype != self.dtype or not qkv.is_cuda or qkv.device != view.k.device or qkv.stride(1) != 1:
             raise KernelError(f"rotate_append: expected {self.dtype} CUDA rows, found {qkv.dtype} on {qkv.device}")
         inv_freq, interleaved, rot_dim = (self._zeros_freq(D), False, 0) if rotary is None else rotary
         if inv_freq.dtype is not torch.float32 or inv_freq.device != qkv.device or 2 * inv_freq.numel() < rot_dim or \
@@ -807,9 +807,9 @@ class CudaOps:
         Kh, win = view.n_kv_heads, int(window or 0)
         self._check_cache8(view, "attention")
         self._check(q, self.dtype, "attention queries")
-        if D != view.head_dim or H != n_heads or H % Kh or T != meta.n_tokens:
-            raise KernelError(f"attention: {T} rows of {H} heads of {D} values, expected {meta.n_tokens} of {n_heads} on {Kh} kv heads of "
-                              f"{view.head_dim}")
+        if D != view.head_dim or H != n_heads or H % Kh or T != meta.n_tokens or q.device != view.k.device:
+            raise KernelError(f"attention: {T} rows of {H} heads of {D} values on {q.device}, expected {meta.n_tokens} of {n_heads} on {Kh} "
+                              f"kv heads of {view.head_dim} on {view.k.device}")
         keep = int(keep_first or 0) if win else 0
         if T == 0:
             return q.new_empty((T, H * D))
@@ -1845,15 +1845,15 @@ class CudaOps:
         not accept, or the last one, a token is taken from max(p - q, 0) (the last row: p) with uniforms[r, 1].
         Returns (accepted int32 [B], tokens int32 [B, most + 1]: the accepted drafts, the token taken, then -1)."""
         for t, dtype, what in ((logits, torch.float32, "logits"), (draft_probs, torch.float32, "draft probabilities")):
-            if t is not None and (t.dtype != dtype or not t.is_cuda or t.dim() != 2 or t.stride(1) != 1):
+            if t is not None and (t.dtype != dtype or not t.is_cuda or t.device != logits.device or t.dim() != 2 or t.stride(1) != 1):
                 raise KernelError(f"verify_drafts {what}: expected float32 CUDA rows, found {t.dtype} {tuple(t.shape)} on {t.device}")
         R, V = logits.shape
         B = first_row.shape[0] - 1
         for t, dtype, shape, what in ((first_row, torch.int32, (B + 1,), "first rows"), (drafts, torch.int32, (R,), "drafts"),
                                       (temperature, torch.float32, (B,), "temperatures"), (uniforms, torch.float32, (R, 2), "uniform numbers")):
             self._check(t, dtype, f"verify_drafts {what}")
-            if tuple(t.shape) != shape:
-                raise KernelError(f"verify_drafts {what}: expected {shape}, found {tuple(t.shape)}")
+            if tuple(t.shape) != shape or t.device != logits.device:
+                raise KernelError(f"verify_drafts {what}: expected {shape} on {logits.device}, found {tuple(t.shape)} on {t.device}")
         if draft_probs is not None and tuple(draft_probs.shape) != (R, V):
             raise KernelError(f"verify_drafts draft probabilities: expected {(R, V)}, found {tuple(draft_probs.shape)}")
         if B < 0 or most < 0 or V < 1:

@@ -136,3 +136,27 @@ def test_frequencies_that_are_too_few_or_elsewhere_are_refused(monkeypatch):
         ops._zf = good
         ops.rotate_append(rows, fine, meta_of(3), view_of(), H)
     assert [name for name, _ in ops.lib.calls] == ["rb_append8"] * 3
+
+
+def test_tensors_on_different_devices_are_refused(monkeypatch):
+    ops, H, D = bare_ops(), 8, 128
+    ops.lib = _Recorder()
+    for name in ("_stream", "_raw_stream"):
+        monkeypatch.setattr(CudaOps, name, lambda self: 0)
+    monkeypatch.setattr(CudaOps, "_check_cache8", lambda self, view, what: 64)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    view = view_of()
+    with pytest.raises(KernelError, match="meta"):
+        ops.attention(torch.zeros(3, H, D, dtype=torch.bfloat16, device="meta"), meta_of(3), view, H, 1.0, None)
+    with pytest.raises(KernelError, match="meta"):
+        ops.rotate_append(torch.zeros(3, (H + 4) * D, dtype=torch.bfloat16, device="meta"), None, meta_of(3), view, H)
+    args = [torch.zeros(3, 10), torch.tensor([0, 2, 3], dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(2), torch.zeros(3, 2)]
+    for i in range(len(args)):
+        with pytest.raises(KernelError, match="meta"):
+            ops.verify_drafts(*[t.to("meta") if j == i else t for j, t in enumerate(args)], 1)
+    with pytest.raises(KernelError, match="meta"):
+        ops.verify_drafts(*args, 1, draft_probs=torch.zeros(3, 10, device="meta"))
+    assert ops.lib.calls == []
+    ops.lib.raw = lambda name: lambda *a: 64
+    ops.verify_drafts(*args, 1)
+    assert [name for name, _ in ops.lib.calls] == ["rb_verify"]
