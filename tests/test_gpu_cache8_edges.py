@@ -189,3 +189,85 @@ def test_sequences_without_tokens_in_a_step(ops, new):
     meta = make_meta([(1, 0, 0), (0, 70, 0)])
     q = ops.rotate_append(x[:0], rotary, meta, view, H)
     assert ops.attention(q, meta, view, H, 0.1, None).shape == (0, H * D)
+
+
+# ---- every way that a step is cut, with everything that a row may be asked for: eights of rows 1 to 4, both head sizes
+OPTIONS = [
+    # heads, kv heads, head size, sequences, positions at most, new tokens at most, window, sinks, cap, first keys that stay, the way it goes
+    (16, 4, 128, 60, 1500, 2, 0, True, 0.0, 0, "dealt"), (16, 4, 128, 60, 1500, 4, 700, False, 0.0, 100, "dealt"),
+    (16, 4, 128, 60, 1500, 5, 0, True, 15.0, 0, "dealt"), (16, 4, 128, 60, 1500, 6, 650, True, 0.0, 0, "dealt"),
+    (16, 4, 128, 60, 1500, 8, 900, True, 20.0, 70, "dealt"), (16, 4, 128, 60, 1500, 16, 0, False, 0.0, 0, "dealt"),
+    (16, 4, 64, 60, 1500, 4, 0, True, 0.0, 0, "dealt"), (16, 4, 64, 60, 1500, 6, 700, False, 10.0, 3, "dealt"),
+    (16, 4, 64, 60, 1500, 8, 800, True, 0.0, 65, "dealt"), (24, 1, 128, 200, 600, 1, 300, True, 0.0, 64, "dealt"),
+    (28, 1, 64, 250, 600, 2, 0, True, 5.0, 0, "dealt"), (8, 4, 128, 60, 1500, 1, 900, True, 12.0, 100, "dealt"),
+    (16, 2, 128, 3, 5000, 2, 0, True, 0.0, 0, "cluster"), (16, 2, 64, 3, 5000, 3, 3000, True, 9.0, 100, "cluster"),
+    (16, 2, 128, 3, 5000, 4, 2500, False, 0.0, 10, "cluster"), (8, 2, 128, 3, 4000, 1, 2000, True, 0.0, 100, "cluster"),
+    (16, 8, 128, 100, 180, 3, 100, True, 8.0, 5, "alone"), (16, 8, 64, 100, 180, 8, 70, True, 0.0, 66, "alone"),
+]
+
+
+@pytest.mark.parametrize("H,Kh,D,B,most,new,window,sinks,cap,keep,cut", OPTIONS)
+def test_options_however_a_step_is_cut(ops, H, Kh, D, B, most, new, window, sinks, cap, keep, cut):
+    tiles = -(-most // 64)
+    view, cpu = make_view(B * tiles, Kh, 64, D, B, tiles, seed=H + D + new)
+    seqs = a_step(B, most, new)
+    q = rows_of(seqs, H * D, seed=8).view(-1, H, D)
+    attended_as_plain(ops, view, cpu, seqs, q, D ** -0.5, window, torch.linspace(-2.0, 3.0, H) if sinks else None, cap, keep, cut)
+
+
+@pytest.mark.parametrize("H,Kh,D,B,most,new,window,sinks,cap,keep,cut", [o for o in OPTIONS if o[5] > 1])
+def test_nan_that_later_tokens_see_however_a_step_is_cut(ops, H, Kh, D, B, most, new, window, sinks, cap, keep, cut):
+    """NaN among the values of a step's later tokens and of a window's oldest: in the sums of the rows that see them, and in no other's."""
+    tiles = -(-most // 64)
+    view, cpu = make_view(B * tiles, Kh, 64, D, B, tiles, seed=H + D + new)
+    seqs = a_step(B, most, new)
+    for slot, start, n in seqs:
+        places = [(start + n - 1, 0, D - 1), (start + n // 2, Kh - 1, 5)]
+        if window and start + 1 - window >= keep:
+            places.append((start + 1 - window, Kh - 1, 7))     # the first token's oldest key, which the second does not see
+        for pos, kvh, d in places:
+            for v in (view, cpu):
+                v.v.view(torch.uint8)[int(cpu.page_table[slot, pos // 64]), kvh, pos % 64, d] = 0x7f
+    q = rows_of(seqs, H * D, seed=8).view(-1, H, D)
+    meta, sink = make_meta(seqs), torch.linspace(-2.0, 3.0, H) if sinks else None
+    got = ops.attention(q.cuda(), meta, view, H, D ** -0.5, window, sinks=None if sink is None else sink.cuda(), softcap=cap, keep_first=keep)
+    parts = [v[5] for k, v in meta.extra.items() if k[0] == "attention8"][0]
+    assert cut == ("cluster" if parts > 0 else "dealt" if parts == 0 else "alone")
+    got, at = got.cpu().to(F64), 0
+    for slot, start, n in seqs:
+        for i in range(n):
+            # (a row at a time: the plain form multiplies what one of its rows sees with all rows' weights)
+            want, size = plain.attend(cpu, slot, start + i, q[at + i:at + i + 1], D ** -0.5, window, sink, cap, keep)
+            nan = want[0].isnan()
+            assert torch.equal(got[at + i].isnan(), nan), (slot, i)
+            off = (got[at + i] - want[0]).abs()[~nan]
+            assert torch.all(off <= (2.0 ** -8 * want[0].abs() + (2.0 ** -8 + 2.0 ** -14) * size[0])[~nan]), (slot, i)
+        at += n
+
+
+@pytest.mark.parametrize("page,D,seqs,window", [
+    (128, 128, [(0, 200, 1), (1, 30, 1)], 0), (128, 64, [(0, 600, 1), (1, 30, 1)], 64), (256, 128, [(0, 300, 4), (1, 130, 2)], 100),
+    (128, 128, [(0, 150, 40), (1, 260, 60)], 0), (128, 80, [(0, 200, 1), (1, 30, 1)], 0), (256, 80, [(0, 300, 3), (1, 130, 20)], 90),
+])
+def test_scales_of_blocks_that_no_row_sees_may_be_nan(ops, page, D, seqs, window):
+    """Behind a sequence's end, and before its window (where steps of many rows read whole pages, only pages before the window)."""
+    H, Kh, max_pages = 8, 2, -(-700 // page)
+    view, cpu = make_view(2 * max_pages, Kh, page, D, 2, max_pages, seed=page + D)
+    whole = max(n for _, _, n in seqs) * H // Kh > 64 or D == 80 and max(n for _, _, n in seqs) > 1
+    for slot, start, n in seqs:
+        first = max(0, start - window + 1) if window else 0
+        first -= first % (page if whole else 64)
+        for block in range(max_pages * page // 64):
+            if block * 64 >= start + n or block * 64 + 64 <= first:
+                p, b = int(cpu.page_table[slot, block * 64 // page]), block % (page // 64)
+                for v in (view, cpu):
+                    for s in v.scales:
+                        s[p, :, b] = math.nan
+    q = rows_of(seqs, H * D, seed=9).view(-1, H, D)
+    got, at = ops.attention(q.cuda(), make_meta(seqs), view, H, D ** -0.5, window).cpu().to(F64), 0
+    for s in cpu.scales:
+        s.nan_to_num_(0.0)                       # (the plain form multiplies them with weights of zero)
+    for slot, start, n in seqs:
+        want, size = plain.attend(cpu, slot, start, q[at:at + n], D ** -0.5, window)
+        assert torch.all((got[at:at + n] - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size), slot
+        at += n
