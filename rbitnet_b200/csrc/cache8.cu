@@ -122,11 +122,12 @@ __device__ __noinline__ void exact_codes(uint8_t* to, const __nv_bfloat16* head,
 }
 
 // The scale too is that of the exact rotation.  Both values of a pair are `amax` at most, so the exact largest value lies within 2 amax 0x1.8p-22
-// of it; where a border of scales, 448 * 2^e, lies in that range (of 500,000 blocks one), the pairs are turned in float64 and compared with it.
-// The border, or 0: float32 leaves no doubt (11 steps of amax's mantissa beside 1.75 are 0x1.8p-21 of it), or the old scale holds the
-// values either way.
+// of it, 11 steps of its mantissa beside a border of scales, 448 * 2^e = 1.75 * 2^(e + 8).  Where a border lies that near (of 500,000 blocks one),
+// the pairs are turned in float64 and compared with it, in functions of their own: a step's kernel runs once a layer, from instructions that
+// are fetched anew, and pays for those that it passes over too.
+__device__ __forceinline__ bool near_border(float amax) { return __builtin_expect((__float_as_uint(amax) - (0x600000u - 11) & 0x7fffffu) <= 22, 0); }
+// The border, or 0: the bounds of a scale, or an old one, leave no choice.
 __device__ __forceinline__ float open_border(float amax, float old) {
-  if ((__float_as_uint(amax) - (0x600000u - 11) & 0x7fffffu) > 22) return 0.f;
   const float lo = scale_for(amax * (1.f - 0x1.8p-21f)), hi = scale_for(amax * (1.f + 0x1.8p-21f));
   return lo < hi && old < hi ? 448.f * lo : 0.f;
 }
@@ -141,6 +142,15 @@ __device__ __noinline__ bool pieces_pass(const __nv_bfloat16* head, const float*
     passed |= fmaxf(fabsf(v.x), fabsf(v.y)) > border;        // (rounded to odd: above the border stays above it)
   }
   return passed;
+}
+// The scale of a token's key of head size D, by a warp.
+__device__ __noinline__ float exact_scale(float amax, float old, const __nv_bfloat16* head, const float* freq, int pos, int D, int interleaved) {
+  const float border = open_border(amax, old);
+  if (!(border > 0.f)) return scale_for(amax);
+  const int e = threadIdx.x & 31;
+  const bool passed = e < D / 16 && pieces_pass(head, freq + 8 * e, pos, border, interleaved ? 16 * e : 8 * e, interleaved ? 16 * e + 8 : D / 2 + 8 * e,
+                                                interleaved);
+  return scale_at_border(border, __any_sync(0xffffffffu, passed));
 }
 
 struct Append8 {
@@ -211,7 +221,7 @@ __global__ void __launch_bounds__(256) append8_kernel(Append8 p) {
       amax = fmaxf(amax, fmaxf(fabsf(ya), fabsf(yb)));
     }
     amax = rb_block_max(amax, scratch);          // (its barriers also make the rows visible)
-    const float old = before > 0 ? *scale : 0.f, border = stream == 0 && p.rot_dim > 0 ? open_border(amax, old) : 0.f;
+    const float old = before > 0 ? *scale : 0.f, border = stream == 0 && p.rot_dim > 0 && near_border(amax) ? open_border(amax, old) : 0.f;
     float needed = scale_for(amax);
     if (border > 0.f) {
       bool passed = false;
@@ -425,7 +435,7 @@ __global__ void __launch_bounds__(THREADS, THREADS * SPAN == 512 ? 2 : 1) append
 #pragma unroll
     for (int w = 1; w < THREADS / 32; ++w) amax = fmaxf(amax, tops[s][w]);
     float needed = scale_for(amax);
-    if (s == 0 && p.rot_dim) {
+    if (s == 0 && near_border(amax) && p.rot_dim) {
       const float border = open_border(amax, old[0]);
       if (border > 0.f) {
         bool passed = false;
@@ -512,13 +522,8 @@ __global__ void __launch_bounds__(256) append8_step_kernel(Append8 p) {
       const float big = largest8(a, b);
       const float top_k = rb_warp_max(is_k ? big : 0.f), top_v = rb_warp_max(is_v ? big : 0.f);
       float needed = scale_for(top_k);
-      if (p.rot_dim) {
-        const float border = open_border(top_k, old_k);
-        if (border > 0.f) {
-          const bool passed = is_k && pieces_pass(src + head * D, p.inv_freq + 8 * e, pos, border, piece_a(p, e), piece_b(p, e), p.interleaved);
-          needed = scale_at_border(border, __any_sync(0xffffffffu, passed));
-        }
-      }
+      if (__builtin_expect(near_border(top_k) && p.rot_dim, 0))
+        needed = exact_scale(top_k, old_k, src + (int64_t)(p.H + kvh) * D, p.inv_freq, pos, D, p.interleaved);
       const float now_k = fmaxf(old_k, needed), now_v = fmaxf(old_v, scale_for(top_v));
       uint8_t* k = (uint8_t*)p.cache.k + at;
       uint8_t* v = (uint8_t*)p.cache.v + at;
