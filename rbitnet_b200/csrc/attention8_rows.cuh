@@ -27,11 +27,11 @@
 // pair that several blocks have worked on is merged by a second kernel.  Where pairs are many and short a pair is one warp's work.
 //
 // Bounded by the cache's bytes where sequences are long: one B200, 64 sequences of up to 8,000 positions, 32 heads on 8 kv heads of 128:
-// 541 MB in 90 us, 6.0 TB/s (0.92 of a copy).  Short pairs are bound by what a pair costs to begin and to join (about 5 us in a block, two
-// blocks an SM) or, a pair a warp, by a warp's chain from score to sum, a microsecond for 32 keys: 24 sequences of 32 heads with a window of
-// 1,024, 202 MB in 45 us, 4.5 TB/s.  More rows add products and exponentials: 16
-// sequences of up to five tokens at up to 6,001 positions, 20 rows, 101 MB in 42 us.  One sequence at 2,048 positions: 8 us, waits.
-// Measured beside it (the first of these): 16-byte cp.async by every thread 154 us, of which the copies alone 136; boxes of 16 positions
+// 541 MB in 90 us within a captured graph and 96 called from Python, 6.0 and 5.7 TB/s (0.92 and 0.86 of a copy).  Short pairs are bound by what
+// a pair costs to begin and to join (about 5 us in a block, two blocks an SM) or, a pair a warp, by a warp's chain from score to sum, a
+// microsecond for 32 keys: 24 sequences of 32 heads with a window of 1,024, 202 MB in 43 us, 4.7 TB/s.  More rows add products and exponentials:
+// 16 sequences of up to five tokens at up to 6,001 positions, 20 rows, 101 MB in 41 us.  One sequence at 2,048 positions: 8 us, waits.
+// Measured beside an earlier form (the first of these, 91 us): 16-byte cp.async by every thread 154 us, of which the copies alone 136; boxes of 16 positions
 // 126 to 136; two stages and three blocks an SM 109; pairs dealt out without what their beginnings cost 113.
 #pragma once
 
@@ -219,7 +219,7 @@ template <int D, int NT> struct Sums {
 
 // The warp's way through a segment, whose first S::NS - 1 units have been asked for.
 // ONE: every row tile is a single token, so that its rows see the same keys (the code for a NaN that only some see,
-// though not run there, cost such steps 94 -> 101 us; without it 91 - 98).
+// though not run there, cost such steps 94 -> 101 us where tiles are dealt out; the other kernels were not tried without it).
 template <int D, int NT, int ALONE, bool ONE = false>
 __device__ __forceinline__ void run(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV, Job<D, NT, ALONE>& job, uint8_t* smem,
                                     uint8_t* stages, uint64_t* full, Ring& ring, Sums<D, NT>& sums) {
@@ -730,7 +730,8 @@ __global__ void __launch_bounds__(WARPS * 32) cluster_kernel(const __grid_consta
 }
 
 // Dealt out: all pairs' tiles of keys in the order (row tile, kv head, tile); a block takes `share` of them, one after the other.  To begin
-// and to end a pair costs as much as BEGIN tiles, which are dealt out with the others, ahead of the pair's own.
+// and to end a pair costs as much as BEGIN tiles (measured for one eight of rows of 128, taken for all), which are dealt out with the others,
+// ahead of the pair's own.
 // What a block leaves for a pair that it shares goes to place block + pair of the scratch: no two blocks' places are the same,
 // and those of one pair follow one another.
 constexpr int BEGIN = 10;
@@ -1056,7 +1057,8 @@ int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, int bl
   RB_CUDA(cudaLaunchKernelEx(&cfg, cluster_kernel<D, NT>, tk, tv, p));
   return 0;
 }
-// Whether a warp a pair is sooner done than tiles dealt out: microseconds of the two on one B200, from 128 to 1,728 pairs of 1 to 30 tiles.  A warp takes
+// Whether a warp a pair is sooner done than tiles dealt out: microseconds of the two on one B200, from 128 to 1,728 pairs of 1 to 30 tiles, heads
+// of 128 with one eight of rows (taken for 64 and for two eights too).  A warp takes
 // two units of 32 keys a tile, one a microsecond, eight warps an SM, or the bytes' time; dealt out a pair costs ten tiles beside its own.
 // (Pairs x tiles, alone and dealt out: 320 x 4 10, 13; 960 x 5 17, 32; 768 x 17 45, 49; 1,024 x 30 78, 88; but 200 x 8 19, 13; 400 x 16 39, 29.)
 inline bool alone_pays(long long pairs, int tiles, int D) {

@@ -559,8 +559,8 @@ __global__ void __launch_bounds__(256) cache8_values_kernel(__nv_bfloat16* k_out
   }
 }
 
-// The same for heads of a multiple of 16 values: a thread turns 16 codes at a time.  Bounded by its bytes: 128 pages of 8 heads of 128, 50 MB in
-// 13 us (a code at a time: 49).
+// The same for heads of a multiple of 16 values: a thread turns 16 codes at a time, two pieces of them on their way.  Bounded by the wait for
+// those: 128 pages of 8 heads of 128, 50 MB in 13 us, 3.8 TB/s (a code at a time: 49 us).
 __global__ void __launch_bounds__(256) cache8_values16_kernel(__nv_bfloat16* k_out, __nv_bfloat16* v_out, RbPagedLayer c, const float* k_scale,
                                                              const float* v_scale, const int* items, int block) {
   rb_pdl_launch_dependents();

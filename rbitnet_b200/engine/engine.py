@@ -69,7 +69,10 @@ class Engine:
         max_tokens: cache size in positions over all live sequences, each rounded up to
         whole pages (default: max_batch sequences of max_seq).
         cache_dtype: None (keys and values in the compute dtype), or "float8_e4m3": codes of 8 bits with a scale per block of
-        positions and kv head, half the bytes.  For the bfloat16 mode and layers of plain attention (``Mixer.cache_in_8_bits``)."""
+        positions and kv head, half the bytes.  For the bfloat16 mode and layers of plain attention (``Mixer.cache_in_8_bits``).
+        Made for heads of 64 and 128 values, at most 32 query heads a kv head: attention of single tokens is right for others too
+        but 10 to 130 times slower than over the 16-bit cache.  A step that brings more than 64 rows (tokens x query heads of a kv head) of any
+        sequence reads all of its sequences' keys and values through a bfloat16 copy, a layer at a time."""
         from ..kernels.ops import CudaOps
         self.config = config
         self.model_path = model_path
@@ -302,7 +305,10 @@ class Engine:
         called for every emitted token as soon as the host has it.
         ``draft_tokens`` > 0: a step checks up to so many tokens that followed the sequence's last ones where they stood before
         (``generate.Lookup``), and takes one of its own behind the accepted ones; the tokens are distributed as without it
-        (greedy: the same, up to rounding).  Needs sequences that can take a step back: no windows, no recurrent state."""
+        (greedy: the same, up to rounding).  Over a cache held in 8 bits that is so up to what its rounding moves: a draft that is not accepted
+        may leave its block of positions a larger scale, to which the kept tokens' smallest codes have been rounded.  Such steps are not captured,
+        whether they hold drafts or not, so they pay where text repeats.  Needs sequences that can take a step back: no windows, no recurrent
+        state."""
         loop = GenerationLoop(self._step_sample, self.cache, max_batch or self.max_batch,
                               decoder=self if self.use_graphs else None)
         stop = self.stop_ids if stop_ids is None else stop_ids
