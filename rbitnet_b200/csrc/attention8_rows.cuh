@@ -299,7 +299,8 @@ __device__ __forceinline__ void run(const Params& p, const CUtensorMap* tmK, con
       l[n][c] = 0.f;
       const int rc = n * 8 + 2 * t + c;
       if (p.a.sinks != nullptr && seg.first == 0 && seg.last > 0 && (ALONE || warp == 0) && rc < n_rows) {     // counted once: by the part with the first tile
-        m[n][c] = fminf(fmaxf(p.a.sinks[kvh * G + rc % G] * LOG2E, FLOOR), -FLOOR);
+        const float sink = p.a.sinks[kvh * G + rc % G] * LOG2E;
+        m[n][c] = sink != sink ? sink : fminf(fmaxf(sink, FLOOR), -FLOOR);
         l[n][c] = g == 0 ? 1.f : 0.f;
       }
     }

@@ -271,3 +271,25 @@ def test_scales_of_blocks_that_no_row_sees_may_be_nan(ops, page, D, seqs, window
         want, size = plain.attend(cpu, slot, start, q[at:at + n], D ** -0.5, window)
         assert torch.all((got[at:at + n] - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size), slot
         at += n
+
+
+@pytest.mark.parametrize("H,Kh,D,B,most,new,cut", CUTS + [(4, 2, 80, 2, 100, 1, None)])
+def test_sinks_that_are_no_numbers(ops, H, Kh, D, B, most, new, cut):
+    """Minus infinity is no sink at all; NaN makes its head's rows NaN, and no other's."""
+    tiles = -(-most // 64)
+    view, cpu = make_view(B * tiles, Kh, 64, D, B, tiles, seed=D)
+    seqs = a_step(B, most, new)
+    q = rows_of(seqs, H * D, seed=8).view(-1, H, D)
+    meta = make_meta(seqs)
+    sink = torch.linspace(-1.0, 1.0, H)
+    sink[1] = -math.inf
+    bare = torch.linspace(-1.0, 1.0, H)
+    bare[1] = -1e30
+    attend = lambda s: ops.attention(q.cuda(), meta, view, H, D ** -0.5, None, sinks=s.cuda()).view(-1, H, D)
+    want = attend(bare)
+    assert torch.equal(attend(sink), want) and torch.isfinite(want).all()
+    sink[2] = math.nan
+    got = attend(sink)
+    assert got[:, 2].isnan().all()
+    rest = [h for h in range(H) if h != 2]
+    assert torch.equal(got[:, rest], want[:, rest])
